@@ -241,6 +241,78 @@ int mg_attn_decode(mg_ctx *ctx, const uint16_t *q, const uint16_t *k_cache, cons
                    int64_t kv_heads, int64_t head_dim, int64_t cache_slots, int64_t q_pos, int64_t window,
                    double scaling, float *out);
 
+/* ---- The paged KV cache: one pool of pages for the keys and values of many
+ * requests. NO COUNTERPART in the reference, whose cache is the ring of one
+ * request. The pool is the ring's layout with num_pages * page_size slots,
+ * [num_pages, page_size, kv_heads, head_dim]; key j of a request lives in slot
+ * page_table[r, j / page_size] * page_size + j % page_size, page_size a power
+ * of two (at most 2^20). The pool holds the storage type, or Q8_0: int8 quants
+ * of the same shape and f16 scales [num_pages, page_size, kv_heads, head_dim /
+ * 32]. Page tables and lengths are int32, slots and positions int64; a table
+ * row holds max_pages pages (row stride ldt, 0 = max_pages) and must stand for
+ * fewer than 2^31 tokens.
+ *
+ * One step's page bookkeeping: every request r goes from old_lens[r] to
+ * new_lens[r] tokens. A growing one takes the pages it needs from the queue of
+ * free pages, a shrinking one (0: finished) gives its last ones back. The queue
+ * is free_ring [num_pages] with two counters in device memory: entries
+ * ends[0] .. ends[1] - 1, each at its value modulo num_pages. Pages are taken in
+ * request order from the front and given back behind the end, for the next
+ * call. ends_out (may be ends) receives the counters after the step, lens (may
+ * be old_lens or new_lens) the lengths after it. Table entries past a request's
+ * pages are left as they were.
+ *   slot_map, positions [tokens]: the step's new tokens, request by request:
+ *     token starts[r] + j is position old_lens[r] + j; entries behind the last
+ *     token are -1. starts [requests + 1] also holds the total last. Each of the
+ *     three may be NULL.
+ * A request is refused, and keeps its old length, when its tokens do not end
+ * within `tokens`, when new_lens[r] is more than its table row can hold, or when
+ * the pages of the requests up to and including it, refused ones too unless for
+ * the first two reasons, are more than the queue holds: its tokens' entries are
+ * -1. Negative lengths count as 0, old ones past the row's capacity as that. A
+ * table entry outside the pool gives slot -1. At most 4096 requests; everything
+ * stays on the device, so a decode loop can be captured. No tensor may overlap
+ * another but as said. */
+int mg_kv_pages(mg_ctx *ctx, int32_t *page_table, int64_t ldt, int64_t requests, int64_t max_pages,
+                const int32_t *old_lens, const int32_t *new_lens, int64_t page_size, int32_t *free_ring,
+                int64_t num_pages, const int64_t *ends, int32_t *lens, int64_t *ends_out, int32_t *starts,
+                int64_t *slot_map, int64_t *positions, int64_t tokens);
+
+/* mg_qk_norm_rope with the append through a slot map: q and k bit for bit as
+ * there (in place), k and v of token t in slot slot_map[t] of the pool of
+ * cache_slots = num_pages * page_size slots; a slot outside it appends nothing.
+ * positions [tokens] (device) picks the RoPE rows; a position outside the table
+ * leaves its token unrotated. dtype MG_BF16 or MG_F16. k_scale and v_scale NULL:
+ * the pool holds the rows at dtype, for any even head_dim up to 512. Else Q8_0
+ * by mg_quantize_q8_0's rule (a NaN becomes 0; a block whose amax passes
+ * 127 * 65504 gets an infinite scale, as there), for head_dim 64, 128 or 256 with
+ * all rows 16-byte aligned. Two tokens with one slot race. */
+int mg_qk_norm_rope_paged(mg_ctx *ctx, void *q, int64_t q_heads, int64_t ldq, void *k, int64_t k_heads, int64_t ldk,
+                          const void *v, int64_t ldv, int64_t tokens, int64_t head_dim, double eps, double qk_scale,
+                          const void *cos_t, const void *sin_t, int64_t table_rows, const int64_t *positions,
+                          const int64_t *slot_map, void *k_cache, void *v_cache, uint16_t *k_scale, uint16_t *v_scale,
+                          int64_t cache_slots, int dtype);
+
+/* Decode attention over the paged cache, one new token of each request:
+ * q [requests, q_heads, head_dim] (row stride ldq, 0 = q_heads*head_dim; after
+ * QK-norm, scale and RoPE); request r attends its keys max(0, lens[r] - window)
+ * (window > 0; else 0) .. lens[r] - 1, the new token's appended before the call;
+ * query head h reads kv head h / (q_heads / kv_heads). out [requests, q_heads,
+ * head_dim] (row stride ldo, 0 = q_heads*head_dim) = softmax(q.k * scaling) v at
+ * dtype_out, MG_F32 or dtype. dtype MG_BF16 or MG_F16 is q's and a 16-bit pool's;
+ * with k_scale and v_scale the pool is Q8_0, each k and v exactly q * d. lens
+ * counts below 0 as 0 and above the row's capacity as that. A request with no key
+ * gives zeros; a key whose page lies outside the pool is left out, as a masked
+ * one; what the pool holds behind a request's length or before its window is
+ * never used. head_dim 64 or 128; any number of query heads per kv head. A
+ * numerical envelope, not bits: f32 sums and weights to 2^-16 relative, keys split
+ * over work-groups and joined, the split depending on the batch's lengths. */
+int mg_attn_decode_paged(mg_ctx *ctx, const void *q, int64_t ldq, const void *k_cache, const void *v_cache,
+                         const uint16_t *k_scale, const uint16_t *v_scale, const int32_t *page_table, int64_t ldt,
+                         int64_t max_pages, const int32_t *lens, int64_t requests, int64_t q_heads, int64_t kv_heads,
+                         int64_t head_dim, int64_t page_size, int64_t num_pages, int64_t window, double scaling,
+                         void *out, int64_t ldo, int dtype, int dtype_out);
+
 /* Q8_0 quantizer, the step before dequant — up_w (src/gpu/gpu_engine.cpp:2722-2755,
  * llama.cpp's quantize_row_q8_0 rule): w bf16 bits [rows, in] (in % 32 == 0) ->
  * qs int8 [rows, in] and d f16 bits [rows, in/32]; per 32-block d = amax/127 in

@@ -8,6 +8,8 @@
 //   q        = rnd(q * qk_scale)      q only; qk_scale an f32 value outside f64
 //   q, k     = apply_rope(., table row pos)   when a table is given
 //   k_cache[pos % slots, g, :] = k,  v_cache[pos % slots, g, :] = v
+// or, for a paged cache, the same rows at slot slot_map[t], kept as they are or
+// as Q8_0 (32 elements to an f16 scale, the rule of k_quantize_q8_0).
 // Each step materializes at storage exactly as the separate primitives do, so
 // the result is bit-identical to running mg_rmsnorm_rows, mg_scale, mg_rope and
 // the two cache copies one after the other.
@@ -32,14 +34,42 @@ namespace mg
     constexpr int kQkWaveRows = 8; // head rows per wave (eight lanes per row for mean_sq)
     constexpr int kQkPieces = 1;   // k_qk_pairs: 8-element pieces per lane in each half of a row
 
+    // where a token's k and v go: the ring slot of its position, or slot_map's slot
+    // (one outside the cache: nowhere), as stored rows or as Q8_0
+    enum : int { kKvRing = 0, kKvSlots = 1, kKvSlotsQ8 = 2 };
+
     struct QkArgs
     {
         int64_t nq, nkv, ldq, ldk, ldv, T, table_rows, pos0, slots;
         int D;
         double eps;
+        const int64_t *slot_map;
+        uint16_t *kd, *vd; // Q8_0 scales
     };
 
-    template <class S, int VEC, bool C>
+    // eight elements of a head row as Q8_0, the four lanes of a quad holding a block's 32:
+    // d = amax / 127 in f32, stored as f16; q = round(x * (d ? 1 / d : 0)), halves away from zero
+    template <class S>
+    MG_DEV void st_q8(const Vec<typename S::raw, 8> &v, int8_t *qs, uint16_t *d, int64_t at)
+    {
+        float x[8], amax = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            x[e] = S::dec(v.v[e]);
+            amax = __builtin_fmaxf(amax, __builtin_fabsf(x[e]));
+        }
+        amax = __builtin_fmaxf(amax, dpp_mov<0xB1, 0xf>(amax, amax)); // quad_perm [1,0,3,2]
+        amax = __builtin_fmaxf(amax, dpp_mov<0x4E, 0xf>(amax, amax)); // quad_perm [2,3,0,1]
+        const float dd = amax / 127.0f;
+        const float id = dd != 0.0f ? 1.0f / dd : 0.0f;
+        uint64_t q = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q |= uint64_t(uint8_t(int8_t(int(__builtin_roundf(x[e] * id))))) << (8 * e);
+        *reinterpret_cast<uint64_t *>(qs + at) = q;
+        if (at % 32 == 0) d[at / 32] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(dd));
+    }
+
+    template <class S, int VEC, bool C, int KV>
     __global__ __launch_bounds__(256) void k_qk_norm_rope(typename S::raw *q, typename S::raw *k,
                                                           const typename S::raw *__restrict__ v, QkArgs a,
                                                           typename S::comp qs,
@@ -76,7 +106,12 @@ namespace mg
             vptr[w0 + lane] = isq || !v ? nullptr : v + t * a.ldv + (hh - a.nq) * D;
             rpos[w0 + lane] = p;
             risq[w0 + lane] = isq;
-            rcache[w0 + lane] = !isq && kc && p >= 0 ? (p % a.slots) * (a.nkv * D) + (hh - a.nq) * D : -1;
+            if constexpr (KV == kKvRing) {
+                rcache[w0 + lane] = !isq && kc && p >= 0 ? (p % a.slots) * (a.nkv * D) + (hh - a.nq) * D : -1;
+            } else {
+                const int64_t sl = a.slot_map[t];
+                rcache[w0 + lane] = !isq && sl >= 0 && sl < a.slots ? sl * (a.nkv * D) + (hh - a.nq) * D : -1;
+            }
         }
         wave_lds_sync();
 
@@ -238,7 +273,7 @@ namespace mg
     // the row's lanes gives mean_sq's bits. A wave with a row outside that
     // bound (or holding inf or NaN) stages its rows in LDS and runs mean_sq's
     // own order (eight interleaved accumulators, fixed tree).
-    template <class S, int D, int NV>
+    template <class S, int D, int NV, int KV>
     __global__ __launch_bounds__(256) void k_qk_pairs(typename S::raw *q, typename S::raw *k,
                                                       const typename S::raw *__restrict__ v, QkArgs a,
                                                       typename S::comp qs,
@@ -275,8 +310,16 @@ namespace mg
             hi[i] = ldv<raw, VEC>(x + half + c0 + VEC * i);
         }
         const int64_t p = pos ? pos[t] : a.pos0 + t;
+        // the row's slot, or -1 where it appends nothing
+        int64_t slot = -1;
+        if constexpr (KV == kKvRing) {
+            if (!isq && kc && p >= 0) slot = p < a.slots ? p : p % a.slots;
+        } else if (!isq) {
+            slot = a.slot_map[t];
+            slot = slot < a.slots ? slot : -1;
+        }
         Vec<raw, VEC> vlo[NV], vhi[NV];
-        if (!isq && vc && p >= 0) {
+        if (vc && slot >= 0) {
             const raw *vr = v + t * a.ldv + int64_t(hh - a.nq) * D + c0;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
@@ -426,9 +469,17 @@ namespace mg
             stv<raw, VEC>(x + c0 + VEC * i, lo[i]);
             stv<raw, VEC>(x + half + c0 + VEC * i, hi[i]);
         }
-        if (!isq && kc && p >= 0) {
-            const int64_t slot = p < a.slots ? p : p % a.slots;
+        if (slot >= 0) {
             const int64_t o = slot * (a.nkv * D) + int64_t(hh - a.nq) * D + c0;
+            if constexpr (KV == kKvSlotsQ8) {
+                static_assert(NV == 1 && TPR >= 4, "a quad holds a block of 32");
+                int8_t *kq = reinterpret_cast<int8_t *>(kc), *vq = reinterpret_cast<int8_t *>(vc);
+                st_q8<S>(lo[0], kq, a.kd, o);
+                st_q8<S>(hi[0], kq, a.kd, o + half);
+                st_q8<S>(vlo[0], vq, a.vd, o);
+                st_q8<S>(vhi[0], vq, a.vd, o + half);
+                return;
+            }
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 stv<raw, VEC>(kc + o + VEC * i, lo[i]);
@@ -441,7 +492,7 @@ namespace mg
         }
     }
 
-    template <class S, bool C = false>
+    template <class S, bool C = false, int KV = kKvRing>
     void launch_qk_t(mg_ctx *c, void *q, void *k, const void *v, const QkArgs &a, double qk_scale, const void *co,
                      const void *si, const int64_t *pos, void *kc, void *vc)
     {
@@ -474,20 +525,24 @@ namespace mg
                                        static_cast<raw *>(kc), static_cast<raw *>(vc));
                 };
                 if (a.D == 64)
-                    gp(k_qk_pairs<S, 64, kQkPieces>);
+                    gp(k_qk_pairs<S, 64, kQkPieces, KV>);
                 else if (a.D == 128)
-                    gp(k_qk_pairs<S, 128, kQkPieces>);
+                    gp(k_qk_pairs<S, 128, kQkPieces, KV>);
                 else
-                    gp(k_qk_pairs<S, 256, kQkPieces>);
+                    gp(k_qk_pairs<S, 256, kQkPieces, KV>);
                 check_launch("k_qk_pairs");
                 return;
             }
         }
-        if (vec)
-            go(k_qk_norm_rope<S, V16, C>);
-        else
-            go(k_qk_norm_rope<S, 1, C>);
-        check_launch("k_qk_norm_rope");
+        if constexpr (KV == kKvSlotsQ8) {
+            fail("qk_norm_rope_paged: Q8_0 pages need head_dim 64, 128 or 256 and 16-byte aligned rows");
+        } else {
+            if (vec)
+                go(k_qk_norm_rope<S, V16, C, KV>);
+            else
+                go(k_qk_norm_rope<S, 1, C, KV>);
+            check_launch("k_qk_norm_rope");
+        }
     }
 
     void launch_qk_norm_rope(mg_ctx *c, void *q, int64_t nq, int64_t ldq, void *k, int64_t nkv, int64_t ldk,
@@ -509,7 +564,8 @@ namespace mg
         need(ldq >= nq * D && ldk >= nkv * D && (v == nullptr || ldv >= nkv * D),
              "qk_norm_rope: token stride smaller than heads*head_dim");
         if (T == 0 || nq + nkv == 0) return;
-        QkArgs a{nq, nkv, ldq, ldk, ldv, T, table_rows, pos0, slots > 0 ? slots : 1, int(D), eps};
+        QkArgs a{nq,      nkv, ldq, ldk, ldv, T, table_rows, pos0, slots > 0 ? slots : 1, int(D), eps, nullptr,
+                 nullptr, nullptr};
         switch (dt) {
         case BF16: launch_qk_t<SBf16>(c, q, k, v, a, qk_scale, co, si, pos, kc, vc); break;
         case F16: launch_qk_t<SF16>(c, q, k, v, a, qk_scale, co, si, pos, kc, vc); break;
@@ -518,5 +574,34 @@ namespace mg
         case F64 | kF32Compat: launch_qk_t<SF64, true>(c, q, k, v, a, qk_scale, co, si, pos, kc, vc); break;
         default: fail("qk_norm_rope: unknown dtype " + std::to_string(dt));
         }
+    }
+
+    void launch_qk_norm_rope_paged(mg_ctx *c, void *q, int64_t nq, int64_t ldq, void *k, int64_t nkv, int64_t ldk,
+                                   const void *v, int64_t ldv, int64_t T, int64_t D, double eps, double qk_scale,
+                                   const void *co, const void *si, int64_t table_rows, const int64_t *pos,
+                                   const int64_t *slot_map, void *kc, void *vc, uint16_t *kd, uint16_t *vd,
+                                   int64_t slots, int dt)
+    {
+        need(D > 0 && D % 2 == 0 && D <= 512, "qk_norm_rope_paged: head_dim must be even and <= 512");
+        need(T >= 0 && nq >= 0 && nkv > 0, "qk_norm_rope_paged: bad shape");
+        if (T == 0) return;
+        need((q || nq == 0) && k && v && kc && vc && slot_map && pos, "qk_norm_rope_paged: NULL tensor");
+        need((co == nullptr) == (si == nullptr), "qk_norm_rope_paged: give both cos and sin, or neither");
+        need(co == nullptr || table_rows > 0, "qk_norm_rope_paged: empty rope table");
+        need((kd == nullptr) == (vd == nullptr), "qk_norm_rope_paged: give both k_scale and v_scale, or neither");
+        need(slots > 0, "qk_norm_rope_paged: empty cache");
+        need(dt == BF16 || dt == F16, "qk_norm_rope_paged: dtype must be bf16 or f16");
+        if (ldq == 0) ldq = nq * D;
+        if (ldk == 0) ldk = nkv * D;
+        if (ldv == 0) ldv = nkv * D;
+        need(ldq >= nq * D && ldk >= nkv * D && ldv >= nkv * D,
+             "qk_norm_rope_paged: token stride smaller than heads*head_dim");
+        const QkArgs a{nq, nkv, ldq, ldk, ldv, T, table_rows, 0, slots, int(D), eps, slot_map, kd, vd};
+        if (dt == BF16)
+            kd ? launch_qk_t<SBf16, false, kKvSlotsQ8>(c, q, k, v, a, qk_scale, co, si, pos, kc, vc)
+               : launch_qk_t<SBf16, false, kKvSlots>(c, q, k, v, a, qk_scale, co, si, pos, kc, vc);
+        else
+            kd ? launch_qk_t<SF16, false, kKvSlotsQ8>(c, q, k, v, a, qk_scale, co, si, pos, kc, vc)
+               : launch_qk_t<SF16, false, kKvSlots>(c, q, k, v, a, qk_scale, co, si, pos, kc, vc);
     }
 } // namespace mg

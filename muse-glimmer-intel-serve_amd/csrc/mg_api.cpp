@@ -416,4 +416,44 @@ int mg_attn_decode(mg_ctx *ctx, const uint16_t *q, const uint16_t *k_cache, cons
     });
 }
 
+int mg_kv_pages(mg_ctx *ctx, int32_t *page_table, int64_t ldt, int64_t requests, int64_t max_pages,
+                const int32_t *old_lens, const int32_t *new_lens, int64_t page_size, int32_t *free_ring,
+                int64_t num_pages, const int64_t *ends, int32_t *lens, int64_t *ends_out, int32_t *starts,
+                int64_t *slot_map, int64_t *positions, int64_t tokens)
+{
+    MG_GUARD(-1, {
+        mg::launch_kv_pages(ctx_of(ctx), page_table, ldt, requests, max_pages, old_lens, new_lens, page_size, free_ring,
+                            num_pages, ends, lens, ends_out, starts, slot_map, positions, tokens);
+        return 0;
+    });
+}
+
+int mg_qk_norm_rope_paged(mg_ctx *ctx, void *q, int64_t q_heads, int64_t ldq, void *k, int64_t k_heads, int64_t ldk,
+                          const void *v, int64_t ldv, int64_t tokens, int64_t head_dim, double eps, double qk_scale,
+                          const void *cos_t, const void *sin_t, int64_t table_rows, const int64_t *positions,
+                          const int64_t *slot_map, void *k_cache, void *v_cache, uint16_t *k_scale, uint16_t *v_scale,
+                          int64_t cache_slots, int dtype)
+{
+    MG_GUARD(-1, {
+        mg::launch_qk_norm_rope_paged(ctx_of(ctx), q, q_heads, ldq, k, k_heads, ldk, v, ldv, tokens, head_dim, eps,
+                                      qk_scale, cos_t, sin_t, table_rows, positions, slot_map, k_cache, v_cache,
+                                      k_scale, v_scale, cache_slots, dtype);
+        return 0;
+    });
+}
+
+int mg_attn_decode_paged(mg_ctx *ctx, const void *q, int64_t ldq, const void *k_cache, const void *v_cache,
+                         const uint16_t *k_scale, const uint16_t *v_scale, const int32_t *page_table, int64_t ldt,
+                         int64_t max_pages, const int32_t *lens, int64_t requests, int64_t q_heads, int64_t kv_heads,
+                         int64_t head_dim, int64_t page_size, int64_t num_pages, int64_t window, double scaling,
+                         void *out, int64_t ldo, int dtype, int dtype_out)
+{
+    MG_GUARD(-1, {
+        mg::launch_attn_decode_paged(ctx_of(ctx), q, ldq, k_cache, v_cache, k_scale, v_scale, page_table, ldt,
+                                     max_pages, lens, requests, q_heads, kv_heads, head_dim, page_size, num_pages,
+                                     window, scaling, out, ldo, dtype, dtype_out);
+        return 0;
+    });
+}
+
 } // extern "C"

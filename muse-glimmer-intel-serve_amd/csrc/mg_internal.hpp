@@ -49,6 +49,14 @@ namespace mg
         if (!ok) fail(m);
     }
 
+    // log2 of a KV page's tokens: a power of two, so that a position's page and place are a shift and a mask
+    inline int page_shift(int64_t page_size, const char *who)
+    {
+        need(page_size > 0 && page_size <= (int64_t(1) << 20) && (page_size & (page_size - 1)) == 0,
+             std::string(who) + ": page_size must be a power of two of at most 2^20 (got " + std::to_string(page_size) + ")");
+        return __builtin_ctzll(static_cast<unsigned long long>(page_size));
+    }
+
     // lookup tables, built at mg_open (k_elementwise.hip)
     void build_luts(mg_ctx *c);
 
@@ -107,6 +115,21 @@ namespace mg
     void launch_attn_decode(mg_ctx *c, const uint16_t *q, const uint16_t *kc, const uint16_t *vc, int64_t nq,
                             int64_t nkv, int64_t D, int64_t slots, int64_t qpos, int64_t window, double scaling,
                             float *out);
+    // the paged KV cache: k_pages.hip (tables and maps), k_qk.hip (append), k_attn_paged.hip (decode attention)
+    void launch_kv_pages(mg_ctx *c, int32_t *table, int64_t ldt, int64_t requests, int64_t max_pages,
+                         const int32_t *old_lens, const int32_t *new_lens, int64_t page_size, int32_t *ring,
+                         int64_t num_pages, const int64_t *ends, int32_t *lens, int64_t *ends_out, int32_t *starts,
+                         int64_t *slots, int64_t *pos, int64_t tokens);
+    void launch_qk_norm_rope_paged(mg_ctx *c, void *q, int64_t nq, int64_t ldq, void *k, int64_t nkv, int64_t ldk,
+                                   const void *v, int64_t ldv, int64_t T, int64_t D, double eps, double qk_scale,
+                                   const void *co, const void *si, int64_t table_rows, const int64_t *pos,
+                                   const int64_t *slot_map, void *kc, void *vc, uint16_t *kd, uint16_t *vd,
+                                   int64_t slots, int dt);
+    void launch_attn_decode_paged(mg_ctx *c, const void *q, int64_t ldq, const void *kc, const void *vc,
+                                  const uint16_t *kd, const uint16_t *vd, const int32_t *table, int64_t ldt,
+                                  int64_t max_pages, const int32_t *lens, int64_t seqs, int64_t nq, int64_t nkv,
+                                  int64_t D, int64_t page_size, int64_t num_pages, int64_t window, double scaling,
+                                  void *out, int64_t ldo, int dt, int dt_out);
     void launch_vocab(mg_ctx *c, const void *logits, int64_t ld, int64_t rows, int64_t V, int dt_in, int64_t K,
                       double *lse, int64_t *amax, int64_t *top_idx, float *top_val, bool tail_on, double mult,
                       double cap, void *logits_out);

@@ -62,6 +62,11 @@ _SIGS = {
     "mg_gemv_q8_0": ([_P, _P, _P, _P, _I, _I, _I, _I, _P, _I, _INT], _INT),
     "mg_attn_decode": ([_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _D, _P], _INT),
     "mg_attn_prefill": ([_P, _P, _I, _P, _P, _I, _I, _I, _I, _I, _I, _I, _D, _P, _I], _INT),
+    "mg_kv_pages": ([_P, _P, _I, _I, _I, _P, _P, _I, _P, _I, _P, _P, _P, _P, _P, _P, _I], _INT),
+    "mg_qk_norm_rope_paged": ([_P, _P, _I, _I, _P, _I, _I, _P, _I, _I, _I, _D, _D, _P, _P, _I, _P, _P, _P, _P, _P, _P,
+                               _I, _INT], _INT),
+    "mg_attn_decode_paged": ([_P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _D, _P, _I, _INT,
+                              _INT], _INT),
     "mg_sample_dist": ([_P, _P, _P, _P, _P, _I, _I, _D, _D, _D, _P, _P, _P], _INT),
     "mg_sample_rows": ([_P, _P, _I, _I, _I, _P, _I, _D, _D, _D, _P, _P, _P], _INT),
     "mg_vocab_reduce_tail": ([_P, _P, _I, _I, _I, _INT, _D, _D, _I, _P, _P, _P, _P, _P], _INT),
@@ -381,6 +386,123 @@ class Prims:
         self._numel("attn_decode out", out, hq * D)
         self._check(self.lib.mg_attn_decode(self.h, _ptr(q), _ptr(k_cache), _ptr(v_cache), hq, hk, D, slots, q_pos,
                                             window, scaling, _ptr(out)))
+        return out
+
+    # ------------------------------------------------------ paged KV cache
+    @staticmethod
+    def _ints(name, dtype, n, *ts):
+        """contiguous integer tensors of n elements (None: skipped)"""
+        for t in ts:
+            if t is not None and (t.dtype != dtype or t.numel() != n or not t.is_contiguous()):
+                raise MgError(f"{name}: expected a contiguous {dtype} tensor of {n}, got {t.dtype} {tuple(t.shape)}")
+
+    def _page_table(self, name, t, requests):
+        import torch
+        if t.dim() != 2 or t.dtype != torch.int32 or t.shape[0] != requests:
+            raise MgError(f"{name}: page_table must be int32 [{requests}, max_pages], got {t.dtype} {tuple(t.shape)}")
+        if t.stride(1) != 1 and t.shape[1] > 1 or requests > 1 and t.stride(0) < t.shape[1]:
+            raise MgError(f"{name}: page_table rows must have unit inner stride and not overlap")
+        return t.stride(0) if requests > 1 else t.shape[1]
+
+    def _token_rows(self, name, t):
+        """_heads for 16-bit or f32 rows whose tokens do not overlap; returns the token stride"""
+        import torch
+        if t.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+            raise MgError(f"{name}: dtype {t.dtype} is not taken")
+        ld = self._heads(name, t)
+        if t.shape[0] > 1 and ld < t.shape[1] * t.shape[2]:
+            raise MgError(f"{name}: rows of consecutive tokens overlap")
+        return ld if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+    def _pool(self, name, k_cache, v_cache, k_scale, v_scale, dtype, heads, dim):
+        """checks a pool [num_pages, page_size, Hk, D] at dtype, or int8 with f16 scales [.., D / 32]"""
+        import torch
+        if k_cache.dim() != 4 or tuple(k_cache.shape[2:]) != (heads, dim):
+            raise MgError(f"{name}: caches must be [num_pages, page_size, {heads}, {dim}], got {tuple(k_cache.shape)}")
+        self._same(name, k_cache, v_cache, "shape")
+        self._contig(name, k_cache, v_cache, k_scale, v_scale)
+        if (k_scale is None) != (v_scale is None):
+            raise MgError(f"{name}: give both k_scale and v_scale, or neither")
+        want = dtype if k_scale is None else torch.int8
+        if k_cache.dtype != want or v_cache.dtype != want:
+            raise MgError(f"{name}: caches of {k_cache.dtype} and {v_cache.dtype}, {want} needed")
+        if k_scale is not None:
+            shape = (*k_cache.shape[:3], dim // 32)
+            for t in (k_scale, v_scale):
+                if t.dtype != torch.float16 or tuple(t.shape) != shape:
+                    raise MgError(f"{name}: scales must be float16 {shape}, got {t.dtype} {tuple(t.shape)}")
+
+    def kv_pages(self, page_table, old_lens, new_lens, page_size, free_ring, ends, lens, ends_out, starts=None,
+                 slot_map=None, positions=None):
+        """One step's page bookkeeping of a paged KV cache (mg_kv_pages): requests go from old_lens to
+        new_lens [R] int32 tokens, taking pages from the queue of free pages and giving them back to it
+        (free_ring [num_pages] int32 with counters ends [2] int64: entries ends[0] .. ends[1] - 1, each
+        modulo num_pages); page_table [R, W] int32 is updated in place. Writes lens [R] (may be old_lens
+        or new_lens), ends_out [2] (may be ends), starts [R + 1] int32, and slot_map and positions
+        [tokens] int64 of the step's new tokens, -1 behind the last and for refused requests."""
+        import torch
+        R = old_lens.numel()
+        T = 0 if slot_map is None else slot_map.numel()
+        if slot_map is None and positions is not None:
+            T = positions.numel()
+        self._dev(page_table, old_lens, new_lens, free_ring, ends, lens, ends_out, starts, slot_map, positions)
+        ldt = self._page_table("kv_pages", page_table, R)
+        self._ints("kv_pages", torch.int32, R, old_lens, new_lens, lens)
+        self._ints("kv_pages", torch.int32, R + 1, starts)
+        self._ints("kv_pages", torch.int32, free_ring.numel(), free_ring)
+        self._ints("kv_pages", torch.int64, 2, ends, ends_out)
+        self._ints("kv_pages", torch.int64, T, slot_map, positions)
+        self._check(self.lib.mg_kv_pages(self.h, _ptr(page_table), ldt, R, page_table.shape[1], _ptr(old_lens),
+                                         _ptr(new_lens), page_size, _ptr(free_ring), free_ring.numel(), _ptr(ends),
+                                         _ptr(lens), _ptr(ends_out), _ptr(starts), _ptr(slot_map), _ptr(positions), T))
+
+    def qk_norm_rope_paged(self, q, k, v, eps, qk_scale, cos, sin, positions, slot_map, k_cache, v_cache,
+                           k_scale=None, v_scale=None):
+        """qk_norm_rope with the append through a slot map (mg_qk_norm_rope_paged): k and v of token t go
+        to slot slot_map[t] of the pool k_cache / v_cache [num_pages, page_size, Hk, D] (a slot outside it:
+        nowhere), at q's dtype or, with k_scale / v_scale [num_pages, page_size, Hk, D / 32] f16, as int8
+        Q8_0. positions [T] pick the rows of cos / sin (None: no rotation)."""
+        import torch
+        name = "qk_norm_rope_paged"
+        self._dev(q, k, v, k_cache, v_cache, k_scale, v_scale, slot_map, positions)
+        ldq, ldk, ldv = (self._token_rows(name, t) for t in (q, k, v))
+        T, qh, D = q.shape
+        kh = k.shape[1]
+        for t in (k, v):
+            self._same(name, q, t)
+            if tuple(t.shape) != (T, kh, D):
+                raise MgError(f"{name}: k and v must be [{T}, {kh}, {D}], got {tuple(t.shape)}")
+        self._ints(name, torch.int64, T, positions, slot_map)
+        self._table(name, q, cos, sin, positions)
+        self._pool(name, k_cache, v_cache, k_scale, v_scale, q.dtype, kh, D)
+        self._check(self.lib.mg_qk_norm_rope_paged(
+            self.h, _ptr(q), qh, ldq, _ptr(k), kh, ldk, _ptr(v), ldv, T, D, eps, qk_scale, _ptr(cos), _ptr(sin),
+            cos.shape[0] if cos is not None else 0, _ptr(positions), _ptr(slot_map), _ptr(k_cache), _ptr(v_cache),
+            _ptr(k_scale), _ptr(v_scale), k_cache.shape[0] * k_cache.shape[1], _dtype_code(q)))
+
+    def attn_decode_paged(self, q, k_cache, v_cache, page_table, lens, scaling, window=0, k_scale=None, v_scale=None,
+                          out=None):
+        """One new token's attention for each of R requests over a paged KV cache (mg_attn_decode_paged):
+        q [R, Hq, D] bf16 or f16; pool [num_pages, page_size, Hk, D] at q's dtype, or int8 Q8_0 with scales
+        [.., D / 32] f16; page_table [R, W] int32, lens [R] int32 keys of each (the new token's among them)
+        -> out [R, Hq, D], float32 (default) or q's dtype. A request without keys gives zeros."""
+        import torch
+        name = "attn_decode_paged"
+        ldq = self._token_rows(name, q)
+        R, hq, D = q.shape
+        if out is None:
+            out = torch.empty((R, hq, D), dtype=torch.float32, device=q.device)
+        self._dev(q, k_cache, v_cache, k_scale, v_scale, page_table, lens, out)
+        ldo = self._token_rows(name, out)
+        self._same(name, q, out, "shape")
+        self._pool(name, k_cache, v_cache, k_scale, v_scale, q.dtype, k_cache.shape[2] if k_cache.dim() == 4 else 0, D)
+        ldt = self._page_table(name, page_table, R)
+        self._ints(name, torch.int32, R, lens)
+        num_pages, page_size, hk, _ = k_cache.shape
+        self._check(self.lib.mg_attn_decode_paged(
+            self.h, _ptr(q), ldq, _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(page_table), ldt,
+            page_table.shape[1], _ptr(lens), R, hq, hk, D, page_size, num_pages, window, scaling, _ptr(out), ldo,
+            _dtype_code(q), _dtype_code(out)))
         return out
 
     # ------------------------------------------------------------ softmax
