@@ -250,7 +250,7 @@ int mg_attn_decode(mg_ctx *ctx, const uint16_t *q, const uint16_t *k_cache, cons
  * of the same shape and f16 scales [num_pages, page_size, kv_heads, head_dim /
  * 32]. Page tables and lengths are int32, slots and positions int64; a table
  * row holds max_pages pages (row stride ldt, 0 = max_pages) and must stand for
- * fewer than 2^31 tokens.
+ * at most 2^30 tokens.
  *
  * One step's page bookkeeping: every request r goes from old_lens[r] to
  * new_lens[r] tokens. A growing one takes the pages it needs from the queue of
@@ -304,8 +304,8 @@ int mg_qk_norm_rope_paged(mg_ctx *ctx, void *q, int64_t q_heads, int64_t ldq, vo
  * counts below 0 as 0 and above the row's capacity as that. A request with no key
  * gives zeros; a key whose page lies outside the pool is left out, as a masked
  * one; what the pool holds behind a request's length or before its window is
- * never used. head_dim 64 or 128; any number of query heads per kv head. A
- * numerical envelope, not bits: f32 sums and weights to 2^-16 relative, keys split
+ * never used. head_dim 64 or 128; any number of query heads per kv head; at most
+ * 65535 requests and 2^31 - 1 slots in the pool. A numerical envelope, not bits: f32 sums and weights to 2^-16 relative, keys split
  * over work-groups and joined, the split depending on the batch's lengths. */
 int mg_attn_decode_paged(mg_ctx *ctx, const void *q, int64_t ldq, const void *k_cache, const void *v_cache,
                          const uint16_t *k_scale, const uint16_t *v_scale, const int32_t *page_table, int64_t ldt,

@@ -8,8 +8,36 @@
 //   s_j = (q_bh . k_j) * scaling,   out_bh = sum_j softmax(s)_j v_j.
 // A request without keys gives zeros. A key whose page is outside the pool is
 // left out, as a masked one. Q8_0 pages hold k_j and v_j as q * d, exactly.
+//
+// Division of the work (mg_paged_plan.hpp): the requests' keys form one line of
+// 128-key units, cut into equal runs; a team of work-groups, one for every KV
+// head (and for every 16 query heads of a larger group), walks a run, so the
+// heads of one key, neighbours in memory, are read at about the same time.
+// Lengths stay on the device: each work-group sums them itself. A request that
+// lies in one run is finished there; the others' partial results (maximum, sum,
+// unnormalized output) are joined by a second kernel.
+//
+// A work-group's four waves take 32-key steps of the run in turn, with no
+// barrier until the request ends. Per step, as in the ring's decode kernel:
+// whole rows are loaded in 16-byte pieces one step ahead and written to LDS;
+// S^T = K Q^T and O += P V run on the matrix cores (16 query heads of the
+// group, zero-padded, as columns), the weights entering as a high and a low
+// 16-bit part, so each is within 2^-16 of p relative. Online softmax in f32 on
+// scores scaled by log2(e).
+//   Pages: lane l holds the slot of key l of the step (its table entry was
+// requested a step before); a load instruction covers 4 to 16 rows, which lie
+// in one page where the page is that large, so one readlane gives their base;
+// else, or where a key is masked, each row's slot comes by a shuffle. The mask
+// is one bit a key, and rows of masked keys are never loaded: what they hold
+// (NaN too) cannot reach the sums.
+//   f16: weights are kept at 2^12 p, so that the low part of a weight down to
+// 2^-26 of the largest is a normal number; sum and output carry the factor.
+//   Q8_0: quants become bf16 (exact: 8 bits) on their way to LDS; a K block's
+// scale multiplies its 32-dim part of the score, a V block's its weights, so no
+// value is rounded to 16 bits. f16 queries enter as a high and a low bf16 part.
 #include "mg_device.hpp"
 #include "mg_internal.hpp"
+#include "mg_paged_plan.hpp"
 
 namespace mg
 {
@@ -19,77 +47,475 @@ namespace mg
         const uint16_t *kd, *vd;
         const int32_t *table, *lens;
         void *out;
-        int64_t ldq, ldt, ldo, window, num_pages;
-        int nq, nkv, W, sh;
-        float scale;
+        float *part;     // [2 teams, vh, hw, D] outputs, then [2 teams, vh, hw] maxima and sums
+        int64_t *first;  // [requests + 1] first unit of each request, and their number
+        int64_t ldq, ldt, ldo, window;
+        int R, nkv, W, sh, num_pages;
+        int hpg, hw, vh; // query heads a kv head, a work-group; work-groups a team
+        int teams;
+        float scale2;    // scaling * log2(e)
     };
 
-    // first and one past the last key of request b
-    MG_DEV void key_range(const PagedArgs &a, int b, int &lo, int &n)
+    typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+    MG_DEV f32x4 mfma_f16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+    // the 16-bit storage types as matrix operands
+    template <class S>
+    struct Mm;
+    template <>
+    struct Mm<SBf16>
     {
-        n = min(max(a.lens[b], 0), a.W << a.sh);
-        lo = a.window > 0 && n > a.window ? int(n - a.window) : 0;
+        using e = __bf16;
+        using x8 = bf16x8;
+        static constexpr float up = 0.0f; // log2 of the weights' factor
+        static MG_DEV f32x4 mma(x8 a, x8 b, f32x4 c) { return mfma_bf16(a, b, c); }
+    };
+    template <>
+    struct Mm<SF16>
+    {
+        using e = _Float16;
+        using x8 = f16x8;
+        static constexpr float up = 12.0f;
+        static MG_DEV f32x4 mma(x8 a, x8 b, f32x4 c) { return mfma_f16(a, b, c); }
+    };
+
+    template <class X8>
+    MG_DEV X8 ld_x8(const uint16_t *p)
+    {
+        return __builtin_bit_cast(X8, *reinterpret_cast<const Vec<uint32_t, 4> *>(p));
+    }
+    // two weights' high and low parts at positions e, e + 1 of an operand
+    template <class M>
+    MG_DEV void split_weights(float p0, float p1, typename M::x8 &hi, typename M::x8 &lo, int e)
+    {
+        const typename M::e h0 = typename M::e(p0), h1 = typename M::e(p1);
+        hi[e] = h0;
+        hi[e + 1] = h1;
+        lo[e] = typename M::e(p0 - float(h0));
+        lo[e + 1] = typename M::e(p1 - float(h1));
     }
 
-    // one work-group per (request, query head): a tile of 256 keys, one a thread, then the
-    // tile's weights over the values, a thread per dim
-    template <class S, class SO, bool Q8>
-    __global__ __launch_bounds__(256) void k_attn_paged(PagedArgs a, int D)
+    // 16 quants as bf16, exactly
+    MG_DEV void q8_bf16(const Vec<uint32_t, 4> &x, uint16_t *dst)
     {
-        using raw = typename S::raw;
-        __shared__ float qf[128], p[256], red[4];
-        __shared__ int64_t sl[256];
-        const int b = blockIdx.x, h = blockIdx.y, g = h / (a.nq / a.nkv), tid = threadIdx.x;
-        int lo, n;
-        key_range(a, b, lo, n);
-        if (tid < D) qf[tid] = S::dec(static_cast<const raw *>(a.q)[b * a.ldq + h * D + tid]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            Vec<uint32_t, 4> w;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t u = x.v[2 * h + i];
+                w.v[2 * i] = bf_pack(float(int8_t(u)), float(int8_t(u >> 8)));
+                w.v[2 * i + 1] = bf_pack(float(int8_t(u >> 16)), float(int32_t(u) >> 24));
+            }
+            *reinterpret_cast<Vec<uint32_t, 4> *>(dst + 8 * h) = w;
+        }
+    }
+
+    // the work-group's run [u0, u1) of its team, the request it starts in and that
+    // request's unit; `keep`: this work-group writes the requests' first units down
+    struct Run
+    {
+        int64_t u0, u1;
+        int b, at;
+    };
+    MG_DEV Run find_run(const PagedArgs &a, int team, bool keep)
+    {
+        __shared__ int64_t red[4];
+        __shared__ Run found;
+        const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+        const int per = (a.R + 255) / 256, b0 = tid * per, b1 = min(b0 + per, a.R);
+        const int cap = a.W << a.sh;
+        int64_t mine = 0;
+        for (int b = b0; b < b1; ++b) mine += paged_span(a.lens[b], cap, a.window).units;
+        int64_t pre = mine;
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            const int64_t u = __shfl_up(pre, m, 64);
+            pre += lane >= m ? u : 0;
+        }
+        if (lane == 63) red[wv] = pre;
         __syncthreads();
-        float m = -__builtin_huge_valf(), l = 0.0f, o = 0.0f;
-        auto val = [&](const void *c, const uint16_t *d, int64_t i) {
-            if constexpr (Q8)
-                return float(static_cast<const int8_t *>(c)[i]) * f16_f32(d[i / 32]);
-            else
-                return S::dec(static_cast<const raw *>(c)[i]);
-        };
-        for (int j0 = lo; j0 < n; j0 += 256) {
-            const int j = j0 + tid;
-            float s = -__builtin_huge_valf();
-            int64_t at = -1;
-            if (j < n) {
-                const int page = a.table[b * a.ldt + (j >> a.sh)];
-                if (page >= 0 && page < a.num_pages) {
-                    at = (((int64_t(page) << a.sh) + (j & ((1 << a.sh) - 1))) * a.nkv + g) * D;
-                    float dot = 0.0f;
-                    for (int i = 0; i < D; ++i) dot = __builtin_fmaf(qf[i], val(a.kc, a.kd, at + i), dot);
-                    s = dot * a.scale;
+        for (int w = 0; w < wv; ++w) pre += red[w];
+        const int64_t total = red[0] + red[1] + red[2] + red[3];
+        const int64_t teams = a.teams < total ? a.teams : total;
+        int64_t p = pre - mine; // the thread's first unit
+        if (keep) {
+            int64_t f = p;
+            for (int b = b0; b < b1; ++b) {
+                a.first[b] = f;
+                f += paged_span(a.lens[b], cap, a.window).units;
+            }
+            if (tid == 0) a.first[a.R] = total;
+        }
+        if (team >= teams) return Run{0, 0, 0, 0};
+        const int64_t u0 = team_first(team, total, teams), u1 = team_first(team + 1, total, teams);
+        if (u0 >= p && u0 < pre) {
+            int b = b0;
+            for (;; ++b) {
+                const int u = paged_span(a.lens[b], cap, a.window).units;
+                if (u0 < p + u) break;
+                p += u;
+            }
+            found = Run{u0, u1, b, int(u0 - p)};
+        }
+        __syncthreads();
+        return found;
+    }
+
+    template <class S, class SO, bool Q8, int KB> // KB = head_dim / 32
+    __global__ __launch_bounds__(256) void k_attn_paged(PagedArgs a)
+    {
+        constexpr int D = 32 * KB, NT = 2 * KB;   // NT output tiles of 16 dims
+        constexpr int EPL = Q8 ? 16 : 8;          // elements a lane loads at once
+        constexpr int LPR = D / EPL;              // lanes a row
+        constexpr int RPI = 64 / LPR;             // rows a load instruction covers
+        constexpr int NLD = kPagedStep / RPI;     // load instructions a step
+        constexpr int SK = D + 8, SV = D + 16;    // LDS row strides (elements): conflict-free reads
+        constexpr int SO4 = D + 4;                // row stride of a wave's output in LDS (floats)
+        constexpr int WB = 32 * (SK + SV) * 2;    // LDS bytes of a wave's K and V
+        static_assert(16 * SO4 * 4 <= WB, "a wave's output takes the place of its K and V");
+        using M = Mm<std::conditional_t<Q8, SBf16, S>>;
+        using x8 = typename M::x8;
+        using raw = typename SO::raw;
+        constexpr int NQ = Q8 && S::dt == F16 ? 2 : 1; // parts of a query
+        constexpr float kLow = -__builtin_huge_valf();
+        __shared__ __align__(16) char lds[4][WB];
+        __shared__ __align__(16) float scl[Q8 ? 4 : 1][2][32][KB];
+        __shared__ float wm[4][16], wl[4][16];
+        const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63;
+        const int team = blockIdx.x / a.vh, v = blockIdx.x - team * a.vh;
+        const Run run = find_run(a, team, blockIdx.x == 0);
+        if (run.u0 >= run.u1) return; // the whole work-group
+        const int nsub = a.hpg / a.hw, g = v / nsub;
+        const int h0 = g * a.hpg + (v - g * nsub) * a.hw;
+        const int n = lane & 15, c = lane >> 4;
+        uint16_t *sk = reinterpret_cast<uint16_t *>(lds[wv]), *sv = sk + 32 * SK;
+        const int pc = lane % LPR, pr = lane / LPR;
+        const int64_t rowb = int64_t(a.nkv) * D * (Q8 ? 1 : 2); // bytes between slots
+        const char *kg = static_cast<const char *>(a.kc) + int64_t(g) * D * (Q8 ? 1 : 2);
+        const char *vg = static_cast<const char *>(a.vc) + int64_t(g) * D * (Q8 ? 1 : 2);
+        const int cap = a.W << a.sh, psm = (1 << a.sh) - 1;
+
+        int64_t left = run.u1 - run.u0;
+        int at = run.at;
+        for (int b = run.b; left > 0; ++b, at = 0) {
+            const PagedSpan sp = paged_span(a.lens[b], cap, a.window);
+            const int end = sp.units - at < left ? sp.units : at + int(left);
+            left -= end - at;
+            const int k0 = sp.base + at * kPagedUnit;                  // first key of the part
+            const int klo = k0 > sp.lo ? k0 : sp.lo;                   // attended keys [klo, khi)
+            const int64_t ke = int64_t(sp.base) + int64_t(end) * kPagedUnit;
+            const int khi = ke < sp.n ? int(ke) : sp.n;
+            const int32_t *tab = a.table + b * a.ldt;
+
+            // B of S^T: lane (head n, c) holds q[n][32 kb + 8c ..], zero for padding heads
+            x8 qop[NQ][KB];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                const uint16_t *qp =
+                    static_cast<const uint16_t *>(a.q) + b * a.ldq + int64_t(h0 + n) * D + 32 * kb + 8 * c;
+                if constexpr (NQ == 1) {
+                    qop[0][kb] = n < a.hw ? ld_x8<x8>(qp) : x8{};
+                } else {
+                    const f16x8 x = n < a.hw ? ld_x8<f16x8>(qp) : f16x8{};
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2)
+                        split_weights<M>(float(x[e]), float(x[e + 1]), qop[0][kb], qop[1][kb], e);
                 }
             }
-            float mt = dpp_max(s);
-            if ((tid & 63) == 0) red[tid >> 6] = mt;
-            __syncthreads();
-            mt = __builtin_fmaxf(__builtin_fmaxf(red[0], red[1]), __builtin_fmaxf(red[2], red[3]));
-            const float mn = __builtin_fmaxf(m, mt);
-            const float ref = mn == -__builtin_huge_valf() ? 0.0f : mn;
-            const float w = at < 0 ? 0.0f : exp_f32(s - ref);
-            p[tid] = w;
-            sl[tid] = at;
-            __syncthreads();
-            const float corr = exp_f32(m - ref);
-            l *= corr;
-            o *= corr;
-            m = mn;
-            for (int i = 0; i < 256; ++i) {
-                const int64_t ai = sl[i];
-                if (ai < 0) continue;
-                l += p[i];
-                if (tid < D) o = __builtin_fmaf(p[i], val(a.vc, a.vd, ai + tid), o);
+            // the slot of key kb + lane % 32, or -1
+            auto slot_of = [&](int kb) {
+                const int key = kb + (lane & 31);
+                if (key < klo || key >= khi) return -1;
+                const int page = tab[key >> a.sh];
+                return page >= 0 && page < a.num_pages ? (page << a.sh) + (key & psm) : -1;
+            };
+            Vec<uint32_t, 4> stk[NLD], stv[NLD];
+            Vec<uint16_t, KB> sts; // scales of key lane % 32: K's in the lower half of the wave, V's in the upper
+            auto stage = [&](int slot, uint32_t seen) {
+                if constexpr (Q8) {
+                    sts = Vec<uint16_t, KB>{};
+                    const uint16_t *sc = lane < 32 ? a.kd : a.vd;
+                    if (slot >= 0)
+                        sts = *reinterpret_cast<const Vec<uint16_t, KB> *>(sc + (int64_t(slot) * a.nkv + g) * KB);
+                }
+                if (seen == 0xffffffffu && psm + 1 >= RPI) {
+#pragma unroll
+                    for (int i = 0; i < NLD; ++i) {
+                        const int64_t s0 = __builtin_amdgcn_readlane(slot, RPI * i);
+                        const int64_t o = s0 * rowb + int64_t(pr) * rowb + 16 * pc;
+                        stk[i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(kg + o));
+                        stv[i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(vg + o));
+                    }
+                    return;
+                }
+#pragma unroll
+                for (int i = 0; i < NLD; ++i) {
+                    const int s = __shfl(slot, pr + RPI * i, 64);
+                    stk[i] = Vec<uint32_t, 4>{{0u, 0u, 0u, 0u}};
+                    stv[i] = stk[i];
+                    if (s >= 0) {
+                        const int64_t o = s * rowb + 16 * pc;
+                        stk[i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(kg + o));
+                        stv[i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(vg + o));
+                    }
+                }
+            };
+
+            f32x4 o[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            float m = kLow, l = 0.0f; // head n (replicated over c)
+            int kb = k0 + kPagedStep * wv;
+            int slot = slot_of(kb);
+            uint32_t seen = uint32_t(__builtin_amdgcn_ballot_w64(slot >= 0)), seen1 = 0;
+            if (kb < khi) stage(slot, seen);
+            slot = slot_of(kb + kPagedUnit);
+            for (; kb < khi; kb += kPagedUnit) {
+#pragma unroll
+                for (int i = 0; i < NLD; ++i) {
+                    const int key = pr + RPI * i;
+                    if constexpr (Q8) {
+                        q8_bf16(stk[i], sk + key * SK + 16 * pc);
+                        q8_bf16(stv[i], sv + key * SV + 16 * pc);
+                    } else {
+                        *reinterpret_cast<Vec<uint32_t, 4> *>(sk + key * SK + 8 * pc) = stk[i];
+                        *reinterpret_cast<Vec<uint32_t, 4> *>(sv + key * SV + 8 * pc) = stv[i];
+                    }
+                }
+                if constexpr (Q8) {
+                    Vec<float, KB> f;
+#pragma unroll
+                    for (int i = 0; i < KB; ++i) f.v[i] = f16_f32(sts.v[i]);
+                    *reinterpret_cast<Vec<float, KB> *>(scl[wv][lane >> 5][lane & 31]) = f;
+                }
+                wave_lds_sync();
+                // K as A of S^T: lane (key n, c) holds dims 32 kb + 8c.. of key 16 t + n
+                x8 kt[2][KB];
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < KB; ++i) kt[t][i] = ld_x8<x8>(sk + (16 * t + n) * SK + 32 * i + 8 * c);
+                // the next step's rows and the table entries of the one behind it are requested now
+                if (kb + kPagedUnit < khi) {
+                    seen1 = uint32_t(__builtin_amdgcn_ballot_w64(slot >= 0));
+                    stage(slot, seen1);
+                    slot = slot_of(kb + 2 * kPagedUnit);
+                }
+                // scores of keys 16 t + 4c + r for head n
+                float sc[2][4], mx = kLow;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    f32x4 st = {0.0f, 0.0f, 0.0f, 0.0f};
+                    if constexpr (Q8) {
+                        f32x4 part[KB];
+#pragma unroll
+                        for (int i = 0; i < KB; ++i) {
+                            part[i] = M::mma(kt[t][i], qop[0][i], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                            if constexpr (NQ == 2) part[i] = M::mma(kt[t][i], qop[1][i], part[i]);
+                        }
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const Vec<float, KB> d =
+                                *reinterpret_cast<const Vec<float, KB> *>(scl[wv][0][16 * t + 4 * c + r]);
+#pragma unroll
+                            for (int i = 0; i < KB; ++i) st[r] = __builtin_fmaf(d.v[i], part[i][r], st[r]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < KB; ++i) st = M::mma(kt[t][i], qop[0][i], st);
+                    }
+                    const uint32_t bits = seen >> (16 * t + 4 * c);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        sc[t][r] = st[r] * a.scale2;
+                        sc[t][r] = (bits >> r & 1) != 0 ? sc[t][r] : kLow;
+                        mx = __builtin_fmaxf(mx, sc[t][r]);
+                    }
+                }
+                mx = rows4_max(mx);
+                const float mn = __builtin_fmaxf(m, mx);
+                // no score above -inf yet: a zero reference, so that -inf scores weigh 0
+                // and only NaN ones reach the sum
+                const float mref = mn == kLow ? 0.0f : mn;
+                // weights: element 4t + r of lane (head n, c) is key 16 t + 4c + r
+                float p[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(sc[e >> 2][e & 3] - (mref - M::up));
+                if (__builtin_amdgcn_ballot_w64(mn != m) != 0) {
+                    // some head's running max moved: rescale its sum and its O row
+                    // (rows are heads 4c + r; their factors come from lanes 4c + r)
+                    const float corr = __builtin_amdgcn_exp2f(m - mref); // first step: 2^-inf = 0
+                    l *= corr;
+                    float cr[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) cr[r] = __shfl(corr, 4 * c + r, 64);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[t][r] *= cr[r];
+                }
+                m = mn;
+                l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                // V as B of P V: lane (dim n, c) needs keys 4c + r and 16 + 4c + r
+                // of dim 16 s + n, through the transposing read
+                const uint16_t *vr = sv + (4 * c + (n >> 2)) * SV + 4 * (n & 3);
+                x8 phi, plo;
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    if constexpr (Q8) {
+                        if (t % 2 == 0)
+#pragma unroll
+                            for (int e = 0; e < 8; e += 2) {
+                                const int key = 16 * (e >> 2) + 4 * c + (e & 3);
+                                split_weights<M>(p[e] * scl[wv][1][key][t / 2], p[e + 1] * scl[wv][1][key + 1][t / 2],
+                                                 phi, plo, e);
+                            }
+                    } else if (t == 0) {
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2) split_weights<M>(p[e], p[e + 1], phi, plo, e);
+                    }
+                    const bf16x4 v0 = lds_read_tr(vr + 16 * t);
+                    const bf16x4 v1 = lds_read_tr(vr + 16 * SV + 16 * t);
+                    const x8 vb =
+                        __builtin_bit_cast(x8, bf16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
+                    o[t] = M::mma(phi, vb, o[t]);
+                    o[t] = M::mma(plo, vb, o[t]);
+                }
+                seen = seen1;
+                wave_lds_sync(); // this step's reads are done before the next step's writes
             }
+
+            // join the four waves: their outputs take the place of K and V in LDS
+            l = rows4_sum(l);
+            float *so = reinterpret_cast<float *>(lds[wv]);
+            if (c == 0) {
+                wm[wv][n] = m;
+                wl[wv][n] = l;
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) so[(4 * c + r) * SO4 + 16 * t + n] = o[t][r];
             __syncthreads();
+            const int hh = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (D / 16);
+            if (hh < a.hw) {
+                const float top = __builtin_fmaxf(__builtin_fmaxf(wm[0][hh], wm[1][hh]), __builtin_fmaxf(wm[2][hh], wm[3][hh]));
+                const float ref = top == kLow ? 0.0f : top;
+                float sum = 0.0f, acc[D / 16];
+#pragma unroll
+                for (int e = 0; e < D / 16; ++e) acc[e] = 0.0f;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const float f = __builtin_amdgcn_exp2f(wm[w][hh] - ref);
+                    sum = __builtin_fmaf(f, wl[w][hh], sum);
+                    const float *src = reinterpret_cast<const float *>(lds[w]) + hh * SO4 + d0;
+#pragma unroll
+                    for (int e = 0; e < D / 16; e += 4) {
+                        const Vec<float, 4> x = *reinterpret_cast<const Vec<float, 4> *>(src + e);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc[e + i] = __builtin_fmaf(f, x.v[i], acc[e + i]);
+                    }
+                }
+                if (at == 0 && end == sp.units) {
+                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    raw *dst = static_cast<raw *>(a.out) + b * a.ldo + int64_t(h0 + hh) * D + d0;
+#pragma unroll
+                    for (int e = 0; e < D / 16; ++e) dst[e] = SO::enc32(acc[e] * inv);
+                } else {
+                    const int64_t pl = 2 * int64_t(team) + (b == run.b ? 0 : 1);
+                    const int64_t row = (pl * a.vh + v) * a.hw + hh;
+                    float *dst = a.part + row * D + d0;
+#pragma unroll
+                    for (int e = 0; e < D / 16; e += 4)
+                        *reinterpret_cast<Vec<float, 4> *>(dst + e) = Vec<float, 4>{{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]}};
+                    if (d0 == 0) {
+                        float *ml = a.part + 2 * int64_t(a.teams) * a.vh * a.hw * D + 2 * row;
+                        ml[0] = top;
+                        ml[1] = sum;
+                    }
+                }
+            }
+            __syncthreads(); // the next request's first step writes where the outputs were
         }
-        if (tid < D) {
-            const float r = l == 0.0f ? 0.0f : o / l;
-            static_cast<typename SO::raw *>(a.out)[b * a.ldo + h * D + tid] = SO::enc32(r);
+    }
+
+    // Joins the partial results of the requests that a team's edge cuts: top = max m_s,
+    // out = sum_s 2^(m_s - top) acc_s / sum_s 2^(m_s - top) l_s over the request's teams.
+    // A work-group takes 4 E of the outputs of one (request, work-group of heads), E
+    // threads wide, 256 / E threads over the teams. blockIdx.x is the request, or, where
+    // there are fewer edges than requests, the edge: its request's first one joins.
+    template <class SO, int E>
+    __global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a, int D, int by_edge)
+    {
+        constexpr int SG = 256 / E;
+        __shared__ float tops[SG][E], sums[SG][E];
+        __shared__ Vec<float, 4> accs[SG][E];
+        const int64_t total = a.first[a.R];
+        const int64_t teams = a.teams < total ? a.teams : total;
+        int b = blockIdx.x;
+        if (by_edge) {
+            const int64_t t = int64_t(blockIdx.x) + 1; // the edge between teams t - 1 and t
+            if (t >= teams) return;
+            const int64_t u = team_first(t, total, teams);
+            int lo = 0, hi = a.R; // the request that holds unit u
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) >> 1;
+                if (a.first[mid] <= u)
+                    lo = mid;
+                else
+                    hi = mid;
+            }
+            b = lo;
+            if (team_of(a.first[b], total, teams) != t - 1) return;
         }
+        const int64_t p0 = a.first[b], p1 = a.first[b + 1];
+        const int64_t t0 = team_of(p0, total, teams);
+        const int nt = int(team_of(p1 - 1, total, teams) - t0) + 1;
+        if (nt == 1) return; // finished in its team
+        const int v = blockIdx.y;
+        const int e = threadIdx.x % E, sg = threadIdx.x / E;
+        const int i0 = (int(blockIdx.z) * E + e) * 4; // the thread's outputs among [hw, D]
+        const bool live = i0 < a.hw * D;
+        const int hh = live ? i0 / D : 0;
+        const float *ml = a.part + 2 * int64_t(a.teams) * a.vh * a.hw * D;
+        auto row = [&](int s) { return (team_place(t0 + s, p0, total, teams) * a.vh + v) * a.hw; };
+        // (a work-group's outputs may be of several heads: each thread goes by its own)
+        float top = -__builtin_huge_valf();
+        for (int s = sg; s < nt; s += SG) top = __builtin_fmaxf(top, ml[2 * (row(s) + hh)]);
+        tops[sg][e] = top;
+        __syncthreads();
+#pragma unroll
+        for (int s = 0; s < SG; ++s) top = __builtin_fmaxf(top, tops[s][e]);
+        const float ref = top == -__builtin_huge_valf() ? 0.0f : top;
+        float sum = 0.0f;
+        Vec<float, 4> acc{{0.0f, 0.0f, 0.0f, 0.0f}};
+        for (int s = sg; s < nt; s += SG) {
+            const int64_t r = row(s);
+            const float f = __builtin_amdgcn_exp2f(ml[2 * (r + hh)] - ref);
+            sum = __builtin_fmaf(f, ml[2 * (r + hh) + 1], sum);
+            if (live) {
+                const Vec<float, 4> x = *reinterpret_cast<const Vec<float, 4> *>(a.part + r * D + i0);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc.v[i] = __builtin_fmaf(f, x.v[i], acc.v[i]);
+            }
+        }
+        sums[sg][e] = sum;
+        accs[sg][e] = acc;
+        __syncthreads();
+        if (sg != 0 || !live) return;
+#pragma unroll
+        for (int s = 1; s < SG; ++s) {
+            sum += sums[s][e];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc.v[i] += accs[s][e].v[i];
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int nsub = a.hpg / a.hw, g = v / nsub;
+        const int h = g * a.hpg + (v - g * nsub) * a.hw + hh;
+        typename SO::raw *dst = static_cast<typename SO::raw *>(a.out) + b * a.ldo + int64_t(h) * D + (i0 - hh * D);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) dst[i] = SO::enc32(acc.v[i] * inv);
     }
 
     void launch_attn_decode_paged(mg_ctx *c, const void *q, int64_t ldq, const void *kc, const void *vc,
@@ -105,10 +531,9 @@ namespace mg
         need(D == 64 || D == 128, "attn_decode_paged: head_dim must be 64 or 128");
         need(dt == BF16 || dt == F16, "attn_decode_paged: dtype must be bf16 or f16");
         need(dt_out == dt || dt_out == F32, "attn_decode_paged: dtype_out must be f32 or q's dtype");
-        need(max_pages > 0 && num_pages > 0 && num_pages < (int64_t(1) << 31), "attn_decode_paged: bad table or pool size");
-        need(max_pages <= ((int64_t(1) << 31) - 1) >> sh, "attn_decode_paged: a row's tokens must be below 2^31");
-        if (seqs == 0) return;
-        need(q && kc && vc && table && lens && out, "attn_decode_paged: NULL tensor");
+        need(max_pages > 0 && num_pages > 0, "attn_decode_paged: bad table or pool size");
+        need(num_pages <= ((int64_t(1) << 31) - 1) >> sh, "attn_decode_paged: a pool must have fewer than 2^31 slots");
+        need(max_pages <= (int64_t(1) << 30) >> sh, "attn_decode_paged: a table row must stand for at most 2^30 tokens");
         need((kd == nullptr) == (vd == nullptr), "attn_decode_paged: give both k_scale and v_scale, or neither");
         if (ldq == 0) ldq = nq * D;
         if (ldo == 0) ldo = nq * D;
@@ -116,20 +541,63 @@ namespace mg
         need(ldq >= nq * D && ldo >= nq * D && ldt >= max_pages, "attn_decode_paged: row stride smaller than a row");
         need(aligned16(q) && aligned16(kc) && aligned16(vc) && ldq % 8 == 0,
              "attn_decode_paged: q rows and caches must be 16-byte aligned");
-        need(seqs < (int64_t(1) << 31), "attn_decode_paged: too many requests");
-        const PagedArgs a{q,   kc,  vc,     kd,        vd,      table,    lens,           out, ldq,
-                          ldt, ldo, window, num_pages, int(nq), int(nkv), int(max_pages), sh,  float(scaling)};
+        need(reinterpret_cast<uintptr_t>(kd) % 8 == 0 && reinterpret_cast<uintptr_t>(vd) % 8 == 0,
+             "attn_decode_paged: scales must be 8-byte aligned");
+        need(seqs <= 65535, "attn_decode_paged: at most 65535 requests");
+        if (seqs == 0) return;
+        need(q && kc && vc && table && lens && out, "attn_decode_paged: NULL tensor");
+        // a wave serves up to 16 query heads (the matrix cores' 16 columns); larger
+        // groups split over work-groups of the largest divisor <= 16
+        const int64_t hpg = nq / nkv;
+        int64_t hw = hpg;
+        while (hw > 16 || hpg % hw != 0) --hw;
+        const int64_t vh = nkv * (hpg / hw);
+        // as many teams as fill the chip twice (two work-groups fit a CU's LDS), not more
+        // than there can be units, nor than the workspace has room for
+        const int64_t span = window > 0 && window < max_pages << sh ? window + kPagedStep : max_pages << sh;
+        const int64_t most = seqs * (span / kPagedUnit + 1);
+        int64_t teams = 2 * int64_t(c->num_cus) / vh;
+        teams = teams < most ? teams : most;
+        const int64_t fbytes = (seqs + 1) * int64_t(sizeof(int64_t));
+        const int64_t tbytes = 2 * vh * hw * (D + 2) * int64_t(sizeof(float));
+        need(fbytes <= c->work_bytes, "attn_decode_paged: the requests' sums exceed the context workspace");
+        // (from a 16-byte boundary behind the sums)
+        const int64_t room = (c->work_bytes - (fbytes + 15) / 16 * 16) / tbytes;
+        teams = teams < room ? teams : room;
+        teams = teams > 1 ? teams : 1;
+        PagedArgs a{};
+        a.q = q, a.kc = kc, a.vc = vc, a.kd = kd, a.vd = vd, a.table = table, a.lens = lens, a.out = out;
+        a.first = static_cast<int64_t *>(c->work);
+        a.part = reinterpret_cast<float *>(static_cast<char *>(c->work) + (fbytes + 15) / 16 * 16);
+        a.ldq = ldq, a.ldt = ldt, a.ldo = ldo, a.window = window;
+        a.R = int(seqs), a.nkv = int(nkv), a.W = int(max_pages), a.sh = sh, a.num_pages = int(num_pages);
+        a.hpg = int(hpg), a.hw = int(hw), a.vh = int(vh), a.teams = int(teams);
+        a.scale2 = float(double(float(scaling)) * 1.4426950408889634);
         auto go = [&](auto kern) {
-            hipLaunchKernelGGL(kern, dim3(unsigned(seqs), unsigned(nq)), dim3(256), 0, c->stream, a, int(D));
+            hipLaunchKernelGGL(kern, dim3(unsigned(teams * vh)), dim3(256), 0, c->stream, a);
             check_launch("k_attn_paged");
         };
-        auto typed = [&](auto s) {
+        auto sized = [&](auto s, auto so) {
             using S = decltype(s);
-            if (dt_out == F32)
-                kd ? go(k_attn_paged<S, SF32, true>) : go(k_attn_paged<S, SF32, false>);
+            using SO = decltype(so);
+            if (kd)
+                D == 128 ? go(k_attn_paged<S, SO, true, 4>) : go(k_attn_paged<S, SO, true, 2>);
             else
-                kd ? go(k_attn_paged<S, S, true>) : go(k_attn_paged<S, S, false>);
+                D == 128 ? go(k_attn_paged<S, SO, false, 4>) : go(k_attn_paged<S, SO, false, 2>);
+            if (teams == 1) return; // nothing is cut
+            const bool by_edge = teams - 1 < seqs;
+            const int64_t who = by_edge ? teams - 1 : seqs;
+            auto join = [&](auto kern, int e) {
+                const dim3 grid{unsigned(who), unsigned(vh), unsigned((hw * D + 4 * e - 1) / (4 * e))};
+                hipLaunchKernelGGL(kern, grid, dim3(256), 0, c->stream, a, int(D), int(by_edge));
+                check_launch("k_attn_paged_join");
+            };
+            // few requests over many teams: threads over the teams; else over the outputs
+            teams / who >= 16 ? join(k_attn_paged_join<SO, 16>, 16) : join(k_attn_paged_join<SO, 64>, 64);
         };
-        dt == BF16 ? typed(SBf16{}) : typed(SF16{});
+        if (dt_out == F32)
+            dt == BF16 ? sized(SBf16{}, SF32{}) : sized(SF16{}, SF32{});
+        else
+            dt == BF16 ? sized(SBf16{}, SBf16{}) : sized(SF16{}, SF16{});
     }
 } // namespace mg

@@ -84,7 +84,7 @@ namespace mg
 
     MG_DEV void lens_of(const PagesArgs &a, int i, int &o, int &n)
     {
-        // capacity W << sh is below 2^31 (checked on the host)
+        // capacity W << sh is at most 2^30 (checked on the host)
         o = min(max(a.old_lens[i], 0), a.W << a.sh);
         n = max(a.new_lens[i], 0);
     }
@@ -198,7 +198,7 @@ namespace mg
         need(requests >= 0 && requests <= kPagesMax,
              "kv_pages: at most " + std::to_string(kPagesMax) + " requests (got " + std::to_string(requests) + ")");
         need(max_pages > 0 && num_pages > 0 && num_pages < (int64_t(1) << 31), "kv_pages: bad table or pool size");
-        need(max_pages <= ((int64_t(1) << 31) - 1) >> sh, "kv_pages: a row's tokens must be below 2^31");
+        need(max_pages <= (int64_t(1) << 30) >> sh, "kv_pages: a table row must stand for at most 2^30 tokens");
         need(requests * max_pages < (int64_t(1) << 31), "kv_pages: a table must have fewer than 2^31 pages");
         need(tokens >= 0 && tokens < (int64_t(1) << 31) - 1, "kv_pages: bad token count");
         need(requests == 0 || (table && old_lens && new_lens && lens), "kv_pages: NULL tensor");

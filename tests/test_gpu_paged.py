@@ -168,7 +168,7 @@ def test_pages_errors(prims):
     l = i32(np.zeros(4097))
     with pytest.raises(Exception, match="4096 requests"):
         prims.kv_pages(**args(page_table=many, old_lens=l, new_lens=l, lens=l))
-    with pytest.raises(Exception, match="2\\^31"):
+    with pytest.raises(Exception, match="2\\^30"):
         prims.kv_pages(**args(page_table=i32(np.zeros((2, 2048))), page_size=1 << 20))
 
 
