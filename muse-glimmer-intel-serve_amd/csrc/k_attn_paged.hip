@@ -10,16 +10,19 @@
 // left out, as a masked one. Q8_0 pages hold k_j and v_j as q * d, exactly.
 //
 // Division of the work (mg_paged_plan.hpp): the requests' keys form one line of
-// 128-key units, cut into equal runs; a team of work-groups, one for every KV
-// head (and for every 16 query heads of a larger group), walks a run, so the
-// heads of one key, neighbours in memory, are read at about the same time.
-// Lengths stay on the device: each work-group sums them itself. A request that
-// lies in one run is finished there; the others' partial results (maximum, sum,
-// unnormalized output) are joined by a second kernel.
+// units, cut into equal runs; a team of work-groups, one for every KV head (and
+// for every 16 query heads of a larger group), walks a run, so the heads of one
+// key, neighbours in memory, are read at about the same time. Lengths stay on
+// the device: each work-group sums them itself. A request that lies in one run
+// is finished there; the others leave partial results (maximum, sum,
+// unnormalized output), which a second kernel joins in team order. (Joined by the
+// last of a request's own work-groups instead, behind device-wide fences, a call
+// took 19 to 52 us longer: a fence writes back an XCD's whole L2.)
 //
-// A work-group's four waves take 32-key steps of the run in turn, with no
-// barrier until the request ends. Per step, as in the ring's decode kernel:
-// whole rows are loaded in 16-byte pieces one step ahead and written to LDS;
+// A work-group's four waves take steps of the run in turn, 32 keys (Q8_0: two
+// halves of 32), with no barrier until the request ends. Per step, as in the
+// ring's decode kernel: whole rows are loaded in 16-byte pieces one step ahead,
+// across the end of a request, and written to LDS;
 // S^T = K Q^T and O += P V run on the matrix cores (16 query heads of the
 // group, zero-padded, as columns), the weights entering as a high and a low
 // 16-bit part, so each is within 2^-16 of p relative. Online softmax in f32 on
@@ -34,7 +37,7 @@
 // 2^-26 of the largest is a normal number; sum and output carry the factor.
 //   Q8_0: quants become bf16 (exact: 8 bits) on their way to LDS; a K block's
 // scale multiplies its 32-dim part of the score, a V block's its weights, so no
-// value is rounded to 16 bits. f16 queries enter as a high and a low bf16 part.
+// value is rounded to 16 bits; the weights get their parts then. f16 queries enter as a high and a low bf16 part.
 #include "mg_device.hpp"
 #include "mg_internal.hpp"
 #include "mg_paged_plan.hpp"
@@ -48,13 +51,18 @@ namespace mg
         const int32_t *table, *lens;
         void *out;
         float *part;     // [2 teams, vh, hw, D] outputs, then [2 teams, vh, hw] maxima and sums
-        int64_t *first;  // [requests + 1] first unit of each request, and their number
+        int4 *cut;       // [requests] or [teams]: what the second kernel joins (Cut)
+        int by_team;     // a Cut for each team (there are fewer than requests), not for each request
         int64_t ldq, ldt, ldo, window;
         int R, nkv, W, sh, num_pages;
         int hpg, hw, vh; // query heads a kv head, a work-group; work-groups a team
         int teams;
         float scale2;    // scaling * log2(e)
     };
+
+    // PagedArgs::cut, for a request (or for the request that begins in a team and passes its end): x the request, y
+    // the number of its partial results (0: none), z the first one's place, w the team of the second; each team
+    // behind the first begins with the request, so its part is at 2 t
 
     typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
     MG_DEV f32x4 mfma_f16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -84,15 +92,18 @@ namespace mg
     {
         return __builtin_bit_cast(X8, *reinterpret_cast<const Vec<uint32_t, 4> *>(p));
     }
-    // two weights' high and low parts at positions e, e + 1 of an operand
-    template <class M>
-    MG_DEV void split_weights(float p0, float p1, typename M::x8 &hi, typename M::x8 &lo, int e)
+    // two weights as sums of NP 16-bit parts, each the rest's nearest, at positions e, e + 1 of NP operands
+    template <class M, int NP>
+    MG_DEV void split_weights(float p0, float p1, typename M::x8 *const (&w)[NP], int e)
     {
-        const typename M::e h0 = typename M::e(p0), h1 = typename M::e(p1);
-        hi[e] = h0;
-        hi[e + 1] = h1;
-        lo[e] = typename M::e(p0 - float(h0));
-        lo[e + 1] = typename M::e(p1 - float(h1));
+#pragma unroll
+        for (int k = 0; k < NP; ++k) {
+            const typename M::e h0 = typename M::e(p0), h1 = typename M::e(p1);
+            (*w[k])[e] = h0;
+            (*w[k])[e + 1] = h1;
+            p0 -= float(h0);
+            p1 -= float(h1);
+        }
     }
 
     // 16 quants as bf16, exactly
@@ -111,65 +122,58 @@ namespace mg
         }
     }
 
-    // the work-group's run [u0, u1) of its team, the request it starts in and that
-    // request's unit; `keep`: this work-group writes the requests' first units down
+    // the work-group's run [u0, u1) of its team, the request it starts in and that request's first unit p
     struct Run
     {
-        int64_t u0, u1;
-        int b, at;
+        PagedTeams d;
+        int u0, u1, p, b;
     };
-    MG_DEV Run find_run(const PagedArgs &a, int team, bool keep)
+    MG_DEV Run find_run(const PagedArgs &a, int team, int unit)
     {
-        __shared__ int64_t red[4];
-        __shared__ Run found;
+        __shared__ int red[4], found[2];
         const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
         const int per = (a.R + 255) / 256, b0 = tid * per, b1 = min(b0 + per, a.R);
         const int cap = a.W << a.sh;
-        int64_t mine = 0;
-        for (int b = b0; b < b1; ++b) mine += paged_span(a.lens[b], cap, a.window).units;
-        int64_t pre = mine;
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-            const int64_t u = __shfl_up(pre, m, 64);
-            pre += lane >= m ? u : 0;
-        }
+        int mine = 0;
+        for (int b = b0; b < b1; ++b) mine += paged_span(a.lens[b], cap, a.window, unit).units;
+        int pre = wave_prefix_sum(mine);
         if (lane == 63) red[wv] = pre;
         __syncthreads();
         for (int w = 0; w < wv; ++w) pre += red[w];
-        const int64_t total = red[0] + red[1] + red[2] + red[3];
-        const int64_t teams = a.teams < total ? a.teams : total;
-        int64_t p = pre - mine; // the thread's first unit
-        if (keep) {
-            int64_t f = p;
-            for (int b = b0; b < b1; ++b) {
-                a.first[b] = f;
-                f += paged_span(a.lens[b], cap, a.window).units;
-            }
-            if (tid == 0) a.first[a.R] = total;
-        }
-        if (team >= teams) return Run{0, 0, 0, 0};
-        const int64_t u0 = team_first(team, total, teams), u1 = team_first(team + 1, total, teams);
-        if (u0 >= p && u0 < pre) {
+        Run r;
+        // (uniform values read from LDS go to scalar registers)
+        r.d = paged_teams(__builtin_amdgcn_readfirstlane(red[0] + red[1] + red[2] + red[3]), a.teams);
+        int p = pre - mine; // the thread's first unit
+        r.u0 = r.u1 = 0;
+        if (team >= r.d.teams) return r;
+        r.u0 = team_first(r.d, team);
+        r.u1 = team_first(r.d, team + 1);
+        if (r.u0 >= p && r.u0 < pre) {
             int b = b0;
             for (;; ++b) {
-                const int u = paged_span(a.lens[b], cap, a.window).units;
-                if (u0 < p + u) break;
+                const int u = paged_span(a.lens[b], cap, a.window, unit).units;
+                if (r.u0 < p + u) break;
                 p += u;
             }
-            found = Run{u0, u1, b, int(u0 - p)};
+            found[0] = p;
+            found[1] = b;
         }
         __syncthreads();
-        return found;
+        r.p = __builtin_amdgcn_readfirstlane(found[0]);
+        r.b = __builtin_amdgcn_readfirstlane(found[1]);
+        return r;
     }
 
     template <class S, class SO, bool Q8, int KB> // KB = head_dim / 32
-    __global__ __launch_bounds__(256) void k_attn_paged(PagedArgs a)
+    __global__ __launch_bounds__(256, 2) void k_attn_paged(PagedArgs a)
     {
         constexpr int D = 32 * KB, NT = 2 * KB;   // NT output tiles of 16 dims
+        constexpr int H = Q8 ? 2 : 1;             // 32-key halves of a step: as many bytes in flight as with 16-bit rows
+        constexpr int U = 4 * H * kPagedStep;     // keys of a unit
         constexpr int EPL = Q8 ? 16 : 8;          // elements a lane loads at once
         constexpr int LPR = D / EPL;              // lanes a row
         constexpr int RPI = 64 / LPR;             // rows a load instruction covers
-        constexpr int NLD = kPagedStep / RPI;     // load instructions a step
+        constexpr int NLD = kPagedStep / RPI;     // load instructions a half
         constexpr int SK = D + 8, SV = D + 16;    // LDS row strides (elements): conflict-free reads
         constexpr int SO4 = D + 4;                // row stride of a wave's output in LDS (floats)
         constexpr int WB = 32 * (SK + SV) * 2;    // LDS bytes of a wave's K and V
@@ -178,14 +182,21 @@ namespace mg
         using x8 = typename M::x8;
         using raw = typename SO::raw;
         constexpr int NQ = Q8 && S::dt == F16 ? 2 : 1; // parts of a query
+        // parts of a weight: two bf16 ones leave 2^-17 of it at most, 1.5e-6 of an output (2-norm), which f32
+        // outputs would show (three: 3e-7) and 16-bit ones do not; two f16 ones 2^-22
+        constexpr int NP = SO::dt == F32 && std::is_same_v<M, Mm<SBf16>> ? 3 : 2;
         constexpr float kLow = -__builtin_huge_valf();
         __shared__ __align__(16) char lds[4][WB];
-        __shared__ __align__(16) float scl[Q8 ? 4 : 1][2][32][KB];
+        __shared__ __align__(16) float scl[Q8 ? 4 : 1][2][KB][32];
         __shared__ float wm[4][16], wl[4][16];
-        const int wv = threadIdx.x >> 6, lane = threadIdx.x & 63;
+        const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
         const int team = blockIdx.x / a.vh, v = blockIdx.x - team * a.vh;
-        const Run run = find_run(a, team, blockIdx.x == 0);
-        if (run.u0 >= run.u1) return; // the whole work-group
+        const Run run = find_run(a, team, U);
+        const bool notes = a.teams > 1 && v == 0 && threadIdx.x == 0; // who writes the cuts down
+        if (run.u0 >= run.u1) { // the whole work-group
+            if (notes && a.by_team) a.cut[team] = int4{0, 0, 0, 0};
+            return;
+        }
         const int nsub = a.hpg / a.hw, g = v / nsub;
         const int h0 = g * a.hpg + (v - g * nsub) * a.hw;
         const int n = lane & 15, c = lane >> 4;
@@ -194,197 +205,245 @@ namespace mg
         const int64_t rowb = int64_t(a.nkv) * D * (Q8 ? 1 : 2); // bytes between slots
         const char *kg = static_cast<const char *>(a.kc) + int64_t(g) * D * (Q8 ? 1 : 2);
         const char *vg = static_cast<const char *>(a.vc) + int64_t(g) * D * (Q8 ? 1 : 2);
+        const uint32_t lane_off = uint32_t(pr * rowb) + 16 * pc; // (checked on the host: below 2^32)
         const int cap = a.W << a.sh, psm = (1 << a.sh) - 1;
 
-        int64_t left = run.u1 - run.u0;
-        int at = run.at;
-        for (int b = run.b; left > 0; ++b, at = 0) {
-            const PagedSpan sp = paged_span(a.lens[b], cap, a.window);
-            const int end = sp.units - at < left ? sp.units : at + int(left);
-            left -= end - at;
-            const int k0 = sp.base + at * kPagedUnit;                  // first key of the part
-            const int klo = k0 > sp.lo ? k0 : sp.lo;                   // attended keys [klo, khi)
-            const int64_t ke = int64_t(sp.base) + int64_t(end) * kPagedUnit;
-            const int khi = ke < sp.n ? int(ke) : sp.n;
-            const int32_t *tab = a.table + b * a.ldt;
+        // a part of a request in the run: units [at, end), attended keys [klo, khi), and the
+        // units of the run behind it
+        struct Part
+        {
+            int b, at, end, units, k0, klo, khi, behind;
+        };
+        auto part_of = [&](int b, int at, int left) {
+            const PagedSpan sp = paged_span(__builtin_amdgcn_readfirstlane(a.lens[b]), cap, a.window, U);
+            Part s;
+            s.b = b;
+            s.at = at;
+            s.units = sp.units;
+            s.end = sp.units - at < left ? sp.units : at + left;
+            s.behind = left - (s.end - at);
+            s.k0 = sp.base + at * U;
+            s.klo = s.k0 > sp.lo ? s.k0 : sp.lo;
+            const int64_t ke = int64_t(sp.base) + int64_t(s.end) * U;
+            s.khi = ke < sp.n ? int(ke) : sp.n;
+            return s;
+        };
+        Part cur = part_of(run.b, run.u0 - run.p, run.u1 - run.u0);
 
+        // the step whose table entries are read next: every wave takes a step of each part, which may be empty
+        Part ahead = cur;
+        int akb = cur.k0 + H * kPagedStep * wv;
+        bool more_ahead = true;
+        auto advance = [&]() {
+            akb += U;
+            if (akb < ahead.khi) return;
+            more_ahead = ahead.behind > 0;
+            if (!more_ahead) return;
+            ahead = part_of(ahead.b + 1, 0, ahead.behind);
+            akb = ahead.k0 + H * kPagedStep * wv;
+        };
+        // the slot of key akb + 32 h + lane % 32, or -1
+        auto slot_of = [&](int h) {
+            const int key = akb + kPagedStep * h + (lane & 31);
+            if (!more_ahead || key < ahead.klo || key >= ahead.khi) return -1;
+            const int page = a.table[ahead.b * a.ldt + (key >> a.sh)];
+            return page >= 0 && page < a.num_pages ? (page << a.sh) + (key & psm) : -1;
+        };
+        Vec<uint32_t, 4> stk[H][NLD], stv[H][NLD];
+        Vec<uint16_t, KB> sts[H]; // scales of key lane % 32: K's in the lower half of the wave, V's in the upper
+        auto stage = [&](int h, int slot, uint32_t seen) {
+            if constexpr (Q8) {
+                sts[h] = Vec<uint16_t, KB>{};
+                const uint16_t *sc = lane < 32 ? a.kd : a.vd;
+                if (slot >= 0)
+                    sts[h] = *reinterpret_cast<const Vec<uint16_t, KB> *>(sc + (int64_t(slot) * a.nkv + g) * KB);
+            }
+            if (seen == 0xffffffffu && psm + 1 >= RPI) {
+#pragma unroll
+                for (int i = 0; i < NLD; ++i) {
+                    int64_t o = __builtin_amdgcn_readlane(slot, RPI * i) * rowb;
+                    __asm__("" : "+s"(o)); // the rows' base stays in scalar registers, the lane's offset in one
+                    const char *kp = kg + o, *vp = vg + o;
+                    stk[h][i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(kp + lane_off));
+                    stv[h][i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(vp + lane_off));
+                }
+                return;
+            }
+#pragma unroll
+            for (int i = 0; i < NLD; ++i) {
+                const int s = __shfl(slot, pr + RPI * i, 64);
+                stk[h][i] = Vec<uint32_t, 4>{{0u, 0u, 0u, 0u}};
+                stv[h][i] = stk[h][i];
+                if (s >= 0) {
+                    const int64_t o = s * rowb + 16 * pc;
+                    stk[h][i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(kg + o));
+                    stv[h][i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(vg + o));
+                }
+            }
+        };
+        int slot[H];
+        uint32_t seen[H]; // keys of the staged halves, one bit each
+#pragma unroll
+        for (int h = 0; h < H; ++h) slot[h] = slot_of(h);
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            seen[h] = uint32_t(__builtin_amdgcn_ballot_w64(slot[h] >= 0));
+            stage(h, slot[h], seen[h]);
+        }
+        advance();
+#pragma unroll
+        for (int h = 0; h < H; ++h) slot[h] = slot_of(h);
+
+        for (;;) {
             // B of S^T: lane (head n, c) holds q[n][32 kb + 8c ..], zero for padding heads
             x8 qop[NQ][KB];
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
                 const uint16_t *qp =
-                    static_cast<const uint16_t *>(a.q) + b * a.ldq + int64_t(h0 + n) * D + 32 * kb + 8 * c;
+                    static_cast<const uint16_t *>(a.q) + cur.b * a.ldq + int64_t(h0 + n) * D + 32 * kb + 8 * c;
                 if constexpr (NQ == 1) {
                     qop[0][kb] = n < a.hw ? ld_x8<x8>(qp) : x8{};
                 } else {
                     const f16x8 x = n < a.hw ? ld_x8<f16x8>(qp) : f16x8{};
+                    x8 *const parts[2] = {&qop[0][kb], &qop[1][kb]};
 #pragma unroll
-                    for (int e = 0; e < 8; e += 2)
-                        split_weights<M>(float(x[e]), float(x[e + 1]), qop[0][kb], qop[1][kb], e);
+                    for (int e = 0; e < 8; e += 2) split_weights<M, 2>(float(x[e]), float(x[e + 1]), parts, e);
                 }
             }
-            // the slot of key kb + lane % 32, or -1
-            auto slot_of = [&](int kb) {
-                const int key = kb + (lane & 31);
-                if (key < klo || key >= khi) return -1;
-                const int page = tab[key >> a.sh];
-                return page >= 0 && page < a.num_pages ? (page << a.sh) + (key & psm) : -1;
-            };
-            Vec<uint32_t, 4> stk[NLD], stv[NLD];
-            Vec<uint16_t, KB> sts; // scales of key lane % 32: K's in the lower half of the wave, V's in the upper
-            auto stage = [&](int slot, uint32_t seen) {
-                if constexpr (Q8) {
-                    sts = Vec<uint16_t, KB>{};
-                    const uint16_t *sc = lane < 32 ? a.kd : a.vd;
-                    if (slot >= 0)
-                        sts = *reinterpret_cast<const Vec<uint16_t, KB> *>(sc + (int64_t(slot) * a.nkv + g) * KB);
-                }
-                if (seen == 0xffffffffu && psm + 1 >= RPI) {
-#pragma unroll
-                    for (int i = 0; i < NLD; ++i) {
-                        const int64_t s0 = __builtin_amdgcn_readlane(slot, RPI * i);
-                        const int64_t o = s0 * rowb + int64_t(pr) * rowb + 16 * pc;
-                        stk[i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(kg + o));
-                        stv[i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(vg + o));
-                    }
-                    return;
-                }
-#pragma unroll
-                for (int i = 0; i < NLD; ++i) {
-                    const int s = __shfl(slot, pr + RPI * i, 64);
-                    stk[i] = Vec<uint32_t, 4>{{0u, 0u, 0u, 0u}};
-                    stv[i] = stk[i];
-                    if (s >= 0) {
-                        const int64_t o = s * rowb + 16 * pc;
-                        stk[i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(kg + o));
-                        stv[i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(vg + o));
-                    }
-                }
-            };
-
             f32x4 o[NT];
 #pragma unroll
             for (int t = 0; t < NT; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             float m = kLow, l = 0.0f; // head n (replicated over c)
-            int kb = k0 + kPagedStep * wv;
-            int slot = slot_of(kb);
-            uint32_t seen = uint32_t(__builtin_amdgcn_ballot_w64(slot >= 0)), seen1 = 0;
-            if (kb < khi) stage(slot, seen);
-            slot = slot_of(kb + kPagedUnit);
-            for (; kb < khi; kb += kPagedUnit) {
+            int kb = cur.k0 + H * kPagedStep * wv;
+            bool more;
+            do {
+                kb += U;
+                more = kb < cur.khi;
+                const bool any = more_ahead;
 #pragma unroll
-                for (int i = 0; i < NLD; ++i) {
-                    const int key = pr + RPI * i;
-                    if constexpr (Q8) {
-                        q8_bf16(stk[i], sk + key * SK + 16 * pc);
-                        q8_bf16(stv[i], sv + key * SV + 16 * pc);
-                    } else {
-                        *reinterpret_cast<Vec<uint32_t, 4> *>(sk + key * SK + 8 * pc) = stk[i];
-                        *reinterpret_cast<Vec<uint32_t, 4> *>(sv + key * SV + 8 * pc) = stv[i];
-                    }
-                }
-                if constexpr (Q8) {
-                    Vec<float, KB> f;
+                for (int h = 0; h < H; ++h) {
+                    const uint32_t now = seen[h];
+                    if (now != 0) {
 #pragma unroll
-                    for (int i = 0; i < KB; ++i) f.v[i] = f16_f32(sts.v[i]);
-                    *reinterpret_cast<Vec<float, KB> *>(scl[wv][lane >> 5][lane & 31]) = f;
-                }
-                wave_lds_sync();
-                // K as A of S^T: lane (key n, c) holds dims 32 kb + 8c.. of key 16 t + n
-                x8 kt[2][KB];
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int i = 0; i < KB; ++i) kt[t][i] = ld_x8<x8>(sk + (16 * t + n) * SK + 32 * i + 8 * c);
-                // the next step's rows and the table entries of the one behind it are requested now
-                if (kb + kPagedUnit < khi) {
-                    seen1 = uint32_t(__builtin_amdgcn_ballot_w64(slot >= 0));
-                    stage(slot, seen1);
-                    slot = slot_of(kb + 2 * kPagedUnit);
-                }
-                // scores of keys 16 t + 4c + r for head n
-                float sc[2][4], mx = kLow;
-#pragma unroll
-                for (int t = 0; t < 2; ++t) {
-                    f32x4 st = {0.0f, 0.0f, 0.0f, 0.0f};
-                    if constexpr (Q8) {
-                        f32x4 part[KB];
-#pragma unroll
-                        for (int i = 0; i < KB; ++i) {
-                            part[i] = M::mma(kt[t][i], qop[0][i], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-                            if constexpr (NQ == 2) part[i] = M::mma(kt[t][i], qop[1][i], part[i]);
-                        }
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            const Vec<float, KB> d =
-                                *reinterpret_cast<const Vec<float, KB> *>(scl[wv][0][16 * t + 4 * c + r]);
-#pragma unroll
-                            for (int i = 0; i < KB; ++i) st[r] = __builtin_fmaf(d.v[i], part[i][r], st[r]);
-                        }
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < KB; ++i) st = M::mma(kt[t][i], qop[0][i], st);
-                    }
-                    const uint32_t bits = seen >> (16 * t + 4 * c);
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        sc[t][r] = st[r] * a.scale2;
-                        sc[t][r] = (bits >> r & 1) != 0 ? sc[t][r] : kLow;
-                        mx = __builtin_fmaxf(mx, sc[t][r]);
-                    }
-                }
-                mx = rows4_max(mx);
-                const float mn = __builtin_fmaxf(m, mx);
-                // no score above -inf yet: a zero reference, so that -inf scores weigh 0
-                // and only NaN ones reach the sum
-                const float mref = mn == kLow ? 0.0f : mn;
-                // weights: element 4t + r of lane (head n, c) is key 16 t + 4c + r
-                float p[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(sc[e >> 2][e & 3] - (mref - M::up));
-                if (__builtin_amdgcn_ballot_w64(mn != m) != 0) {
-                    // some head's running max moved: rescale its sum and its O row
-                    // (rows are heads 4c + r; their factors come from lanes 4c + r)
-                    const float corr = __builtin_amdgcn_exp2f(m - mref); // first step: 2^-inf = 0
-                    l *= corr;
-                    float cr[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) cr[r] = __shfl(corr, 4 * c + r, 64);
-#pragma unroll
-                    for (int t = 0; t < NT; ++t)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) o[t][r] *= cr[r];
-                }
-                m = mn;
-                l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-                // V as B of P V: lane (dim n, c) needs keys 4c + r and 16 + 4c + r
-                // of dim 16 s + n, through the transposing read
-                const uint16_t *vr = sv + (4 * c + (n >> 2)) * SV + 4 * (n & 3);
-                x8 phi, plo;
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    if constexpr (Q8) {
-                        if (t % 2 == 0)
-#pragma unroll
-                            for (int e = 0; e < 8; e += 2) {
-                                const int key = 16 * (e >> 2) + 4 * c + (e & 3);
-                                split_weights<M>(p[e] * scl[wv][1][key][t / 2], p[e + 1] * scl[wv][1][key + 1][t / 2],
-                                                 phi, plo, e);
+                        for (int i = 0; i < NLD; ++i) {
+                            const int key = pr + RPI * i;
+                            if constexpr (Q8) {
+                                q8_bf16(stk[h][i], sk + key * SK + 16 * pc);
+                                q8_bf16(stv[h][i], sv + key * SV + 16 * pc);
+                            } else {
+                                *reinterpret_cast<Vec<uint32_t, 4> *>(sk + key * SK + 8 * pc) = stk[h][i];
+                                *reinterpret_cast<Vec<uint32_t, 4> *>(sv + key * SV + 8 * pc) = stv[h][i];
                             }
-                    } else if (t == 0) {
+                        }
+                        if constexpr (Q8)
 #pragma unroll
-                        for (int e = 0; e < 8; e += 2) split_weights<M>(p[e], p[e + 1], phi, plo, e);
+                            for (int i = 0; i < KB; ++i) scl[wv][lane >> 5][i][lane & 31] = f16_f32(sts[h].v[i]);
+                        wave_lds_sync();
                     }
-                    const bf16x4 v0 = lds_read_tr(vr + 16 * t);
-                    const bf16x4 v1 = lds_read_tr(vr + 16 * SV + 16 * t);
-                    const x8 vb =
-                        __builtin_bit_cast(x8, bf16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
-                    o[t] = M::mma(phi, vb, o[t]);
-                    o[t] = M::mma(plo, vb, o[t]);
+                    // the next step's rows and the table entries of the one behind it are requested now
+                    if (any) {
+                        seen[h] = uint32_t(__builtin_amdgcn_ballot_w64(slot[h] >= 0));
+                        stage(h, slot[h], seen[h]);
+                        if (h == H - 1) {
+                            advance();
+#pragma unroll
+                            for (int i = 0; i < H; ++i) slot[i] = slot_of(i);
+                        }
+                    }
+                    if (now == 0) continue;
+                    // K as A of S^T: lane (key n, c) holds dims 32 i + 8c.. of key 16 t + n
+                    x8 kt[2][KB];
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int i = 0; i < KB; ++i) kt[t][i] = ld_x8<x8>(sk + (16 * t + n) * SK + 32 * i + 8 * c);
+                    // scores of keys 16 t + 4c + r for head n
+                    float sc[2][4], mx = kLow;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        f32x4 st = {0.0f, 0.0f, 0.0f, 0.0f};
+                        if constexpr (Q8) {
+#pragma unroll
+                            for (int i = 0; i < KB; ++i) {
+                                f32x4 part = M::mma(kt[t][i], qop[0][i], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                                if constexpr (NQ == 2) part = M::mma(kt[t][i], qop[1][i], part);
+                                const Vec<float, 4> d =
+                                    *reinterpret_cast<const Vec<float, 4> *>(scl[wv][0][i] + 16 * t + 4 * c);
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) st[r] = __builtin_fmaf(d.v[r], part[r], st[r]);
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < KB; ++i) st = M::mma(kt[t][i], qop[0][i], st);
+                        }
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) sc[t][r] = st[r] * a.scale2;
+                        if (now != 0xffffffffu) {
+                            const uint32_t bits = now >> (16 * t + 4 * c);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) sc[t][r] = (bits >> r & 1) != 0 ? sc[t][r] : kLow;
+                        }
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) mx = __builtin_fmaxf(mx, sc[t][r]);
+                    }
+                    mx = rows4_max(mx);
+                    const float mn = __builtin_fmaxf(m, mx);
+                    // no score above -inf yet: a zero reference, so that -inf scores weigh 0
+                    // and only NaN ones reach the sum
+                    const float mref = mn == kLow ? 0.0f : mn;
+                    // weights: element 4t + r of lane (head n, c) is key 16 t + 4c + r
+                    float p[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(sc[e >> 2][e & 3] - (mref - M::up));
+                    if (__builtin_amdgcn_ballot_w64(mn != m) != 0) {
+                        // some head's running max moved: rescale its sum and its O row
+                        // (rows are heads 4c + r; their factors come from lanes 4c + r)
+                        const float corr = __builtin_amdgcn_exp2f(m - mref); // first step: 2^-inf = 0
+                        l *= corr;
+                        float cr[4];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) cr[r] = __shfl(corr, 4 * c + r, 64);
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) o[t][r] *= cr[r];
+                    }
+                    m = mn;
+                    l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                    // V as B of P V: lane (dim n, c) needs keys 4c + r and 16 + 4c + r
+                    // of dim 16 s + n, through the transposing read
+                    const uint16_t *vr = sv + (4 * c + (n >> 2)) * SV + 4 * (n & 3);
+                    x8 w[NP];
+                    x8 *parts[NP];
+#pragma unroll
+                    for (int k = 0; k < NP; ++k) parts[k] = &w[k];
+#pragma unroll
+                    for (int t = 0; t < NT; ++t) {
+                        if constexpr (Q8) {
+                            if (t % 2 == 0) {
+                                const float *d = scl[wv][1][t / 2] + 4 * c;
+                                const Vec<float, 4> d0 = *reinterpret_cast<const Vec<float, 4> *>(d);
+                                const Vec<float, 4> d1 = *reinterpret_cast<const Vec<float, 4> *>(d + 16);
+#pragma unroll
+                                for (int e = 0; e < 4; e += 2) {
+                                    split_weights<M, NP>(p[e] * d0.v[e], p[e + 1] * d0.v[e + 1], parts, e);
+                                    split_weights<M, NP>(p[4 + e] * d1.v[e], p[5 + e] * d1.v[e + 1], parts, 4 + e);
+                                }
+                            }
+                        } else if (t == 0) {
+#pragma unroll
+                            for (int e = 0; e < 8; e += 2) split_weights<M, NP>(p[e], p[e + 1], parts, e);
+                        }
+                        const bf16x4 v0 = lds_read_tr(vr + 16 * t);
+                        const bf16x4 v1 = lds_read_tr(vr + 16 * SV + 16 * t);
+                        const x8 vb =
+                            __builtin_bit_cast(x8, bf16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
+#pragma unroll
+                        for (int k = 0; k < NP; ++k) o[t] = M::mma(w[k], vb, o[t]);
+                    }
+                    wave_lds_sync(); // this half's reads are done before the next one's writes
                 }
-                seen = seen1;
-                wave_lds_sync(); // this step's reads are done before the next step's writes
-            }
+            } while (more);
 
             // join the four waves: their outputs take the place of K and V in LDS
             l = rows4_sum(l);
@@ -398,6 +457,15 @@ namespace mg
 #pragma unroll
                 for (int r = 0; r < 4; ++r) so[(4 * c + r) * SO4 + 16 * t + n] = o[t][r];
             __syncthreads();
+            const bool whole = cur.at == 0 && cur.end == cur.units;
+            if (notes && (a.by_team ? cur.behind == 0 : cur.at == 0)) {
+                int4 cut{cur.b, 0, 2 * team + (cur.b == run.b ? 0 : 1), team + 1};
+                if (cur.at == 0 && !whole) {
+                    const int first = run.u1 - cur.behind - cur.end; // the request's first unit
+                    cut.y = team_of(run.d, first + cur.units - 1) - team + 1;
+                }
+                a.cut[a.by_team ? team : cur.b] = cut;
+            }
             const int hh = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (D / 16);
             if (hh < a.hw) {
                 const float top = __builtin_fmaxf(__builtin_fmaxf(wm[0][hh], wm[1][hh]), __builtin_fmaxf(wm[2][hh], wm[3][hh]));
@@ -417,13 +485,13 @@ namespace mg
                         for (int i = 0; i < 4; ++i) acc[e + i] = __builtin_fmaf(f, x.v[i], acc[e + i]);
                     }
                 }
-                if (at == 0 && end == sp.units) {
+                if (whole) {
                     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                    raw *dst = static_cast<raw *>(a.out) + b * a.ldo + int64_t(h0 + hh) * D + d0;
+                    raw *dst = static_cast<raw *>(a.out) + cur.b * a.ldo + int64_t(h0 + hh) * D + d0;
 #pragma unroll
                     for (int e = 0; e < D / 16; ++e) dst[e] = SO::enc32(acc[e] * inv);
                 } else {
-                    const int64_t pl = 2 * int64_t(team) + (b == run.b ? 0 : 1);
+                    const int64_t pl = 2 * int64_t(team) + (cur.b == run.b ? 0 : 1);
                     const int64_t row = (pl * a.vh + v) * a.hw + hh;
                     float *dst = a.part + row * D + d0;
 #pragma unroll
@@ -436,59 +504,41 @@ namespace mg
                     }
                 }
             }
-            __syncthreads(); // the next request's first step writes where the outputs were
+            __syncthreads(); // the next part's first step writes where the outputs were
+            if (cur.behind == 0) break;
+            cur = part_of(cur.b + 1, 0, cur.behind);
         }
     }
 
-    // Joins the partial results of the requests that a team's edge cuts: top = max m_s,
-    // out = sum_s 2^(m_s - top) acc_s / sum_s 2^(m_s - top) l_s over the request's teams.
-    // A work-group takes 4 E of the outputs of one (request, work-group of heads), E
-    // threads wide, 256 / E threads over the teams. blockIdx.x is the request, or, where
-    // there are fewer edges than requests, the edge: its request's first one joins.
+    // Joins the partial results of one request and work-group of heads: top = max m_s,
+    // out = sum_s 2^(m_s - top) acc_s / sum_s 2^(m_s - top) l_s. A work-group takes 4 E of the
+    // outputs, thread (e, sg) four of them over every SG-th part from sg; SG threads' shares
+    // are added in LDS, in the order of sg.
     template <class SO, int E>
-    __global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a, int D, int by_edge)
+    __global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a, int D)
     {
         constexpr int SG = 256 / E;
         __shared__ float tops[SG][E], sums[SG][E];
         __shared__ Vec<float, 4> accs[SG][E];
-        const int64_t total = a.first[a.R];
-        const int64_t teams = a.teams < total ? a.teams : total;
-        int b = blockIdx.x;
-        if (by_edge) {
-            const int64_t t = int64_t(blockIdx.x) + 1; // the edge between teams t - 1 and t
-            if (t >= teams) return;
-            const int64_t u = team_first(t, total, teams);
-            int lo = 0, hi = a.R; // the request that holds unit u
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (a.first[mid] <= u)
-                    lo = mid;
-                else
-                    hi = mid;
-            }
-            b = lo;
-            if (team_of(a.first[b], total, teams) != t - 1) return;
-        }
-        const int64_t p0 = a.first[b], p1 = a.first[b + 1];
-        const int64_t t0 = team_of(p0, total, teams);
-        const int nt = int(team_of(p1 - 1, total, teams) - t0) + 1;
-        if (nt == 1) return; // finished in its team
-        const int v = blockIdx.y;
-        const int e = threadIdx.x % E, sg = threadIdx.x / E;
+        const int4 cut = a.cut[blockIdx.x];
+        const int nt = cut.y;
+        if (nt == 0) return; // finished in its team
+        const int v = blockIdx.y, e = threadIdx.x % E, sg = threadIdx.x / E;
         const int i0 = (int(blockIdx.z) * E + e) * 4; // the thread's outputs among [hw, D]
         const bool live = i0 < a.hw * D;
-        const int hh = live ? i0 / D : 0;
+        const int hh = live ? i0 / D : 0; // (a work-group's outputs may be of several heads)
         const float *ml = a.part + 2 * int64_t(a.teams) * a.vh * a.hw * D;
-        auto row = [&](int s) { return (team_place(t0 + s, p0, total, teams) * a.vh + v) * a.hw; };
-        // (a work-group's outputs may be of several heads: each thread goes by its own)
-        float top = -__builtin_huge_valf();
+        auto row = [&](int s) {
+            const int place = s == 0 ? cut.z : 2 * (cut.w + s - 1);
+            return (int64_t(place) * a.vh + v) * a.hw;
+        };
+        float top = -__builtin_huge_valf(), sum = 0.0f;
         for (int s = sg; s < nt; s += SG) top = __builtin_fmaxf(top, ml[2 * (row(s) + hh)]);
         tops[sg][e] = top;
         __syncthreads();
 #pragma unroll
         for (int s = 0; s < SG; ++s) top = __builtin_fmaxf(top, tops[s][e]);
         const float ref = top == -__builtin_huge_valf() ? 0.0f : top;
-        float sum = 0.0f;
         Vec<float, 4> acc{{0.0f, 0.0f, 0.0f, 0.0f}};
         for (int s = sg; s < nt; s += SG) {
             const int64_t r = row(s);
@@ -512,8 +562,8 @@ namespace mg
         }
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
         const int nsub = a.hpg / a.hw, g = v / nsub;
-        const int h = g * a.hpg + (v - g * nsub) * a.hw + hh;
-        typename SO::raw *dst = static_cast<typename SO::raw *>(a.out) + b * a.ldo + int64_t(h) * D + (i0 - hh * D);
+        const int h0 = g * a.hpg + (v - g * nsub) * a.hw;
+        typename SO::raw *dst = static_cast<typename SO::raw *>(a.out) + cut.x * a.ldo + int64_t(h0) * D + i0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) dst[i] = SO::enc32(acc.v[i] * inv);
     }
@@ -527,7 +577,7 @@ namespace mg
         const int sh = page_shift(page_size, "attn_decode_paged");
         need(seqs >= 0 && nq > 0 && nkv > 0 && nq % nkv == 0,
              "attn_decode_paged: q_heads must be a multiple of kv_heads");
-        need(nq <= 65535, "attn_decode_paged: too many heads");
+        need(nq <= 65535, "attn_decode_paged: too many heads"); // (16 rows of a load stay below 2^32 bytes)
         need(D == 64 || D == 128, "attn_decode_paged: head_dim must be 64 or 128");
         need(dt == BF16 || dt == F16, "attn_decode_paged: dtype must be bf16 or f16");
         need(dt_out == dt || dt_out == F32, "attn_decode_paged: dtype_out must be f32 or q's dtype");
@@ -552,23 +602,26 @@ namespace mg
         int64_t hw = hpg;
         while (hw > 16 || hpg % hw != 0) --hw;
         const int64_t vh = nkv * (hpg / hw);
-        // as many teams as fill the chip twice (two work-groups fit a CU's LDS), not more
-        // than there can be units, nor than the workspace has room for
+        // as many teams as the chip holds at once (the work-groups that a CU's LDS and registers
+        // take), not more than there can be units, nor than the workspace has room for
+        const int per_cu = D == 128 ? 2 : kd ? 3 : 4;
+        const int unit = 4 * kPagedStep * (kd ? 2 : 1);
         const int64_t span = window > 0 && window < max_pages << sh ? window + kPagedStep : max_pages << sh;
-        const int64_t most = seqs * (span / kPagedUnit + 1);
-        int64_t teams = 2 * int64_t(c->num_cus) / vh;
+        const int64_t most = seqs * (span / unit + 1);
+        need(most < (int64_t(1) << 31), "attn_decode_paged: the table must stand for fewer than 2^31 units of " +
+                                            std::to_string(unit) + " keys");
+        int64_t teams = per_cu * int64_t(c->num_cus) / vh;
         teams = teams < most ? teams : most;
-        const int64_t fbytes = (seqs + 1) * int64_t(sizeof(int64_t));
-        const int64_t tbytes = 2 * vh * hw * (D + 2) * int64_t(sizeof(float));
-        need(fbytes <= c->work_bytes, "attn_decode_paged: the requests' sums exceed the context workspace");
-        // (from a 16-byte boundary behind the sums)
-        const int64_t room = (c->work_bytes - (fbytes + 15) / 16 * 16) / tbytes;
-        teams = teams < room ? teams : room;
+        // (the cuts, then the partial results' outputs, then their maxima and sums)
+        const int64_t tbytes = 2 * vh * hw * (D + 2) * int64_t(sizeof(float)) + int64_t(sizeof(int4));
+        teams = teams < c->work_bytes / tbytes ? teams : c->work_bytes / tbytes;
         teams = teams > 1 ? teams : 1;
+        const bool by_team = teams < seqs; // else there is room for a cut of each request among the teams'
         PagedArgs a{};
         a.q = q, a.kc = kc, a.vc = vc, a.kd = kd, a.vd = vd, a.table = table, a.lens = lens, a.out = out;
-        a.first = static_cast<int64_t *>(c->work);
-        a.part = reinterpret_cast<float *>(static_cast<char *>(c->work) + (fbytes + 15) / 16 * 16);
+        a.cut = static_cast<int4 *>(c->work);
+        a.part = reinterpret_cast<float *>(a.cut + teams);
+        a.by_team = by_team;
         a.ldq = ldq, a.ldt = ldt, a.ldo = ldo, a.window = window;
         a.R = int(seqs), a.nkv = int(nkv), a.W = int(max_pages), a.sh = sh, a.num_pages = int(num_pages);
         a.hpg = int(hpg), a.hw = int(hw), a.vh = int(vh), a.teams = int(teams);
@@ -585,15 +638,14 @@ namespace mg
             else
                 D == 128 ? go(k_attn_paged<S, SO, false, 4>) : go(k_attn_paged<S, SO, false, 2>);
             if (teams == 1) return; // nothing is cut
-            const bool by_edge = teams - 1 < seqs;
-            const int64_t who = by_edge ? teams - 1 : seqs;
+            const int64_t who = by_team ? teams - 1 : seqs; // (the last team's end cuts nothing)
             auto join = [&](auto kern, int e) {
                 const dim3 grid{unsigned(who), unsigned(vh), unsigned((hw * D + 4 * e - 1) / (4 * e))};
-                hipLaunchKernelGGL(kern, grid, dim3(256), 0, c->stream, a, int(D), int(by_edge));
+                hipLaunchKernelGGL(kern, grid, dim3(256), 0, c->stream, a, int(D));
                 check_launch("k_attn_paged_join");
             };
             // few requests over many teams: threads over the teams; else over the outputs
-            teams / who >= 16 ? join(k_attn_paged_join<SO, 16>, 16) : join(k_attn_paged_join<SO, 64>, 64);
+            teams / who >= 8 ? join(k_attn_paged_join<SO, 16>, 16) : join(k_attn_paged_join<SO, 64>, 64);
         };
         if (dt_out == F32)
             dt == BF16 ? sized(SBf16{}, SF32{}) : sized(SF16{}, SF32{});
