@@ -19,8 +19,8 @@
 // last of a request's own work-groups instead, behind device-wide fences, a call
 // took 19 to 52 us longer: a fence writes back an XCD's whole L2.)
 //
-// A work-group's four waves take steps of the run in turn, 32 keys (Q8_0: two
-// halves of 32), with no barrier until the request ends. Per step, as in the
+// A work-group's four waves take steps of 32 keys of the run in turn, with no
+// barrier until the request ends. Per step, as in the
 // ring's decode kernel: whole rows are loaded in 16-byte pieces one step ahead,
 // across the end of a request, and written to LDS;
 // S^T = K Q^T and O += P V run on the matrix cores (16 query heads of the
@@ -35,9 +35,9 @@
 // (NaN too) cannot reach the sums.
 //   f16: weights are kept at 2^12 p, so that the low part of a weight down to
 // 2^-26 of the largest is a normal number; sum and output carry the factor.
-//   Q8_0: quants become bf16 (exact: 8 bits) on their way to LDS; a K block's
-// scale multiplies its 32-dim part of the score, a V block's its weights, so no
-// value is rounded to 16 bits; the weights get their parts then. f16 queries enter as a high and a low bf16 part.
+//   Q8_0: quants become bf16, or f16 beside f16 queries, on their way from LDS,
+// exactly (8 bits); a K block's scale multiplies its 32-dim part of the score, a
+// V block's its weights before they are split, so no value is rounded to 16 bits.
 #include "mg_device.hpp"
 #include "mg_internal.hpp"
 #include "mg_paged_plan.hpp"
@@ -106,20 +106,41 @@ namespace mg
         }
     }
 
-    // 16 quants as bf16, exactly
-    MG_DEV void q8_bf16(const Vec<uint32_t, 4> &x, uint16_t *dst)
+    // eight quants as bf16, exactly
+    MG_DEV bf16x8 q8_bf16(Vec<uint32_t, 2> x)
     {
+        Vec<uint32_t, 4> w;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            Vec<uint32_t, 4> w;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const uint32_t u = x.v[2 * h + i];
-                w.v[2 * i] = bf_pack(float(int8_t(u)), float(int8_t(u >> 8)));
-                w.v[2 * i + 1] = bf_pack(float(int8_t(u >> 16)), float(int32_t(u) >> 24));
-            }
-            *reinterpret_cast<Vec<uint32_t, 4> *>(dst + 8 * h) = w;
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t u = x.v[i];
+            w.v[2 * i] = bf_pack(float(int8_t(u)), float(int8_t(u >> 8)));
+            w.v[2 * i + 1] = bf_pack(float(int8_t(u >> 16)), float(int32_t(u) >> 24));
         }
+        return __builtin_bit_cast(bf16x8, w);
+    }
+    // eight quants as f16, exactly: 1024 + u in the mantissa of u = q + 128, less 1152
+    MG_DEV f16x8 q8_f16(Vec<uint32_t, 2> x)
+    {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        const f16x2 off = {_Float16(-1152.0f), _Float16(-1152.0f)};
+        Vec<uint32_t, 4> w;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const uint32_t u = x.v[i] ^ 0x80808080u;
+            w.v[2 * i] = __builtin_bit_cast(
+                uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + off);
+            w.v[2 * i + 1] = __builtin_bit_cast(
+                uint32_t, __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + off);
+        }
+        return __builtin_bit_cast(f16x8, w);
+    }
+    // ds_read_b64_tr_b8: within each 16-lane group, lane i receives byte i % 8 of the
+    // 8-byte pieces addressed by lanes 2j + i / 8, j = 0..7
+    MG_DEV Vec<uint32_t, 2> lds_read_tr8(const char *p)
+    {
+        typedef int i32x2 __attribute__((ext_vector_type(2)));
+        typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+        return __builtin_bit_cast(Vec<uint32_t, 2>, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2 *)(p)));
     }
 
     // the work-group's run [u0, u1) of its team, the request it starts in and that request's first unit p
@@ -128,14 +149,14 @@ namespace mg
         PagedTeams d;
         int u0, u1, p, b;
     };
-    MG_DEV Run find_run(const PagedArgs &a, int team, int unit)
+    MG_DEV Run find_run(const PagedArgs &a, int team)
     {
         __shared__ int red[4], found[2];
         const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
         const int per = (a.R + 255) / 256, b0 = tid * per, b1 = min(b0 + per, a.R);
         const int cap = a.W << a.sh;
         int mine = 0;
-        for (int b = b0; b < b1; ++b) mine += paged_span(a.lens[b], cap, a.window, unit).units;
+        for (int b = b0; b < b1; ++b) mine += paged_span(a.lens[b], cap, a.window).units;
         int pre = wave_prefix_sum(mine);
         if (lane == 63) red[wv] = pre;
         __syncthreads();
@@ -151,7 +172,7 @@ namespace mg
         if (r.u0 >= p && r.u0 < pre) {
             int b = b0;
             for (;; ++b) {
-                const int u = paged_span(a.lens[b], cap, a.window, unit).units;
+                const int u = paged_span(a.lens[b], cap, a.window).units;
                 if (r.u0 < p + u) break;
                 p += u;
             }
@@ -165,23 +186,23 @@ namespace mg
     }
 
     template <class S, class SO, bool Q8, int KB> // KB = head_dim / 32
-    __global__ __launch_bounds__(256, 2) void k_attn_paged(PagedArgs a)
+    __global__ __launch_bounds__(256, Q8 ? 3 : 2) void k_attn_paged(PagedArgs a)
     {
         constexpr int D = 32 * KB, NT = 2 * KB;   // NT output tiles of 16 dims
-        constexpr int H = Q8 ? 2 : 1;             // 32-key halves of a step: as many bytes in flight as with 16-bit rows
-        constexpr int U = 4 * H * kPagedStep;     // keys of a unit
+        constexpr int U = kPagedUnit;
         constexpr int EPL = Q8 ? 16 : 8;          // elements a lane loads at once
         constexpr int LPR = D / EPL;              // lanes a row
         constexpr int RPI = 64 / LPR;             // rows a load instruction covers
         constexpr int NLD = kPagedStep / RPI;     // load instructions a half
-        constexpr int SK = D + 8, SV = D + 16;    // LDS row strides (elements): conflict-free reads
+        // LDS row strides (bytes): conflict-free reads (V's quants: two-way)
+        constexpr int SK = Q8 ? D + 16 : 2 * (D + 8), SV = Q8 ? D + 16 : 2 * (D + 16);
         constexpr int SO4 = D + 4;                // row stride of a wave's output in LDS (floats)
-        constexpr int WB = 32 * (SK + SV) * 2;    // LDS bytes of a wave's K and V
+        constexpr int WB = 32 * (SK + SV);        // LDS bytes of a wave's K and V
         static_assert(16 * SO4 * 4 <= WB, "a wave's output takes the place of its K and V");
-        using M = Mm<std::conditional_t<Q8, SBf16, S>>;
+        using MS = Mm<S>;                               // the scores' product, at q's type
+        using M = Mm<std::conditional_t<Q8, SBf16, S>>; // the outputs'
         using x8 = typename M::x8;
         using raw = typename SO::raw;
-        constexpr int NQ = Q8 && S::dt == F16 ? 2 : 1; // parts of a query
         // parts of a weight: two bf16 ones leave 2^-17 of it at most, 1.5e-6 of an output (2-norm), which f32
         // outputs would show (three: 3e-7) and 16-bit ones do not; two f16 ones 2^-22
         constexpr int NP = SO::dt == F32 && std::is_same_v<M, Mm<SBf16>> ? 3 : 2;
@@ -191,7 +212,7 @@ namespace mg
         __shared__ float wm[4][16], wl[4][16];
         const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
         const int team = blockIdx.x / a.vh, v = blockIdx.x - team * a.vh;
-        const Run run = find_run(a, team, U);
+        const Run run = find_run(a, team);
         const bool notes = a.teams > 1 && v == 0 && threadIdx.x == 0; // who writes the cuts down
         if (run.u0 >= run.u1) { // the whole work-group
             if (notes && a.by_team) a.cut[team] = int4{0, 0, 0, 0};
@@ -200,7 +221,7 @@ namespace mg
         const int nsub = a.hpg / a.hw, g = v / nsub;
         const int h0 = g * a.hpg + (v - g * nsub) * a.hw;
         const int n = lane & 15, c = lane >> 4;
-        uint16_t *sk = reinterpret_cast<uint16_t *>(lds[wv]), *sv = sk + 32 * SK;
+        char *sk = lds[wv], *sv = sk + 32 * SK;
         const int pc = lane % LPR, pr = lane / LPR;
         const int64_t rowb = int64_t(a.nkv) * D * (Q8 ? 1 : 2); // bytes between slots
         const char *kg = static_cast<const char *>(a.kc) + int64_t(g) * D * (Q8 ? 1 : 2);
@@ -215,7 +236,7 @@ namespace mg
             int b, at, end, units, k0, klo, khi, behind;
         };
         auto part_of = [&](int b, int at, int left) {
-            const PagedSpan sp = paged_span(__builtin_amdgcn_readfirstlane(a.lens[b]), cap, a.window, U);
+            const PagedSpan sp = paged_span(__builtin_amdgcn_readfirstlane(a.lens[b]), cap, a.window);
             Part s;
             s.b = b;
             s.at = at;
@@ -232,7 +253,7 @@ namespace mg
 
         // the step whose table entries are read next: every wave takes a step of each part, which may be empty
         Part ahead = cur;
-        int akb = cur.k0 + H * kPagedStep * wv;
+        int akb = cur.k0 + kPagedStep * wv;
         bool more_ahead = true;
         auto advance = [&]() {
             akb += U;
@@ -240,23 +261,23 @@ namespace mg
             more_ahead = ahead.behind > 0;
             if (!more_ahead) return;
             ahead = part_of(ahead.b + 1, 0, ahead.behind);
-            akb = ahead.k0 + H * kPagedStep * wv;
+            akb = ahead.k0 + kPagedStep * wv;
         };
-        // the slot of key akb + 32 h + lane % 32, or -1
-        auto slot_of = [&](int h) {
-            const int key = akb + kPagedStep * h + (lane & 31);
+        // the slot of key akb + lane % 32, or -1
+        auto slot_of = [&]() {
+            const int key = akb + (lane & 31);
             if (!more_ahead || key < ahead.klo || key >= ahead.khi) return -1;
             const int page = a.table[ahead.b * a.ldt + (key >> a.sh)];
             return page >= 0 && page < a.num_pages ? (page << a.sh) + (key & psm) : -1;
         };
-        Vec<uint32_t, 4> stk[H][NLD], stv[H][NLD];
-        Vec<uint16_t, KB> sts[H]; // scales of key lane % 32: K's in the lower half of the wave, V's in the upper
-        auto stage = [&](int h, int slot, uint32_t seen) {
+        Vec<uint32_t, 4> stk[NLD], stv[NLD];
+        Vec<uint16_t, KB> sts; // scales of key lane % 32: K's in the lower half of the wave, V's in the upper
+        auto stage = [&](int slot, uint32_t seen) {
             if constexpr (Q8) {
-                sts[h] = Vec<uint16_t, KB>{};
+                sts = Vec<uint16_t, KB>{};
                 const uint16_t *sc = lane < 32 ? a.kd : a.vd;
                 if (slot >= 0)
-                    sts[h] = *reinterpret_cast<const Vec<uint16_t, KB> *>(sc + (int64_t(slot) * a.nkv + g) * KB);
+                    sts = *reinterpret_cast<const Vec<uint16_t, KB> *>(sc + (int64_t(slot) * a.nkv + g) * KB);
             }
             if (seen == 0xffffffffu && psm + 1 >= RPI) {
 #pragma unroll
@@ -264,185 +285,170 @@ namespace mg
                     int64_t o = __builtin_amdgcn_readlane(slot, RPI * i) * rowb;
                     __asm__("" : "+s"(o)); // the rows' base stays in scalar registers, the lane's offset in one
                     const char *kp = kg + o, *vp = vg + o;
-                    stk[h][i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(kp + lane_off));
-                    stv[h][i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(vp + lane_off));
+                    stk[i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(kp + lane_off));
+                    stv[i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(vp + lane_off));
                 }
                 return;
             }
 #pragma unroll
             for (int i = 0; i < NLD; ++i) {
                 const int s = __shfl(slot, pr + RPI * i, 64);
-                stk[h][i] = Vec<uint32_t, 4>{{0u, 0u, 0u, 0u}};
-                stv[h][i] = stk[h][i];
+                stk[i] = Vec<uint32_t, 4>{{0u, 0u, 0u, 0u}};
+                stv[i] = stk[i];
                 if (s >= 0) {
                     const int64_t o = s * rowb + 16 * pc;
-                    stk[h][i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(kg + o));
-                    stv[h][i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(vg + o));
+                    stk[i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(kg + o));
+                    stv[i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(vg + o));
                 }
             }
         };
-        int slot[H];
-        uint32_t seen[H]; // keys of the staged halves, one bit each
-#pragma unroll
-        for (int h = 0; h < H; ++h) slot[h] = slot_of(h);
-#pragma unroll
-        for (int h = 0; h < H; ++h) {
-            seen[h] = uint32_t(__builtin_amdgcn_ballot_w64(slot[h] >= 0));
-            stage(h, slot[h], seen[h]);
-        }
+        int slot = slot_of();
+        uint32_t seen = uint32_t(__builtin_amdgcn_ballot_w64(slot >= 0)); // keys of the staged step, one bit each
+        stage(slot, seen);
         advance();
-#pragma unroll
-        for (int h = 0; h < H; ++h) slot[h] = slot_of(h);
+        slot = slot_of();
 
         for (;;) {
             // B of S^T: lane (head n, c) holds q[n][32 kb + 8c ..], zero for padding heads
-            x8 qop[NQ][KB];
+            typename MS::x8 qop[KB];
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
+            for (int i = 0; i < KB; ++i) {
                 const uint16_t *qp =
-                    static_cast<const uint16_t *>(a.q) + cur.b * a.ldq + int64_t(h0 + n) * D + 32 * kb + 8 * c;
-                if constexpr (NQ == 1) {
-                    qop[0][kb] = n < a.hw ? ld_x8<x8>(qp) : x8{};
-                } else {
-                    const f16x8 x = n < a.hw ? ld_x8<f16x8>(qp) : f16x8{};
-                    x8 *const parts[2] = {&qop[0][kb], &qop[1][kb]};
-#pragma unroll
-                    for (int e = 0; e < 8; e += 2) split_weights<M, 2>(float(x[e]), float(x[e + 1]), parts, e);
-                }
+                    static_cast<const uint16_t *>(a.q) + cur.b * a.ldq + int64_t(h0 + n) * D + 32 * i + 8 * c;
+                qop[i] = n < a.hw ? ld_x8<typename MS::x8>(qp) : typename MS::x8{};
             }
             f32x4 o[NT];
 #pragma unroll
             for (int t = 0; t < NT; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             float m = kLow, l = 0.0f; // head n (replicated over c)
-            int kb = cur.k0 + H * kPagedStep * wv;
+            int kb = cur.k0 + kPagedStep * wv;
             bool more;
             do {
                 kb += U;
                 more = kb < cur.khi;
-                const bool any = more_ahead;
+                const uint32_t now = seen;
+                if (now != 0) {
 #pragma unroll
-                for (int h = 0; h < H; ++h) {
-                    const uint32_t now = seen[h];
-                    if (now != 0) {
-#pragma unroll
-                        for (int i = 0; i < NLD; ++i) {
-                            const int key = pr + RPI * i;
-                            if constexpr (Q8) {
-                                q8_bf16(stk[h][i], sk + key * SK + 16 * pc);
-                                q8_bf16(stv[h][i], sv + key * SV + 16 * pc);
-                            } else {
-                                *reinterpret_cast<Vec<uint32_t, 4> *>(sk + key * SK + 8 * pc) = stk[h][i];
-                                *reinterpret_cast<Vec<uint32_t, 4> *>(sv + key * SV + 8 * pc) = stv[h][i];
-                            }
-                        }
-                        if constexpr (Q8)
-#pragma unroll
-                            for (int i = 0; i < KB; ++i) scl[wv][lane >> 5][i][lane & 31] = f16_f32(sts[h].v[i]);
-                        wave_lds_sync();
+                    for (int i = 0; i < NLD; ++i) {
+                        const int key = pr + RPI * i;
+                        *reinterpret_cast<Vec<uint32_t, 4> *>(sk + key * SK + 16 * pc) = stk[i];
+                        *reinterpret_cast<Vec<uint32_t, 4> *>(sv + key * SV + 16 * pc) = stv[i];
                     }
-                    // the next step's rows and the table entries of the one behind it are requested now
-                    if (any) {
-                        seen[h] = uint32_t(__builtin_amdgcn_ballot_w64(slot[h] >= 0));
-                        stage(h, slot[h], seen[h]);
-                        if (h == H - 1) {
-                            advance();
+                    if constexpr (Q8)
 #pragma unroll
-                            for (int i = 0; i < H; ++i) slot[i] = slot_of(i);
-                        }
-                    }
-                    if (now == 0) continue;
-                    // K as A of S^T: lane (key n, c) holds dims 32 i + 8c.. of key 16 t + n
-                    x8 kt[2][KB];
-#pragma unroll
-                    for (int t = 0; t < 2; ++t)
-#pragma unroll
-                        for (int i = 0; i < KB; ++i) kt[t][i] = ld_x8<x8>(sk + (16 * t + n) * SK + 32 * i + 8 * c);
-                    // scores of keys 16 t + 4c + r for head n
-                    float sc[2][4], mx = kLow;
-#pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        f32x4 st = {0.0f, 0.0f, 0.0f, 0.0f};
-                        if constexpr (Q8) {
-#pragma unroll
-                            for (int i = 0; i < KB; ++i) {
-                                f32x4 part = M::mma(kt[t][i], qop[0][i], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-                                if constexpr (NQ == 2) part = M::mma(kt[t][i], qop[1][i], part);
-                                const Vec<float, 4> d =
-                                    *reinterpret_cast<const Vec<float, 4> *>(scl[wv][0][i] + 16 * t + 4 * c);
-#pragma unroll
-                                for (int r = 0; r < 4; ++r) st[r] = __builtin_fmaf(d.v[r], part[r], st[r]);
-                            }
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < KB; ++i) st = M::mma(kt[t][i], qop[0][i], st);
-                        }
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) sc[t][r] = st[r] * a.scale2;
-                        if (now != 0xffffffffu) {
-                            const uint32_t bits = now >> (16 * t + 4 * c);
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) sc[t][r] = (bits >> r & 1) != 0 ? sc[t][r] : kLow;
-                        }
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) mx = __builtin_fmaxf(mx, sc[t][r]);
-                    }
-                    mx = rows4_max(mx);
-                    const float mn = __builtin_fmaxf(m, mx);
-                    // no score above -inf yet: a zero reference, so that -inf scores weigh 0
-                    // and only NaN ones reach the sum
-                    const float mref = mn == kLow ? 0.0f : mn;
-                    // weights: element 4t + r of lane (head n, c) is key 16 t + 4c + r
-                    float p[8];
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(sc[e >> 2][e & 3] - (mref - M::up));
-                    if (__builtin_amdgcn_ballot_w64(mn != m) != 0) {
-                        // some head's running max moved: rescale its sum and its O row
-                        // (rows are heads 4c + r; their factors come from lanes 4c + r)
-                        const float corr = __builtin_amdgcn_exp2f(m - mref); // first step: 2^-inf = 0
-                        l *= corr;
-                        float cr[4];
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) cr[r] = __shfl(corr, 4 * c + r, 64);
-#pragma unroll
-                        for (int t = 0; t < NT; ++t)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) o[t][r] *= cr[r];
-                    }
-                    m = mn;
-                    l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-                    // V as B of P V: lane (dim n, c) needs keys 4c + r and 16 + 4c + r
-                    // of dim 16 s + n, through the transposing read
-                    const uint16_t *vr = sv + (4 * c + (n >> 2)) * SV + 4 * (n & 3);
-                    x8 w[NP];
-                    x8 *parts[NP];
-#pragma unroll
-                    for (int k = 0; k < NP; ++k) parts[k] = &w[k];
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        if constexpr (Q8) {
-                            if (t % 2 == 0) {
-                                const float *d = scl[wv][1][t / 2] + 4 * c;
-                                const Vec<float, 4> d0 = *reinterpret_cast<const Vec<float, 4> *>(d);
-                                const Vec<float, 4> d1 = *reinterpret_cast<const Vec<float, 4> *>(d + 16);
-#pragma unroll
-                                for (int e = 0; e < 4; e += 2) {
-                                    split_weights<M, NP>(p[e] * d0.v[e], p[e + 1] * d0.v[e + 1], parts, e);
-                                    split_weights<M, NP>(p[4 + e] * d1.v[e], p[5 + e] * d1.v[e + 1], parts, 4 + e);
-                                }
-                            }
-                        } else if (t == 0) {
-#pragma unroll
-                            for (int e = 0; e < 8; e += 2) split_weights<M, NP>(p[e], p[e + 1], parts, e);
-                        }
-                        const bf16x4 v0 = lds_read_tr(vr + 16 * t);
-                        const bf16x4 v1 = lds_read_tr(vr + 16 * SV + 16 * t);
-                        const x8 vb =
-                            __builtin_bit_cast(x8, bf16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
-#pragma unroll
-                        for (int k = 0; k < NP; ++k) o[t] = M::mma(w[k], vb, o[t]);
-                    }
-                    wave_lds_sync(); // this half's reads are done before the next one's writes
+                        for (int i = 0; i < KB; ++i) scl[wv][lane >> 5][i][lane & 31] = f16_f32(sts.v[i]);
+                    wave_lds_sync();
                 }
+                // the next step's rows and the table entries of the one behind it are requested now
+                if (more_ahead) {
+                    seen = uint32_t(__builtin_amdgcn_ballot_w64(slot >= 0));
+                    stage(slot, seen);
+                    advance();
+                    slot = slot_of();
+                }
+                if (now == 0) continue;
+                // K as A of S^T: lane (key n, c) holds dims 32 i + 8c.. of key 16 t + n
+                Vec<uint32_t, EPL == 16 ? 2 : 4> kt[2][KB];
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < KB; ++i)
+                        kt[t][i] = *reinterpret_cast<const decltype(&kt[0][0])>(sk + (16 * t + n) * SK +
+                                                                                (32 * i + 8 * c) * (16 / EPL));
+                // scores of keys 16 t + 4c + r for head n
+                float sc[2][4], mx = kLow;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    f32x4 st = {0.0f, 0.0f, 0.0f, 0.0f};
+                    if constexpr (Q8) {
+#pragma unroll
+                        for (int i = 0; i < KB; ++i) {
+                            typename MS::x8 k;
+                            if constexpr (S::dt == BF16)
+                                k = q8_bf16(kt[t][i]);
+                            else
+                                k = q8_f16(kt[t][i]);
+                            const f32x4 part = MS::mma(k, qop[i], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                            const Vec<float, 4> d =
+                                *reinterpret_cast<const Vec<float, 4> *>(scl[wv][0][i] + 16 * t + 4 * c);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) st[r] = __builtin_fmaf(d.v[r], part[r], st[r]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < KB; ++i) st = MS::mma(__builtin_bit_cast(x8, kt[t][i]), qop[i], st);
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) sc[t][r] = st[r] * a.scale2;
+                    if (now != 0xffffffffu) {
+                        const uint32_t bits = now >> (16 * t + 4 * c);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) sc[t][r] = (bits >> r & 1) != 0 ? sc[t][r] : kLow;
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) mx = __builtin_fmaxf(mx, sc[t][r]);
+                }
+                mx = rows4_max(mx);
+                const float mn = __builtin_fmaxf(m, mx);
+                // no score above -inf yet: a zero reference, so that -inf scores weigh 0
+                // and only NaN ones reach the sum
+                const float mref = mn == kLow ? 0.0f : mn;
+                // weights: element 4t + r of lane (head n, c) is key 16 t + 4c + r
+                float p[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(sc[e >> 2][e & 3] - (mref - M::up));
+                if (__builtin_amdgcn_ballot_w64(mn != m) != 0) {
+                    // some head's running max moved: rescale its sum and its O row
+                    // (rows are heads 4c + r; their factors come from lanes 4c + r)
+                    const float corr = __builtin_amdgcn_exp2f(m - mref); // first step: 2^-inf = 0
+                    l *= corr;
+                    float cr[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) cr[r] = __shfl(corr, 4 * c + r, 64);
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[t][r] *= cr[r];
+                }
+                m = mn;
+                l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                // V as B of P V: lane (dim n, c) needs keys 4c + r and 16 + 4c + r
+                // of dim 16 s + n, through the transposing read
+                const char *vr = Q8 ? sv + (16 * (n >> 3) + 4 * c + (n >> 1 & 3)) * SV + 8 * (n & 1)
+                                    : sv + (4 * c + (n >> 2)) * SV + 8 * (n & 3);
+                x8 w[NP];
+                x8 *parts[NP];
+#pragma unroll
+                for (int k = 0; k < NP; ++k) parts[k] = &w[k];
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    if constexpr (Q8) {
+                        if (t % 2 == 0) {
+                            const float *d = scl[wv][1][t / 2] + 4 * c;
+                            const Vec<float, 4> d0 = *reinterpret_cast<const Vec<float, 4> *>(d);
+                            const Vec<float, 4> d1 = *reinterpret_cast<const Vec<float, 4> *>(d + 16);
+#pragma unroll
+                            for (int e = 0; e < 4; e += 2) {
+                                split_weights<M, NP>(p[e] * d0.v[e], p[e + 1] * d0.v[e + 1], parts, e);
+                                split_weights<M, NP>(p[4 + e] * d1.v[e], p[5 + e] * d1.v[e + 1], parts, 4 + e);
+                            }
+                        }
+                    } else if (t == 0) {
+#pragma unroll
+                        for (int e = 0; e < 8; e += 2) split_weights<M, NP>(p[e], p[e + 1], parts, e);
+                    }
+                    x8 vb;
+                    if constexpr (Q8) {
+                        vb = q8_bf16(lds_read_tr8(vr + 16 * t));
+                    } else {
+                        const bf16x4 v0 = lds_read_tr(reinterpret_cast<const uint16_t *>(vr + 32 * t));
+                        const bf16x4 v1 = lds_read_tr(reinterpret_cast<const uint16_t *>(vr + 16 * SV + 32 * t));
+                        vb = __builtin_bit_cast(x8, bf16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
+                    }
+#pragma unroll
+                    for (int k = 0; k < NP; ++k) o[t] = M::mma(w[k], vb, o[t]);
+                }
+                wave_lds_sync(); // this step's reads are done before the next one's writes
             } while (more);
 
             // join the four waves: their outputs take the place of K and V in LDS
@@ -604,12 +610,10 @@ namespace mg
         const int64_t vh = nkv * (hpg / hw);
         // as many teams as the chip holds at once (the work-groups that a CU's LDS and registers
         // take), not more than there can be units, nor than the workspace has room for
-        const int per_cu = D == 128 ? 2 : kd ? 3 : 4;
-        const int unit = 4 * kPagedStep * (kd ? 2 : 1);
+        const int per_cu = kd ? 3 : D == 128 ? 2 : 4;
         const int64_t span = window > 0 && window < max_pages << sh ? window + kPagedStep : max_pages << sh;
-        const int64_t most = seqs * (span / unit + 1);
-        need(most < (int64_t(1) << 31), "attn_decode_paged: the table must stand for fewer than 2^31 units of " +
-                                            std::to_string(unit) + " keys");
+        const int64_t most = seqs * (span / kPagedUnit + 1);
+        need(most < (int64_t(1) << 31), "attn_decode_paged: the table must stand for fewer than 2^38 keys");
         int64_t teams = per_cu * int64_t(c->num_cus) / vh;
         teams = teams < most ? teams : most;
         // (the cuts, then the partial results' outputs, then their maxima and sums)

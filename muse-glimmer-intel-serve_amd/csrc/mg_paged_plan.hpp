@@ -1,9 +1,9 @@
 // How decode attention over a paged cache divides its keys among work-groups:
 // plain arithmetic, the same on the host (its checker) and on the device.
 //
-// A request's attended keys [lo, n) are cut into units of 128 or 256 keys from
-// `base`, lo rounded down to a step of 32 (a request without keys has one empty
-// unit, so that somebody writes its zeros). The units of all requests form one line
+// A request's attended keys [lo, n) are cut into units of 128 keys from `base`,
+// lo rounded down to a step of 32 (a request without keys has one empty unit,
+// so that somebody writes its zeros). The units of all requests form one line
 // of T; it is cut into `teams` equal runs, whatever requests they cross, and
 // each team has a work-group for every group of query heads. A request inside
 // one team is finished there; one that a team's edge cuts leaves a partial
@@ -21,21 +21,22 @@
 
 namespace mg
 {
-    constexpr int kPagedStep = 32; // keys a wave takes at once
+    constexpr int kPagedStep = 32;  // keys a wave takes at once
+    constexpr int kPagedUnit = 128; // a step of each of a work-group's four waves
 
     struct PagedSpan
     {
         int lo, n, base, units;
     };
 
-    // `cap`: the tokens a table row can hold; `unit`: keys that a work-group's four waves take in a turn
-    MG_HD PagedSpan paged_span(int len, int cap, int64_t window, int unit)
+    // `cap`: the tokens a table row can hold
+    MG_HD PagedSpan paged_span(int len, int cap, int64_t window)
     {
         PagedSpan s;
         s.n = len < 0 ? 0 : len > cap ? cap : len;
         s.lo = window > 0 && s.n > window ? int(s.n - window) : 0;
         s.base = s.lo / kPagedStep * kPagedStep;
-        const int u = (s.n - s.base) / unit + ((s.n - s.base) % unit != 0);
+        const int u = (s.n - s.base) / kPagedUnit + ((s.n - s.base) % kPagedUnit != 0);
         s.units = u > 0 ? u : 1;
         return s;
     }

@@ -27,19 +27,18 @@ int main()
         const int R = 1 + int(upto(batch % 3 ? 12 : 300));
         const int cap = 1 << (batch % 5 == 0 ? (batch % 3 ? 30 : 24) : 5 + upto(12));
         const int64_t window = batch % 2 ? 0 : 1 + upto(2000);
-        const int unit = batch % 4 < 2 ? 128 : 256;
         const int teams_asked = 1 + int(upto(batch % 7 ? 80 : 600));
         std::vector<PagedSpan> sp(R);
         std::vector<int64_t> first(R + 1, 0);
         for (int b = 0; b < R; ++b) {
             const int64_t pick = upto(5);
             const int len = pick == 0 ? 0 : pick == 1 ? -5 : pick == 2 ? cap : pick == 3 ? int(upto(300)) : int(upto(cap));
-            const PagedSpan s = sp[b] = paged_span(len, cap, window, unit);
+            const PagedSpan s = sp[b] = paged_span(len, cap, window);
             CHECK(s.n == (len < 0 ? 0 : len > cap ? cap : len));
             CHECK(s.lo == (window > 0 && s.n > window ? s.n - window : 0));
             CHECK(s.base % kPagedStep == 0 && s.base <= s.lo && s.lo - s.base < kPagedStep);
-            CHECK(s.units >= 1 && int64_t(s.base) + int64_t(s.units) * unit >= s.n);
-            CHECK(s.units == 1 || int64_t(s.base) + int64_t(s.units - 1) * unit < s.n);
+            CHECK(s.units >= 1 && int64_t(s.base) + int64_t(s.units) * kPagedUnit >= s.n);
+            CHECK(s.units == 1 || int64_t(s.base) + int64_t(s.units - 1) * kPagedUnit < s.n);
             first[b + 1] = first[b] + s.units;
         }
         CHECK(first[R] < (int64_t(1) << 31));
