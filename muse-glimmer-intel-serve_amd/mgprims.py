@@ -145,6 +145,9 @@ class Prims:
         self._check(self.lib.mg_open(device, ctypes.c_void_p(stream), workspace_bytes, ctypes.byref(h)))
         self.h = h
         self.device = device
+        # what the calls of a decode step look up
+        self._i32, self._i64, self._i8, self._f16 = torch.int32, torch.int64, torch.int8, torch.float16
+        self._codes = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32}
 
     def _check(self, rc):
         if rc != 0:
@@ -389,48 +392,67 @@ class Prims:
         return out
 
     # ------------------------------------------------------ paged KV cache
-    @staticmethod
-    def _ints(name, dtype, n, *ts):
-        """contiguous integer tensors of n elements (None: skipped)"""
+    # These run once or more a layer in a decode step, where the host's time counts: their
+    # checks read each property of a tensor once, and addresses go to the library as integers.
+    def _here(self, *ts):
         for t in ts:
-            if t is not None and (t.dtype != dtype or t.numel() != n or not t.is_contiguous()):
-                raise MgError(f"{name}: expected a contiguous {dtype} tensor of {n}, got {t.dtype} {tuple(t.shape)}")
+            if t is not None and t.get_device() != self.device:
+                raise MgError(f"tensor on {t.device}, context on cuda:{self.device}")
+
+    @staticmethod
+    def _ints(name, dtype, n, t):
+        """address of a contiguous integer tensor of n elements (None: NULL)"""
+        if t is None:
+            return None
+        if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+            raise MgError(f"{name}: expected a contiguous {dtype} tensor of {n}, got {t.dtype} {tuple(t.shape)}")
+        return t.data_ptr()
 
     def _page_table(self, name, t, requests):
-        import torch
-        if t.dim() != 2 or t.dtype != torch.int32 or t.shape[0] != requests:
-            raise MgError(f"{name}: page_table must be int32 [{requests}, max_pages], got {t.dtype} {tuple(t.shape)}")
-        if t.stride(1) != 1 and t.shape[1] > 1 or requests > 1 and t.stride(0) < t.shape[1]:
+        """(row stride, pages a row) of an int32 [requests, max_pages] table"""
+        shape = t.shape
+        if len(shape) != 2 or t.dtype != self._i32 or shape[0] != requests:
+            raise MgError(f"{name}: page_table must be int32 [{requests}, max_pages], got {t.dtype} {tuple(shape)}")
+        ld, inner = t.stride()
+        if inner != 1 and shape[1] > 1 or requests > 1 and ld < shape[1]:
             raise MgError(f"{name}: page_table rows must have unit inner stride and not overlap")
-        return t.stride(0) if requests > 1 else t.shape[1]
+        return (ld if requests > 1 else shape[1]), shape[1]
 
     def _token_rows(self, name, t):
-        """_heads for 16-bit or f32 rows whose tokens do not overlap; returns the token stride"""
-        import torch
-        if t.dtype not in (torch.bfloat16, torch.float16, torch.float32):
-            raise MgError(f"{name}: dtype {t.dtype} is not taken")
-        ld = self._heads(name, t)
-        if t.shape[0] > 1 and ld < t.shape[1] * t.shape[2]:
+        """(shape, token stride, dtype code) of 16-bit or f32 rows [T, heads, D], each token's heads
+        contiguous, tokens not overlapping"""
+        shape, code = t.shape, self._codes.get(t.dtype)
+        if code is None or len(shape) != 3:
+            raise MgError(f"{name}: expected [T, heads, D] of a 16-bit or f32 dtype, got {t.dtype} {tuple(shape)}")
+        n = shape[1] * shape[2]
+        ld, head, inner = t.stride()
+        if inner != 1 and shape[2] > 1 or head != shape[2] and shape[1] > 1:
+            raise MgError(f"{name}: expected [T, heads, D] with each token's heads contiguous")
+        if shape[0] > 1 and ld < n:
             raise MgError(f"{name}: rows of consecutive tokens overlap")
-        return ld if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+        return shape, (ld if shape[0] > 1 else n), code
 
     def _pool(self, name, k_cache, v_cache, k_scale, v_scale, dtype, heads, dim):
-        """checks a pool [num_pages, page_size, Hk, D] at dtype, or int8 with f16 scales [.., D / 32]"""
-        import torch
-        if k_cache.dim() != 4 or tuple(k_cache.shape[2:]) != (heads, dim):
-            raise MgError(f"{name}: caches must be [num_pages, page_size, {heads}, {dim}], got {tuple(k_cache.shape)}")
-        self._same(name, k_cache, v_cache, "shape")
-        self._contig(name, k_cache, v_cache, k_scale, v_scale)
+        """shape of a pool [num_pages, page_size, Hk, D] at dtype, or int8 with f16 scales [.., D / 32]
+        (heads None: any number)"""
+        shape = k_cache.shape
+        if len(shape) != 4 or shape[3] != dim or heads is not None and shape[2] != heads:
+            raise MgError(f"{name}: caches must be [num_pages, page_size, {heads or 'heads'}, {dim}], got {tuple(shape)}")
+        if v_cache.shape != shape:
+            raise MgError(f"{name}: shape {tuple(shape)} and {tuple(v_cache.shape)} differ")
+        if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+            raise MgError(f"{name}: caches must be contiguous")
         if (k_scale is None) != (v_scale is None):
             raise MgError(f"{name}: give both k_scale and v_scale, or neither")
-        want = dtype if k_scale is None else torch.int8
+        want = dtype if k_scale is None else self._i8
         if k_cache.dtype != want or v_cache.dtype != want:
             raise MgError(f"{name}: caches of {k_cache.dtype} and {v_cache.dtype}, {want} needed")
         if k_scale is not None:
-            shape = (*k_cache.shape[:3], dim // 32)
+            want = (*shape[:3], dim // 32)
             for t in (k_scale, v_scale):
-                if t.dtype != torch.float16 or tuple(t.shape) != shape:
-                    raise MgError(f"{name}: scales must be float16 {shape}, got {t.dtype} {tuple(t.shape)}")
+                if t.dtype != self._f16 or t.shape != want or not t.is_contiguous():
+                    raise MgError(f"{name}: scales must be contiguous float16 {want}, got {t.dtype} {tuple(t.shape)}")
+        return shape
 
     def kv_pages(self, page_table, old_lens, new_lens, page_size, free_ring, ends, lens, ends_out, starts=None,
                  slot_map=None, positions=None):
@@ -440,21 +462,16 @@ class Prims:
         modulo num_pages); page_table [R, W] int32 is updated in place. Writes lens [R] (may be old_lens
         or new_lens), ends_out [2] (may be ends), starts [R + 1] int32, and slot_map and positions
         [tokens] int64 of the step's new tokens, -1 behind the last and for refused requests."""
-        import torch
-        R = old_lens.numel()
-        T = 0 if slot_map is None else slot_map.numel()
-        if slot_map is None and positions is not None:
-            T = positions.numel()
-        self._dev(page_table, old_lens, new_lens, free_ring, ends, lens, ends_out, starts, slot_map, positions)
-        ldt = self._page_table("kv_pages", page_table, R)
-        self._ints("kv_pages", torch.int32, R, old_lens, new_lens, lens)
-        self._ints("kv_pages", torch.int32, R + 1, starts)
-        self._ints("kv_pages", torch.int32, free_ring.numel(), free_ring)
-        self._ints("kv_pages", torch.int64, 2, ends, ends_out)
-        self._ints("kv_pages", torch.int64, T, slot_map, positions)
-        self._check(self.lib.mg_kv_pages(self.h, _ptr(page_table), ldt, R, page_table.shape[1], _ptr(old_lens),
-                                         _ptr(new_lens), page_size, _ptr(free_ring), free_ring.numel(), _ptr(ends),
-                                         _ptr(lens), _ptr(ends_out), _ptr(starts), _ptr(slot_map), _ptr(positions), T))
+        name, i32, i64, ints = "kv_pages", self._i32, self._i64, self._ints
+        R, N = old_lens.numel(), free_ring.numel()
+        T = slot_map.numel() if slot_map is not None else positions.numel() if positions is not None else 0
+        self._here(page_table, old_lens, new_lens, free_ring, ends, lens, ends_out, starts, slot_map, positions)
+        ldt, W = self._page_table(name, page_table, R)
+        self._check(self.lib.mg_kv_pages(
+            self.h, page_table.data_ptr(), ldt, R, W, ints(name, i32, R, old_lens), ints(name, i32, R, new_lens), page_size,
+            ints(name, i32, N, free_ring), N, ints(name, i64, 2, ends), ints(name, i32, R, lens),
+            ints(name, i64, 2, ends_out), ints(name, i32, R + 1, starts), ints(name, i64, T, slot_map),
+            ints(name, i64, T, positions), T))
 
     def qk_norm_rope_paged(self, q, k, v, eps, qk_scale, cos, sin, positions, slot_map, k_cache, v_cache,
                            k_scale=None, v_scale=None):
@@ -462,23 +479,28 @@ class Prims:
         to slot slot_map[t] of the pool k_cache / v_cache [num_pages, page_size, Hk, D] (a slot outside it:
         nowhere), at q's dtype or, with k_scale / v_scale [num_pages, page_size, Hk, D / 32] f16, as int8
         Q8_0. positions [T] pick the rows of cos / sin (None: no rotation)."""
-        import torch
-        name = "qk_norm_rope_paged"
-        self._dev(q, k, v, k_cache, v_cache, k_scale, v_scale, slot_map, positions)
-        ldq, ldk, ldv = (self._token_rows(name, t) for t in (q, k, v))
-        T, qh, D = q.shape
-        kh = k.shape[1]
-        for t in (k, v):
-            self._same(name, q, t)
-            if tuple(t.shape) != (T, kh, D):
-                raise MgError(f"{name}: k and v must be [{T}, {kh}, {D}], got {tuple(t.shape)}")
-        self._ints(name, torch.int64, T, positions, slot_map)
-        self._table(name, q, cos, sin, positions)
-        self._pool(name, k_cache, v_cache, k_scale, v_scale, q.dtype, kh, D)
+        name, dtype = "qk_norm_rope_paged", q.dtype
+        self._here(q, k, v, k_cache, v_cache, slot_map, positions, cos, sin, k_scale, v_scale)
+        (T, qh, D), ldq, code = self._token_rows(name, q)
+        kshape, ldk, _ = self._token_rows(name, k)
+        vshape, ldv, _ = self._token_rows(name, v)
+        if kshape != vshape or kshape[0] != T or kshape[2] != D or k.dtype != dtype or v.dtype != dtype:
+            raise MgError(f"{name}: k and v must be {dtype} [{T}, kv heads, {D}], got {k.dtype} {tuple(kshape)} and "
+                          f"{v.dtype} {tuple(vshape)}")
+        kh = kshape[1]
+        pages, page_size, _, _ = self._pool(name, k_cache, v_cache, k_scale, v_scale, dtype, kh, D)
+        rows = 0
+        if cos is not None or sin is not None:
+            if cos is None or sin is None or cos.dtype != dtype or sin.dtype != dtype or cos.shape != sin.shape or \
+                    cos.dim() != 2 or cos.shape[1] != D // 2 or not (cos.is_contiguous() and sin.is_contiguous()):
+                raise MgError(f"{name}: cos and sin must be contiguous {dtype} [positions, {D // 2}], or both None")
+            rows = cos.shape[0]
         self._check(self.lib.mg_qk_norm_rope_paged(
-            self.h, _ptr(q), qh, ldq, _ptr(k), kh, ldk, _ptr(v), ldv, T, D, eps, qk_scale, _ptr(cos), _ptr(sin),
-            cos.shape[0] if cos is not None else 0, _ptr(positions), _ptr(slot_map), _ptr(k_cache), _ptr(v_cache),
-            _ptr(k_scale), _ptr(v_scale), k_cache.shape[0] * k_cache.shape[1], _dtype_code(q)))
+            self.h, q.data_ptr(), qh, ldq, k.data_ptr(), kh, ldk, v.data_ptr(), ldv, T, D, eps, qk_scale,
+            cos.data_ptr() if rows else None, sin.data_ptr() if rows else None, rows,
+            self._ints(name, self._i64, T, positions), self._ints(name, self._i64, T, slot_map), k_cache.data_ptr(),
+            v_cache.data_ptr(), None if k_scale is None else k_scale.data_ptr(),
+            None if v_scale is None else v_scale.data_ptr(), pages * page_size, code))
 
     def attn_decode_paged(self, q, k_cache, v_cache, page_table, lens, scaling, window=0, k_scale=None, v_scale=None,
                           out=None):
@@ -486,23 +508,23 @@ class Prims:
         q [R, Hq, D] bf16 or f16; pool [num_pages, page_size, Hk, D] at q's dtype, or int8 Q8_0 with scales
         [.., D / 32] f16; page_table [R, W] int32, lens [R] int32 keys of each (the new token's among them)
         -> out [R, Hq, D], float32 (default) or q's dtype. A request without keys gives zeros."""
-        import torch
         name = "attn_decode_paged"
-        ldq = self._token_rows(name, q)
-        R, hq, D = q.shape
         if out is None:
-            out = torch.empty((R, hq, D), dtype=torch.float32, device=q.device)
-        self._dev(q, k_cache, v_cache, k_scale, v_scale, page_table, lens, out)
-        ldo = self._token_rows(name, out)
-        self._same(name, q, out, "shape")
-        self._pool(name, k_cache, v_cache, k_scale, v_scale, q.dtype, k_cache.shape[2] if k_cache.dim() == 4 else 0, D)
-        ldt = self._page_table(name, page_table, R)
-        self._ints(name, torch.int32, R, lens)
-        num_pages, page_size, hk, _ = k_cache.shape
+            import torch
+            out = torch.empty(q.shape, dtype=torch.float32, device=q.device)
+        self._here(q, k_cache, v_cache, page_table, lens, out, k_scale, v_scale)
+        shape, ldq, code = self._token_rows(name, q)
+        oshape, ldo, ocode = self._token_rows(name, out)
+        if oshape != shape:
+            raise MgError(f"{name}: shape {tuple(shape)} and {tuple(oshape)} differ")
+        R, hq, D = shape
+        pages, page_size, hk, _ = self._pool(name, k_cache, v_cache, k_scale, v_scale, q.dtype, None, D)
+        ldt, W = self._page_table(name, page_table, R)
         self._check(self.lib.mg_attn_decode_paged(
-            self.h, _ptr(q), ldq, _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(page_table), ldt,
-            page_table.shape[1], _ptr(lens), R, hq, hk, D, page_size, num_pages, window, scaling, _ptr(out), ldo,
-            _dtype_code(q), _dtype_code(out)))
+            self.h, q.data_ptr(), ldq, k_cache.data_ptr(), v_cache.data_ptr(),
+            None if k_scale is None else k_scale.data_ptr(), None if v_scale is None else v_scale.data_ptr(),
+            page_table.data_ptr(), ldt, W, self._ints(name, self._i32, R, lens), R, hq, hk, D, page_size, pages, window,
+            scaling, out.data_ptr(), ldo, code, ocode))
         return out
 
     # ------------------------------------------------------------ softmax
