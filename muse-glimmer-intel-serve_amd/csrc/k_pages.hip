@@ -24,8 +24,9 @@
 // page given back) then finds its request by bisection there. A step with few
 // tokens ends in that launch. One with more leaves the sums in the workspace and
 // a second launch of many work-groups, each with the sums in its own LDS, does
-// the items. Two launches cost what about kPagesAlone tokens cost one
-// work-group.
+// the items. Measured, us a call (64 requests): 2191 tokens 8.1 in one launch, 11.0
+// in two; 4344 10.0 and 11.0; 8803 15.0 and 11.4; 17570 25.2 and 10.7. Latency bounds
+// both: a launch, then chains of a bisection and two or three dependent loads.
 #include "mg_device.hpp"
 #include "mg_internal.hpp"
 

@@ -303,29 +303,31 @@ namespace mg
         const bool isq = hh < a.nq;
         raw *x = isq ? q + t * a.ldq + int64_t(hh) * D : k + t * a.ldk + int64_t(hh - a.nq) * D;
         const int c0 = NH * j; // the lane's first column of each half
+        // the token's position and slot first: the table's rows wait for them
+        const int64_t p = pos ? pos[t] : a.pos0 + t;
+        int64_t slot = -1; // the row's, or -1 where it appends nothing
+        if constexpr (KV != kKvRing) {
+            if (!isq) slot = a.slot_map[t];
+        }
         Vec<raw, VEC> lo[NV], hi[NV];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             lo[i] = ldv<raw, VEC>(x + c0 + VEC * i);
             hi[i] = ldv<raw, VEC>(x + half + c0 + VEC * i);
         }
-        const int64_t p = pos ? pos[t] : a.pos0 + t;
-        // the row's slot, or -1 where it appends nothing
-        int64_t slot = -1;
-        if constexpr (KV == kKvRing) {
-            if (!isq && kc && p >= 0) slot = p < a.slots ? p : p % a.slots;
-        } else if (!isq) {
-            slot = a.slot_map[t];
-            slot = slot < a.slots ? slot : -1;
-        }
         Vec<raw, VEC> vlo[NV], vhi[NV];
-        if (vc && slot >= 0) {
+        if (!isq && vc) {
             const raw *vr = v + t * a.ldv + int64_t(hh - a.nq) * D + c0;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 vlo[i] = ldv<raw, VEC>(vr + VEC * i);
                 vhi[i] = ldv<raw, VEC>(vr + half + VEC * i);
             }
+        }
+        if constexpr (KV == kKvRing) {
+            if (!isq && kc && p >= 0) slot = p < a.slots ? p : p % a.slots;
+        } else {
+            slot = slot < a.slots ? slot : -1;
         }
         const bool rot = co && p >= 0 && p < a.table_rows;
         Vec<raw, VEC> cv[NV], sv[NV];
@@ -399,21 +401,29 @@ namespace mg
             rs = rsf[wv][lane / TPR];
         }
 
-        if constexpr (S::dt == BF16) {
-            // every intermediate is held as the f32 of its bf16 value (one
-            // conversion per rounding) and the last rounding packs two
-            // elements per word. NaN propagates through every step and the
-            // twin's NaN is the one pattern 0x7FC0: the steps round without
-            // NaN checks and a lane whose outputs hold a NaN makes them
+        {
+            // every intermediate is held as the f32 of its stored value (one or two
+            // conversions per rounding) and the last rounding packs two elements per
+            // word. NaN propagates through every step, with its sign, and the twin's
+            // NaN is one pattern (bf16 0x7FC0, f16 0x7E00 and the sign): the steps
+            // round without NaN checks and a lane whose outputs hold a NaN makes them
             // canonical once
+            auto rnd = [](float f) {
+                if constexpr (S::dt == BF16)
+                    return bf_round(f);
+                else
+                    return hf_round(f);
+            };
+            auto lo16 = [](uint32_t w) { return S::dt == BF16 ? bf_lo(w) : f16_f32(uint16_t(w)); };
+            auto hi16 = [](uint32_t w) { return S::dt == BF16 ? bf_hi(w) : f16_f32(uint16_t(w >> 16)); };
             float fl[NH], fh[NH];
 #pragma unroll
             for (int e = 0; e < NH; ++e) {
-                fl[e] = bf_round(float(double(S::dec(lo[e / VEC].v[e % VEC])) * rs));
-                fh[e] = bf_round(float(double(S::dec(hi[e / VEC].v[e % VEC])) * rs));
+                fl[e] = rnd(float(double(S::dec(lo[e / VEC].v[e % VEC])) * rs));
+                fh[e] = rnd(float(double(S::dec(hi[e / VEC].v[e % VEC])) * rs));
                 if (isq) {
-                    fl[e] = bf_round(fl[e] * qs);
-                    fh[e] = bf_round(fh[e] * qs);
+                    fl[e] = rnd(fl[e] * qs);
+                    fh[e] = rnd(fh[e] * qs);
                 }
             }
             if (rot) {
@@ -421,46 +431,37 @@ namespace mg
                 for (int e = 0; e < NH; ++e) {
                     const uint32_t cw = __builtin_bit_cast(W4, cv[e / VEC]).v[(e % VEC) / 2];
                     const uint32_t sw = __builtin_bit_cast(W4, sv[e / VEC]).v[(e % VEC) / 2];
-                    const float cc = e & 1 ? bf_hi(cw) : bf_lo(cw), sn = e & 1 ? bf_hi(sw) : bf_lo(sw);
+                    const float cc = e & 1 ? hi16(cw) : lo16(cw), sn = e & 1 ? hi16(sw) : lo16(sw);
                     const float l = fl[e], h = fh[e];
-                    fl[e] = bf_round(l * cc) + bf_round(-(h * sn)); // rounded by the packing below
-                    fh[e] = bf_round(h * cc) + bf_round(l * sn);
+                    fl[e] = rnd(l * cc) + rnd(-(h * sn)); // rounded by the packing below
+                    fh[e] = rnd(h * cc) + rnd(l * sn);
                 }
             }
             W4 l4[NV], h4[NV];
             uint32_t mag = 0;
 #pragma unroll
             for (int w = 0; w < 4 * NV; ++w) {
-                const uint32_t lw = bf_pack(fl[2 * w], fl[2 * w + 1]), hw = bf_pack(fh[2 * w], fh[2 * w + 1]);
+                uint32_t lw, hw;
+                if constexpr (S::dt == BF16)
+                    lw = bf_pack(fl[2 * w], fl[2 * w + 1]), hw = bf_pack(fh[2 * w], fh[2 * w + 1]);
+                else
+                    lw = hf_pack(fl[2 * w], fl[2 * w + 1]), hw = hf_pack(fh[2 * w], fh[2 * w + 1]);
                 l4[w / 4].v[w % 4] = lw;
                 h4[w / 4].v[w % 4] = hw;
                 mag = pk_max_u16(mag, pk_max_u16(lw & 0x7fff7fffu, hw & 0x7fff7fffu));
             }
-            if (max(mag & 0xffffu, mag >> 16) > 0x7f80u) {
+            if (max(mag & 0xffffu, mag >> 16) > (S::dt == BF16 ? 0x7f80u : 0x7c00u)) {
+                auto canon = [](uint32_t w) { return S::dt == BF16 ? bf_canon(w) : hf_canon(w); };
 #pragma unroll
                 for (int w = 0; w < 4 * NV; ++w) {
-                    l4[w / 4].v[w % 4] = bf_canon(l4[w / 4].v[w % 4]);
-                    h4[w / 4].v[w % 4] = bf_canon(h4[w / 4].v[w % 4]);
+                    l4[w / 4].v[w % 4] = canon(l4[w / 4].v[w % 4]);
+                    h4[w / 4].v[w % 4] = canon(h4[w / 4].v[w % 4]);
                 }
             }
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 lo[i] = __builtin_bit_cast(Vec<raw, VEC>, l4[i]);
                 hi[i] = __builtin_bit_cast(Vec<raw, VEC>, h4[i]);
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < NH; ++e) {
-                raw &lr = lo[e / VEC].v[e % VEC], &hr = hi[e / VEC].v[e % VEC];
-                raw l = S::enc64(double(S::dec(lr)) * rs);
-                raw h = S::enc64(double(S::dec(hr)) * rs);
-                if (isq) {
-                    l = S::enc(S::dec(l) * qs);
-                    h = S::enc(S::dec(h) * qs);
-                }
-                if (rot) rope_pair<S>(l, h, cv[e / VEC].v[e % VEC], sv[e / VEC].v[e % VEC]);
-                lr = l;
-                hr = h;
             }
         }
         if (!live) return;

@@ -295,6 +295,21 @@ namespace mg
         const f2 v = {0.0f, opaque(x)};
         return __builtin_bit_cast(float, __builtin_convertvector(v, h2));
     }
+    // the same for f16: RNE of two values into one word, of one value returned as f32,
+    // and the NaN pattern of f16_bits
+    MG_DEV uint32_t hf_pack(float a, float b)
+    {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        const h2 h = {static_cast<_Float16>(opaque(a)), static_cast<_Float16>(opaque(b))};
+        return __builtin_bit_cast(uint32_t, h);
+    }
+    MG_DEV float hf_round(float x) { return float(static_cast<_Float16>(opaque(x))); }
+    MG_DEV uint32_t hf_canon(uint32_t w)
+    {
+        const uint32_t a = w & 0xffffu, b = w >> 16;
+        return ((a & 0x7fffu) > 0x7c00u ? (a & 0x8000u) | 0x7e00u : a) |
+               ((b & 0x7fffu) > 0x7c00u ? (b & 0x8000u) | 0x7e00u : b) << 16;
+    }
     MG_DEV uint32_t bf_canon(uint32_t w)
     {
         const uint32_t a = w & 0xffffu, b = w >> 16;
