@@ -291,17 +291,19 @@ namespace mg
         __shared__ __align__(16) raw st[4][RPW][D + 8];
         __shared__ double rsf[4][RPW];
         const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
-        const int64_t heads = a.nq + a.nkv, rows = a.T * heads;
+        // q's rows first, then k's: a wave's rows are of one kind (but for one wave), so only k's take the append
+        const int64_t qrows = a.T * a.nq, rows = qrows + a.T * a.nkv;
         const int64_t wrow0 = (int64_t(blockIdx.x) * 256 + wv * 64) / TPR; // the wave's first row
         if (wrow0 >= rows) return; // the whole wave
         const int64_t r = wrow0 + lane / TPR;
         const int j = lane & (TPR - 1);
         const bool live = r < rows;
         const int64_t rc = live ? r : rows - 1; // addresses of a dead lane stay in bounds
-        const int64_t t = rows <= int64_t(0xffffffff) ? int64_t(uint32_t(rc) / uint32_t(heads)) : rc / heads;
-        const int hh = int(rc - t * heads);
-        const bool isq = hh < a.nq;
-        raw *x = isq ? q + t * a.ldq + int64_t(hh) * D : k + t * a.ldk + int64_t(hh - a.nq) * D;
+        const bool isq = rc < qrows;
+        const int64_t rk = isq ? rc : rc - qrows, heads = isq ? a.nq : a.nkv;
+        const int64_t t = rows <= int64_t(0xffffffff) ? int64_t(uint32_t(rk) / uint32_t(heads)) : rk / heads;
+        const int64_t hh = rk - t * heads;
+        raw *x = (isq ? q + t * a.ldq : k + t * a.ldk) + hh * D;
         const int c0 = NH * j; // the lane's first column of each half
         // the token's position and slot first: the table's rows wait for them
         const int64_t p = pos ? pos[t] : a.pos0 + t;
@@ -317,7 +319,7 @@ namespace mg
         }
         Vec<raw, VEC> vlo[NV], vhi[NV];
         if (!isq && vc) {
-            const raw *vr = v + t * a.ldv + int64_t(hh - a.nq) * D + c0;
+            const raw *vr = v + t * a.ldv + hh * D + c0;
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 vlo[i] = ldv<raw, VEC>(vr + VEC * i);
@@ -471,7 +473,7 @@ namespace mg
             stv<raw, VEC>(x + half + c0 + VEC * i, hi[i]);
         }
         if (slot >= 0) {
-            const int64_t o = slot * (a.nkv * D) + int64_t(hh - a.nq) * D + c0;
+            const int64_t o = slot * (a.nkv * D) + hh * D + c0;
             if constexpr (KV == kKvSlotsQ8) {
                 static_assert(NV == 1 && TPR >= 4, "a quad holds a block of 32");
                 int8_t *kq = reinterpret_cast<int8_t *>(kc), *vq = reinterpret_cast<int8_t *>(vc);
