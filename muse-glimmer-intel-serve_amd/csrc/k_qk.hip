@@ -404,54 +404,68 @@ namespace mg
         }
 
         {
-            // every intermediate is held as the f32 of its stored value (one or two
-            // conversions per rounding) and the last rounding packs two elements per
+            // bf16: every intermediate is held as the f32 of its stored value (one
+            // conversion per rounding) and the last rounding packs two elements per
             // word. NaN propagates through every step, with its sign, and the twin's
             // NaN is one pattern (bf16 0x7FC0, f16 0x7E00 and the sign): the steps
             // round without NaN checks and a lane whose outputs hold a NaN makes them
             // canonical once
-            auto rnd = [](float f) {
-                if constexpr (S::dt == BF16)
-                    return bf_round(f);
-                else
-                    return hf_round(f);
-            };
-            auto lo16 = [](uint32_t w) { return S::dt == BF16 ? bf_lo(w) : f16_f32(uint16_t(w)); };
-            auto hi16 = [](uint32_t w) { return S::dt == BF16 ? bf_hi(w) : f16_f32(uint16_t(w >> 16)); };
-            float fl[NH], fh[NH];
-#pragma unroll
-            for (int e = 0; e < NH; ++e) {
-                fl[e] = rnd(float(double(S::dec(lo[e / VEC].v[e % VEC])) * rs));
-                fh[e] = rnd(float(double(S::dec(hi[e / VEC].v[e % VEC])) * rs));
-                if (isq) {
-                    fl[e] = rnd(fl[e] * qs);
-                    fh[e] = rnd(fh[e] * qs);
-                }
-            }
-            if (rot) {
-#pragma unroll
-                for (int e = 0; e < NH; ++e) {
-                    const uint32_t cw = __builtin_bit_cast(W4, cv[e / VEC]).v[(e % VEC) / 2];
-                    const uint32_t sw = __builtin_bit_cast(W4, sv[e / VEC]).v[(e % VEC) / 2];
-                    const float cc = e & 1 ? hi16(cw) : lo16(cw), sn = e & 1 ? hi16(sw) : lo16(sw);
-                    const float l = fl[e], h = fh[e];
-                    fl[e] = rnd(l * cc) + rnd(-(h * sn)); // rounded by the packing below
-                    fh[e] = rnd(h * cc) + rnd(l * sn);
-                }
-            }
             W4 l4[NV], h4[NV];
             uint32_t mag = 0;
+            if constexpr (S::dt == BF16) {
+                float fl[NH], fh[NH];
 #pragma unroll
-            for (int w = 0; w < 4 * NV; ++w) {
-                uint32_t lw, hw;
-                if constexpr (S::dt == BF16)
-                    lw = bf_pack(fl[2 * w], fl[2 * w + 1]), hw = bf_pack(fh[2 * w], fh[2 * w + 1]);
-                else
-                    lw = hf_pack(fl[2 * w], fl[2 * w + 1]), hw = hf_pack(fh[2 * w], fh[2 * w + 1]);
-                l4[w / 4].v[w % 4] = lw;
-                h4[w / 4].v[w % 4] = hw;
-                mag = pk_max_u16(mag, pk_max_u16(lw & 0x7fff7fffu, hw & 0x7fff7fffu));
+                for (int e = 0; e < NH; ++e) {
+                    fl[e] = bf_round(float(double(S::dec(lo[e / VEC].v[e % VEC])) * rs));
+                    fh[e] = bf_round(float(double(S::dec(hi[e / VEC].v[e % VEC])) * rs));
+                    if (isq) {
+                        fl[e] = bf_round(fl[e] * qs);
+                        fh[e] = bf_round(fh[e] * qs);
+                    }
+                }
+                if (rot) {
+#pragma unroll
+                    for (int e = 0; e < NH; ++e) {
+                        const uint32_t cw = __builtin_bit_cast(W4, cv[e / VEC]).v[(e % VEC) / 2];
+                        const uint32_t sw = __builtin_bit_cast(W4, sv[e / VEC]).v[(e % VEC) / 2];
+                        const float cc = e & 1 ? bf_hi(cw) : bf_lo(cw), sn = e & 1 ? bf_hi(sw) : bf_lo(sw);
+                        const float l = fl[e], h = fh[e];
+                        fl[e] = bf_round(l * cc) + bf_round(-(h * sn)); // rounded by the packing below
+                        fh[e] = bf_round(h * cc) + bf_round(l * sn);
+                    }
+                }
+#pragma unroll
+                for (int w = 0; w < 4 * NV; ++w) {
+                    l4[w / 4].v[w % 4] = bf_pack(fl[2 * w], fl[2 * w + 1]);
+                    h4[w / 4].v[w % 4] = bf_pack(fh[2 * w], fh[2 * w + 1]);
+                }
+            } else {
+                // f16 products and sums of stored values, two at a time: f32's 24 bits are twice f16's 11
+                // and two more, so rounding through f32 first, as the steps are defined, changes nothing
+                typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+                auto norm = [&](typename S::raw x) {
+                    _Float16 y = _Float16(opaque(float(double(S::dec(x)) * rs)));
+                    if (isq) y = _Float16(opaque(float(y) * qs));
+                    return y;
+                };
+#pragma unroll
+                for (int w = 0; w < 4 * NV; ++w) {
+                    const int i = 2 * w / VEC, e = 2 * w % VEC;
+                    h2 l = {norm(lo[i].v[e]), norm(lo[i].v[e + 1])}, h = {norm(hi[i].v[e]), norm(hi[i].v[e + 1])};
+                    if (rot) {
+                        const h2 cc = __builtin_bit_cast(h2, __builtin_bit_cast(W4, cv[i]).v[e / 2]);
+                        const h2 sn = __builtin_bit_cast(h2, __builtin_bit_cast(W4, sv[i]).v[e / 2]);
+                        const h2 lr = l * cc + -(h * sn), hr = h * cc + l * sn;
+                        l = lr;
+                        h = hr;
+                    }
+                    l4[w / 4].v[w % 4] = __builtin_bit_cast(uint32_t, l);
+                    h4[w / 4].v[w % 4] = __builtin_bit_cast(uint32_t, h);
+                }
             }
+#pragma unroll
+            for (int w = 0; w < 4 * NV; ++w)
+                mag = pk_max_u16(mag, pk_max_u16(l4[w / 4].v[w % 4] & 0x7fff7fffu, h4[w / 4].v[w % 4] & 0x7fff7fffu));
             if (max(mag & 0xffffu, mag >> 16) > (S::dt == BF16 ? 0x7f80u : 0x7c00u)) {
                 auto canon = [](uint32_t w) { return S::dt == BF16 ? bf_canon(w) : hf_canon(w); };
 #pragma unroll

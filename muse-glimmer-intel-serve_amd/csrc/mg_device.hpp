@@ -295,15 +295,7 @@ namespace mg
         const f2 v = {0.0f, opaque(x)};
         return __builtin_bit_cast(float, __builtin_convertvector(v, h2));
     }
-    // the same for f16: RNE of two values into one word, of one value returned as f32,
-    // and the NaN pattern of f16_bits
-    MG_DEV uint32_t hf_pack(float a, float b)
-    {
-        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-        const h2 h = {static_cast<_Float16>(opaque(a)), static_cast<_Float16>(opaque(b))};
-        return __builtin_bit_cast(uint32_t, h);
-    }
-    MG_DEV float hf_round(float x) { return float(static_cast<_Float16>(opaque(x))); }
+    // the NaN pattern of f16_bits in both halves
     MG_DEV uint32_t hf_canon(uint32_t w)
     {
         const uint32_t a = w & 0xffffu, b = w >> 16;
