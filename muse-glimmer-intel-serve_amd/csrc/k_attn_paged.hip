@@ -151,8 +151,22 @@ namespace mg
     };
     MG_DEV Run find_run(const PagedArgs &a, int team)
     {
-        __shared__ int red[4], found[2];
         const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+        if (a.R <= 64) {
+            // each wave by itself, a request a lane
+            const int own = lane < a.R ? paged_span(a.lens[lane], a.W << a.sh, a.window).units : 0;
+            const int pre = wave_prefix_sum(own);
+            Run r;
+            r.d = paged_teams(__builtin_amdgcn_readlane(pre, 63), a.teams);
+            r.u0 = r.u1 = r.p = r.b = 0;
+            if (team >= r.d.teams) return r;
+            r.u0 = team_first(r.d, team);
+            r.u1 = team_first(r.d, team + 1);
+            r.b = wave_count(pre <= r.u0); // the requests that end before it
+            r.p = r.b > 0 ? __builtin_amdgcn_readlane(pre, r.b - 1) : 0;
+            return r;
+        }
+        __shared__ int red[4], found[2];
         const int per = (a.R + 255) / 256, b0 = tid * per, b1 = min(b0 + per, a.R);
         const int cap = a.W << a.sh;
         int mine = 0;
@@ -538,22 +552,48 @@ namespace mg
             const int place = s == 0 ? cut.z : 2 * (cut.w + s - 1);
             return (int64_t(place) * a.vh + v) * a.hw;
         };
-        float top = -__builtin_huge_valf(), sum = 0.0f;
-        for (int s = sg; s < nt; s += SG) top = __builtin_fmaxf(top, ml[2 * (row(s) + hh)]);
+        // every part's maximum, sum and outputs at once where a thread has at most P of them, else in two passes
+        constexpr int P = 4;
+        float pm[P], pl[P], top = -__builtin_huge_valf(), sum = 0.0f;
+        Vec<float, 4> px[P], acc{{0.0f, 0.0f, 0.0f, 0.0f}};
+        const bool few = nt <= P * SG;
+        if (few) {
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                const int s = sg + k * SG;
+                pm[k] = -__builtin_huge_valf();
+                pl[k] = 0.0f;
+                px[k] = Vec<float, 4>{{0.0f, 0.0f, 0.0f, 0.0f}};
+                if (s < nt && live) {
+                    const int64_t r = row(s);
+                    pm[k] = ml[2 * (r + hh)];
+                    pl[k] = ml[2 * (r + hh) + 1];
+                    px[k] = *reinterpret_cast<const Vec<float, 4> *>(a.part + r * D + i0);
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < P; ++k) top = __builtin_fmaxf(top, pm[k]);
+        } else if (live) {
+            for (int s = sg; s < nt; s += SG) top = __builtin_fmaxf(top, ml[2 * (row(s) + hh)]);
+        }
         tops[sg][e] = top;
         __syncthreads();
 #pragma unroll
         for (int s = 0; s < SG; ++s) top = __builtin_fmaxf(top, tops[s][e]);
         const float ref = top == -__builtin_huge_valf() ? 0.0f : top;
-        Vec<float, 4> acc{{0.0f, 0.0f, 0.0f, 0.0f}};
-        for (int s = sg; s < nt; s += SG) {
-            const int64_t r = row(s);
-            const float f = __builtin_amdgcn_exp2f(ml[2 * (r + hh)] - ref);
-            sum = __builtin_fmaf(f, ml[2 * (r + hh) + 1], sum);
-            if (live) {
-                const Vec<float, 4> x = *reinterpret_cast<const Vec<float, 4> *>(a.part + r * D + i0);
+        auto add = [&](float m, float l, const Vec<float, 4> &x) {
+            const float f = __builtin_amdgcn_exp2f(m - ref);
+            sum = __builtin_fmaf(f, l, sum);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) acc.v[i] = __builtin_fmaf(f, x.v[i], acc.v[i]);
+            for (int i = 0; i < 4; ++i) acc.v[i] = __builtin_fmaf(f, x.v[i], acc.v[i]);
+        };
+        if (few) {
+#pragma unroll
+            for (int k = 0; k < P; ++k) add(pm[k], pl[k], px[k]);
+        } else if (live) {
+            for (int s = sg; s < nt; s += SG) {
+                const int64_t r = row(s);
+                add(ml[2 * (r + hh)], ml[2 * (r + hh) + 1], *reinterpret_cast<const Vec<float, 4> *>(a.part + r * D + i0));
             }
         }
         sums[sg][e] = sum;
