@@ -322,15 +322,17 @@ namespace mg
         advance();
         slot = slot_of();
 
-        for (;;) {
-            // B of S^T: lane (head n, c) holds q[n][32 kb + 8c ..], zero for padding heads
-            typename MS::x8 qop[KB];
+        // B of S^T: lane (head n, c) holds q[n][32 i + 8c ..], zero for padding heads
+        typename MS::x8 qop[KB];
+        auto load_q = [&](int b) {
 #pragma unroll
             for (int i = 0; i < KB; ++i) {
-                const uint16_t *qp =
-                    static_cast<const uint16_t *>(a.q) + cur.b * a.ldq + int64_t(h0 + n) * D + 32 * i + 8 * c;
+                const uint16_t *qp = static_cast<const uint16_t *>(a.q) + b * a.ldq + int64_t(h0 + n) * D + 32 * i + 8 * c;
                 qop[i] = n < a.hw ? ld_x8<typename MS::x8>(qp) : typename MS::x8{};
             }
+        };
+        load_q(cur.b);
+        for (;;) {
             f32x4 o[NT];
 #pragma unroll
             for (int t = 0; t < NT; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -464,6 +466,13 @@ namespace mg
                 }
                 wave_lds_sync(); // this step's reads are done before the next one's writes
             } while (more);
+            // the next request, while the waves join
+            const bool go_on = cur.behind > 0;
+            Part next = cur;
+            if (go_on) {
+                next = part_of(cur.b + 1, 0, cur.behind);
+                load_q(next.b);
+            }
 
             // join the four waves: their outputs take the place of K and V in LDS
             l = rows4_sum(l);
@@ -525,8 +534,8 @@ namespace mg
                 }
             }
             __syncthreads(); // the next part's first step writes where the outputs were
-            if (cur.behind == 0) break;
-            cur = part_of(cur.b + 1, 0, cur.behind);
+            if (!go_on) break;
+            cur = next;
         }
     }
 
