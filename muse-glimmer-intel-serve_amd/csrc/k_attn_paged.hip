@@ -73,18 +73,26 @@ namespace mg
     template <>
     struct Mm<SBf16>
     {
-        using e = __bf16;
         using x8 = bf16x8;
         static constexpr float up = 0.0f; // log2 of the weights' factor
         static MG_DEV f32x4 mma(x8 a, x8 b, f32x4 c) { return mfma_bf16(a, b, c); }
+        static MG_DEV uint32_t pack(float a, float b) { return bf_pack(a, b); }
+        static MG_DEV float low(uint32_t w) { return bf_lo(w); }
+        static MG_DEV float high(uint32_t w) { return bf_hi(w); }
     };
     template <>
     struct Mm<SF16>
     {
-        using e = _Float16;
         using x8 = f16x8;
         static constexpr float up = 12.0f;
         static MG_DEV f32x4 mma(x8 a, x8 b, f32x4 c) { return mfma_f16(a, b, c); }
+        static MG_DEV uint32_t pack(float a, float b)
+        {
+            typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+            return __builtin_bit_cast(uint32_t, h2{_Float16(a), _Float16(b)});
+        }
+        static MG_DEV float low(uint32_t w) { return f16_f32(uint16_t(w)); }
+        static MG_DEV float high(uint32_t w) { return f16_f32(uint16_t(w >> 16)); }
     };
 
     template <class X8>
@@ -92,17 +100,17 @@ namespace mg
     {
         return __builtin_bit_cast(X8, *reinterpret_cast<const Vec<uint32_t, 4> *>(p));
     }
-    // two weights as sums of NP 16-bit parts, each the rest's nearest, at positions e, e + 1 of NP operands
+    // two weights as sums of NP 16-bit parts, each the rest's nearest, as the pair `at` of NP operands
     template <class M, int NP>
-    MG_DEV void split_weights(float p0, float p1, typename M::x8 *const (&w)[NP], int e)
+    MG_DEV void split_weights(float p0, float p1, Vec<uint32_t, 4> (&w)[NP], int at)
     {
 #pragma unroll
         for (int k = 0; k < NP; ++k) {
-            const typename M::e h0 = typename M::e(p0), h1 = typename M::e(p1);
-            (*w[k])[e] = h0;
-            (*w[k])[e + 1] = h1;
-            p0 -= float(h0);
-            p1 -= float(h1);
+            w[k].v[at] = M::pack(p0, p1);
+            if (k + 1 < NP) {
+                p0 -= M::low(w[k].v[at]);
+                p1 -= M::high(w[k].v[at]);
+            }
         }
     }
 
@@ -225,7 +233,17 @@ namespace mg
         __shared__ __align__(16) float scl[Q8 ? 4 : 1][2][KB][32];
         __shared__ float wm[4][16], wl[4][16];
         const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-        const int team = blockIdx.x / a.vh, v = blockIdx.x - team * a.vh;
+        // Work-groups go to the XCDs in turn. A Q8_0 key's scales of all heads share a 64-byte piece or two, so runs
+        // of eight work-groups (a key's heads) are put on one XCD, whose L2 then fetches it once: 5 requests of
+        // 100003 keys, 40/8 heads, 240 -> 209 us (head_dim 64: 190 -> 158); 32/2 heads 60.7 -> 61.5. 16-bit rows
+        // are better off spread (40/8 heads of 64: 375 us, 388 in runs; of 128: 643, 700 all heads on one XCD).
+        constexpr int G = Q8 ? 8 : 1;
+        int wg = blockIdx.x;
+        if (wg < int(gridDim.x) / (8 * G) * (8 * G)) {
+            const int xcd = wg % 8, turn = wg / 8;
+            wg = turn / G * (8 * G) + xcd * G + turn % G;
+        }
+        const int team = wg / a.vh, v = wg - team * a.vh;
         const Run run = find_run(a, team);
         const bool notes = a.teams > 1 && v == 0 && threadIdx.x == 0; // who writes the cuts down
         if (run.u0 >= run.u1) { // the whole work-group
@@ -432,10 +450,7 @@ namespace mg
                 // of dim 16 s + n, through the transposing read
                 const char *vr = Q8 ? sv + (16 * (n >> 3) + 4 * c + (n >> 1 & 3)) * SV + 8 * (n & 1)
                                     : sv + (4 * c + (n >> 2)) * SV + 8 * (n & 3);
-                x8 w[NP];
-                x8 *parts[NP];
-#pragma unroll
-                for (int k = 0; k < NP; ++k) parts[k] = &w[k];
+                Vec<uint32_t, 4> w[NP];
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
                     if constexpr (Q8) {
@@ -445,13 +460,13 @@ namespace mg
                             const Vec<float, 4> d1 = *reinterpret_cast<const Vec<float, 4> *>(d + 16);
 #pragma unroll
                             for (int e = 0; e < 4; e += 2) {
-                                split_weights<M, NP>(p[e] * d0.v[e], p[e + 1] * d0.v[e + 1], parts, e);
-                                split_weights<M, NP>(p[4 + e] * d1.v[e], p[5 + e] * d1.v[e + 1], parts, 4 + e);
+                                split_weights<M, NP>(p[e] * d0.v[e], p[e + 1] * d0.v[e + 1], w, e / 2);
+                                split_weights<M, NP>(p[4 + e] * d1.v[e], p[5 + e] * d1.v[e + 1], w, 2 + e / 2);
                             }
                         }
                     } else if (t == 0) {
 #pragma unroll
-                        for (int e = 0; e < 8; e += 2) split_weights<M, NP>(p[e], p[e + 1], parts, e);
+                        for (int e = 0; e < 8; e += 2) split_weights<M, NP>(p[e], p[e + 1], w, e / 2);
                     }
                     x8 vb;
                     if constexpr (Q8) {
@@ -462,7 +477,7 @@ namespace mg
                         vb = __builtin_bit_cast(x8, bf16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
                     }
 #pragma unroll
-                    for (int k = 0; k < NP; ++k) o[t] = M::mma(w[k], vb, o[t]);
+                    for (int k = 0; k < NP; ++k) o[t] = M::mma(__builtin_bit_cast(x8, w[k]), vb, o[t]);
                 }
                 wave_lds_sync(); // this step's reads are done before the next one's writes
             } while (more);
