@@ -627,3 +627,107 @@ def test_other_stream_and_current_device(prims):
     b = decode_case(prims, [100, 0, 2000], 10, 2, 128, 16)
     assert np.array_equal(a, b)
     p.close()
+
+
+# -------------------------------------------------- paths by batch and workspace
+@pytest.mark.parametrize("dt,q8", FORMS)
+def test_decode_more_than_64_requests(prims, dt, q8):
+    """lengths summed by the whole work-group, runs that begin and end inside requests, a join note a team"""
+    rng = np.random.default_rng(11)
+    lens = rng.integers(0, 900, 100).tolist()
+    lens[7] = lens[99] = 0
+    decode_case(prims, lens, 16, 8, 64, 16, dt, q8, out="same")
+
+
+@pytest.mark.parametrize("R", (63, 64, 65, 257))
+def test_decode_request_counts(prims, R):
+    """at the limits of a wave's and of a work-group's requests, the first and last ones long"""
+    lens = [1000] + [3] * (R - 2) + [777]
+    decode_case(prims, lens, 4, 2, 64, 16, window=0)
+
+
+def test_decode_small_workspaces(prims):
+    """room for a few teams, for one (nothing is cut), for none of it"""
+    import mgprims
+    for size in (64, 40000, 200000):
+        p = mgprims.Prims(0, workspace_bytes=size)
+        decode_case(p, [3000, 5, 0, 900], 10, 2, 128, 16, ws=p)
+        decode_case(p, [200] * 90, 10, 2, 64, 16, q8=True, ws=p)
+        p.close()
+
+
+def test_pages_small_workspace(prims):
+    """a large step without room for its sums: one work-group does it"""
+    import mgprims
+    rng = np.random.default_rng(12)
+    p = mgprims.Prims(0, workspace_bytes=64)
+    old = [0] * 90
+    new = [int(x) for x in rng.integers(0, 200, 90)]
+    table, ring, ends = pages_state(rng, 90, 14, 16, old, 90 * 14)
+    assert sum(new) > 4096
+    run_pages(p, table, old, new, 16, ring, ends, sum(new) + 3)
+    run_pages(prims, table, old, new, 16, ring, ends, sum(new) + 3, in_place=True)
+    # too few pages and maps that end early, in the form of two launches
+    run_pages(prims, table, old, new, 16, ring, [ends[0], ends[0] + 200], sum(new))
+    run_pages(prims, table, old, new, 16, ring, ends, 5000)
+    p.close()
+
+
+@pytest.mark.parametrize("q8", (False, True))
+def test_append_many_tokens(prims, q8):
+    """many work-groups, q's rows and k's, a wave of both kinds"""
+    run_append(prims, BF16, 701, 5, 3, 128, 16, q8, pad=3)
+    run_append(prims, F16, 701, 40, 8, 64, 64, q8, pad=3)
+
+
+def test_two_contexts_at_once(prims):
+    """two contexts on two streams, their calls interleaved"""
+    import torch
+    import mgprims
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    ps = [mgprims.Prims(0, stream=s.cuda_stream) for s in streams]
+    g = torch.Generator(device=DEV).manual_seed(9)
+    kc, vc = (torch.randn((400, 16, 2, 128), generator=g, device=DEV).bfloat16() for _ in range(2))
+    sets = []
+    for i, lens in enumerate(([3000, 40, 0, 900], [17] * 20 + [2500])):
+        R = len(lens)
+        q = torch.randn((R, 32, 128), generator=g, device=DEV).bfloat16()
+        t = torch.randint(0, 400, (R, 200), generator=g, device=DEV).int()
+        sets.append((q, kc, vc, t, i32(lens), 0.088))
+    want = [prims.attn_decode_paged(*x) for x in sets]
+    torch.cuda.synchronize()
+    out = [torch.empty_like(w) for w in want]
+    for _ in range(20):
+        for p, x, o in zip(ps, sets, out):
+            p.attn_decode_paged(*x, out=o)
+    torch.cuda.synchronize()
+    for o, w in zip(out, want):
+        assert torch.equal(o, w)
+    for p in ps:
+        p.close()
+
+
+def test_refused_request_attends_its_old_keys(prims):
+    """a request without a free page keeps its length, appends nothing, and attends what it has"""
+    import torch
+    e = Engine(prims, 3, 4, 16, 4, False, BF16, 3)
+    e.new.copy_(i32([16, 16, 16]))
+    e.slots, e.pos = i64([0] * 48), i64([0] * 48)
+    q, k, v = e.q, e.k, e.v
+    e.q, e.k, e.v = (torch.zeros((48, *t.shape[1:]), dtype=t.dtype, device=DEV) for t in (q, k, v))
+    feed(e, 3)
+    e.step()
+    assert e.lens.tolist() == [16] * 3
+    e.slots, e.pos, e.q, e.k, e.v = i64([0] * 3), i64([0] * 3), q, k, v
+    feed(e, 4)
+    e.new.copy_(i32([17, 17, 16]))  # one page is left
+    before = e.kc.clone()
+    e.step()
+    assert e.lens.tolist() == [17, 16, 16] and e.ends.tolist() == [4, 4]
+    assert e.slots.tolist() == [int(e.table[0, 1]) * 16, -1, -1]
+    changed = (e.kc != before).view(-1, 2 * 128).any(1).nonzero().flatten().tolist()
+    assert changed == [e.slots[0].item()]
+    e.attend()
+    K, V = (c.double().cpu().numpy() for c in (e.kc, e.vc))
+    ref, bound = PO.attn_decode(e.q.double().cpu().numpy(), K, V, e.table.cpu().numpy(), [17, 16, 16], 16, 0, 0.088)
+    assert np.all(np.abs(e.out.double().cpu().numpy() - ref) <= bound)
