@@ -672,9 +672,10 @@ namespace mg
         int64_t hw = hpg;
         while (hw > 16 || hpg % hw != 0) --hw;
         const int64_t vh = nkv * (hpg / hw);
-        // as many teams as the chip holds at once (the work-groups that a CU's LDS and registers
-        // take), not more than there can be units, nor than the workspace has room for
-        const int per_cu = kd ? 3 : D == 128 ? 2 : 4;
+        // Teams for 2 to 4 work-groups a CU: as many as its registers take, but three, not four, for 16-bit rows of
+        // 64 (10 requests of 100003 keys 351 us, four 372, two 358; Q8_0: four 69, three 72, two 81 at 64 ragged
+        // requests of up to 8000). Not more than there can be units, nor than the workspace has room for.
+        const int per_cu = kd ? (D == 128 ? 3 : 4) : (D == 128 ? 2 : 3);
         const int64_t span = window > 0 && window < max_pages << sh ? window + kPagedStep : max_pages << sh;
         const int64_t most = seqs * (span / kPagedUnit + 1);
         need(most < (int64_t(1) << 31), "attn_decode_paged: the table must stand for fewer than 2^38 keys");
