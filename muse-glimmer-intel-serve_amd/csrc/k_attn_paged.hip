@@ -25,8 +25,8 @@
 // across the end of a request, and written to LDS;
 // S^T = K Q^T and O += P V run on the matrix cores (16 query heads of the
 // group, zero-padded, as columns), the weights entering as a high and a low
-// 16-bit part, so each is within 2^-16 of p relative. Online softmax in f32 on
-// scores scaled by log2(e).
+// 16-bit part (three for f32 outputs), so each is within 2^-16 of p relative.
+// Online softmax in f32 on scores scaled by log2(e).
 //   Pages: lane l holds the slot of key l of the step (its table entry was
 // requested a step before); a load instruction covers 4 to 16 rows, which lie
 // in one page where the page is that large, so one readlane gives their base;
@@ -38,6 +38,15 @@
 //   Q8_0: quants become bf16, or f16 beside f16 queries, on their way from LDS,
 // exactly (8 bits); a K block's scale multiplies its 32-dim part of the score, a
 // V block's its weights before they are split, so no value is rounded to 16 bits.
+//
+// What bounds it: HBM where requests are long. 8 requests of 131072 keys (40/8
+// heads of 128, bf16): 646 us, 6.65 TB/s of the 7.04 that a plain read reaches; 64
+// ragged ones of up to 8000: 157, 6.1; 250 of up to 700: 68, 5.1 (waves wait 62 % of
+// their cycles: a request's last step and the waves' meeting leave little in flight).
+// About 6 us of each is launch, sums and the first step's chain of table entry, rows
+// and products; the join adds 4 to 6. Q8_0: 5 of 100003 keys (32/2 heads) 56 us, 4.8
+// TB/s; 550 vector instructions a step and wave keep the SIMDs 58 % busy and three
+// waves each do not cover the rest of the step's chain.
 #include "mg_device.hpp"
 #include "mg_internal.hpp"
 #include "mg_paged_plan.hpp"
@@ -76,7 +85,12 @@ namespace mg
         using x8 = bf16x8;
         static constexpr float up = 0.0f; // log2 of the weights' factor
         static MG_DEV f32x4 mma(x8 a, x8 b, f32x4 c) { return mfma_bf16(a, b, c); }
-        static MG_DEV uint32_t pack(float a, float b) { return bf_pack(a, b); }
+        static MG_DEV uint32_t pack(float a, float b) // (bf_pack, without its copies of values that live on)
+        {
+            typedef float f2 __attribute__((ext_vector_type(2)));
+            typedef __bf16 h2 __attribute__((ext_vector_type(2)));
+            return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), h2));
+        }
         static MG_DEV float low(uint32_t w) { return bf_lo(w); }
         static MG_DEV float high(uint32_t w) { return bf_hi(w); }
     };
@@ -121,8 +135,8 @@ namespace mg
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const uint32_t u = x.v[i];
-            w.v[2 * i] = bf_pack(float(int8_t(u)), float(int8_t(u >> 8)));
-            w.v[2 * i + 1] = bf_pack(float(int8_t(u >> 16)), float(int32_t(u) >> 24));
+            w.v[2 * i] = Mm<SBf16>::pack(float(int8_t(u)), float(int8_t(u >> 8)));
+            w.v[2 * i + 1] = Mm<SBf16>::pack(float(int8_t(u >> 16)), float(int32_t(u) >> 24));
         }
         return __builtin_bit_cast(bf16x8, w);
     }
