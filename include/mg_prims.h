@@ -270,7 +270,8 @@ int mg_attn_decode(mg_ctx *ctx, const uint16_t *q, const uint16_t *k_cache, cons
  * the pages of the requests up to and including it, refused ones too unless for
  * the first two reasons, are more than the queue holds: its tokens' entries are
  * -1. Negative lengths count as 0, old ones past the row's capacity as that. A
- * table entry outside the pool gives slot -1. At most 4096 requests; everything
+ * table entry outside the pool gives slot -1. At most 4096 requests, 2^30 tokens
+ * and fewer than 2^31 table entries and pages; everything
  * stays on the device, so a decode loop can be captured (these calls, as others,
  * use the context's workspace: graphs captured from one context are replayed one
  * after another). No tensor may overlap another but as said. */
@@ -305,9 +306,12 @@ int mg_qk_norm_rope_paged(mg_ctx *ctx, void *q, int64_t q_heads, int64_t ldq, vo
  * counts below 0 as 0 and above the row's capacity as that. A request with no key
  * gives zeros; a key whose page lies outside the pool is left out, as a masked
  * one; what the pool holds behind a request's length or before its window is
- * never used. head_dim 64 or 128; any number of query heads per kv head; at most
- * 65535 requests and 2^31 - 1 slots in the pool. A numerical envelope, not bits: f32 sums and weights to 2^-16 relative, keys split
- * over work-groups and joined, the split depending on the batch's lengths. */
+ * never used. An attended value that is not finite makes the outputs it enters
+ * not finite (an infinite one may give NaN). head_dim 64 or 128; any number of
+ * query heads per kv head; at most 65535 requests, 2^31 - 1 slots in the pool and
+ * tables (or windows of them) of fewer than 2^38 keys. A numerical envelope, not
+ * bits: f32 sums and weights to 2^-16 relative, keys split over work-groups and
+ * joined, the split depending on the batch's lengths. */
 int mg_attn_decode_paged(mg_ctx *ctx, const void *q, int64_t ldq, const void *k_cache, const void *v_cache,
                          const uint16_t *k_scale, const uint16_t *v_scale, const int32_t *page_table, int64_t ldt,
                          int64_t max_pages, const int32_t *lens, int64_t requests, int64_t q_heads, int64_t kv_heads,

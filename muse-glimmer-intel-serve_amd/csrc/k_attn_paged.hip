@@ -45,7 +45,7 @@
 // their cycles: a request's last step and the waves' meeting leave little in flight).
 // About 6 us of each is launch, sums and the first step's chain of table entry, rows
 // and products; the join adds 4 to 6. Q8_0: 5 of 100003 keys (32/2 heads) 56 us, 4.8
-// TB/s; 550 vector instructions a step and wave keep the SIMDs 58 % busy and three
+// TB/s; 580 vector instructions a step and wave keep the SIMDs 58 % busy and three
 // waves each do not cover the rest of the step's chain.
 #include "mg_device.hpp"
 #include "mg_internal.hpp"

@@ -1,5 +1,5 @@
 // How decode attention over a paged cache divides its keys among work-groups:
-// plain arithmetic, the same on the host (its checker) and on the device.
+// plain arithmetic, the same on the host (its host test) and on the device.
 //
 // A request's attended keys [lo, n) are cut into units of 128 keys from `base`,
 // lo rounded down to a step of 32 (a request without keys has one empty unit,

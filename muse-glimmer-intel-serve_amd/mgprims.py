@@ -461,7 +461,8 @@ class Prims:
         (free_ring [num_pages] int32 with counters ends [2] int64: entries ends[0] .. ends[1] - 1, each
         modulo num_pages); page_table [R, W] int32 is updated in place. Writes lens [R] (may be old_lens
         or new_lens), ends_out [2] (may be ends), starts [R + 1] int32, and slot_map and positions
-        [tokens] int64 of the step's new tokens, -1 behind the last and for refused requests."""
+        [tokens] int64 of the step's new tokens, -1 behind the last and for refused requests (without
+        both maps there is room for no token: requests can only shrink)."""
         name, i32, i64, ints = "kv_pages", self._i32, self._i64, self._ints
         R, N = old_lens.numel(), free_ring.numel()
         T = slot_map.numel() if slot_map is not None else positions.numel() if positions is not None else 0
