@@ -19,21 +19,28 @@
 // requests behind it either way, so the granted ones take a prefix of the
 // queue. Every sum is of whole numbers: results do not depend on the order.
 //
-// One work-group takes the three sums (prefix sums over 1024 requests at a time)
-// into LDS; every item of the step (a token, a page taken, a
-// page given back) then finds its request by bisection there. A step with few
-// tokens ends in that launch. One with more leaves the sums in the workspace and
-// a second launch of many work-groups, each with the sums in its own LDS, does
-// the items. Measured, us a call (64 requests): 2191 tokens 8.1 in one launch, 11.0
-// in two; 4344 10.0 and 11.0; 8803 15.0 and 11.4; 17570 25.2 and 10.7. Latency bounds
-// both: a launch, then chains of a bisection and two or three dependent loads.
+// A work-group takes the three sums (prefix sums over 1024 requests at a time)
+// into LDS; every item of the step (a token, a page taken, a page given back)
+// then finds its request by bisection there. Small steps run in one work-group;
+// larger ones in a work-group for every 1024 tokens, each with all the sums for itself
+// (R lengths from L2: cheaper than sums from memory in a second launch; 1000
+// requests, 94 000 tokens 13.3 -> 7.3 us a call, 200 requests, 520 000 tokens 11.2 -> 7.3),
+// and the first also writes the new lengths and counters. Where those replace their
+// old values, which the others still read, they are left to a second launch of one
+// work-group, from 4096 tokens on (10.1 us, what one work-group takes at 4300).
+//
+// Latency bounds it: 4.4 us of kernel for a decode step of 48 requests, 6.7 and 7.2 for the two
+// above: a launch, the sums, then chains of a bisection and two or three dependent loads.
 #include "mg_device.hpp"
 #include "mg_internal.hpp"
 
 namespace mg
 {
     constexpr int kPagesMax = 4096;   // requests: three sums of each fit 64 KiB of LDS
-    constexpr int kPagesAlone = 4096; // tokens up to which one work-group does the whole step
+    constexpr int kPagesGroup = 1024; // tokens a work-group
+    constexpr int kPagesAlone = 4096; // tokens up to which one does the whole of a step in place
+
+    enum : int { kPagesItems = 1, kPagesEnd = 2 }; // what a launch does: the items, the lengths and counters
 
     struct PagesArgs
     {
@@ -45,9 +52,9 @@ namespace mg
         int64_t *ends_out;
         int32_t *starts;
         int64_t *slots, *pos;
-        int *sums;    // workspace: the three sums, R + 1 each, then old and new lengths, then head and tail in the ring
         int64_t ldt;
         int R, W, N, T, sh;
+        int what;
     };
 
     // the last index in [0, n) whose sum is at most x (sums: n + 1 entries from 0, not
@@ -65,30 +72,40 @@ namespace mg
         return lo;
     }
 
-    // inclusive sums of two values over the work-group's threads on top of their carries, which move on
-    template <int NT>
-    MG_DEV void group_prefix_u64(uint64_t &u, uint64_t &v, uint64_t &cu, uint64_t &cv, uint64_t (&red)[2][NT / 64])
+    MG_DEV uint32_t add_sat(uint32_t a, uint32_t b) { return __builtin_elementwise_add_sat(a, b); }
+    // wave_prefix_sum with sums that stop at 2^32 - 1
+    MG_DEV uint32_t wave_prefix_sat(uint32_t u)
     {
-        const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6;
+        uint32_t t = u;
+        t = add_sat(t, dpp32<0x111, 0xf>(0u, u));
+        t = add_sat(t, dpp32<0x112, 0xf>(0u, u));
+        t = add_sat(t, dpp32<0x113, 0xf>(0u, u));
+        t = add_sat(t, dpp32<0x114, 0xf, 0xe>(0u, t));
+        t = add_sat(t, dpp32<0x118, 0xf, 0xc>(0u, t));
+        t = add_sat(t, dpp32<0x142, 0xa>(0u, t));
+        t = add_sat(t, dpp32<0x143, 0xc>(0u, t));
+        return t;
+    }
+    // inclusive sums of three values over the work-group's first `waves` waves (the others hold none) on top of
+    // their carries, which move on; they stop at 2^32 - 1
+    template <int NT>
+    MG_DEV void group_prefix(uint32_t (&u)[3], uint32_t (&carry)[3], uint32_t (&red)[3][NT / 64], int waves)
+    {
+        const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        if (wv < waves) {
 #pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-            const uint64_t x = __shfl_up(u, m, 64), y = __shfl_up(v, m, 64);
-            u += lane >= m ? x : 0;
-            v += lane >= m ? y : 0;
-        }
-        if (lane == 63) {
-            red[0][wv] = u;
-            red[1][wv] = v;
+            for (int k = 0; k < 3; ++k) {
+                u[k] = wave_prefix_sat(u[k]);
+                if (lane == 63) red[k][wv] = u[k];
+            }
         }
         __syncthreads();
-        u += cu;
-        v += cv;
-        for (int w = 0; w < NT / 64; ++w) {
-            const uint64_t x = red[0][w], y = red[1][w];
-            u += w < wv ? x : 0;
-            v += w < wv ? y : 0;
-            cu += x;
-            cv += y;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            const int r = int(wave_prefix_sat(lane < waves ? red[k][lane] : 0u));
+            const uint32_t before = wv > 0 ? uint32_t(__builtin_amdgcn_readlane(r, wv - 1)) : 0u;
+            u[k] = add_sat(add_sat(u[k], before), carry[k]);
+            carry[k] = add_sat(carry[k], uint32_t(__builtin_amdgcn_readlane(r, 63)));
         }
         __syncthreads();
     }
@@ -170,54 +187,47 @@ namespace mg
         }
     };
 
-    template <int NT, bool ALONE>
+    template <int NT>
     __global__ __launch_bounds__(NT) void k_kv_pages(PagesArgs a)
     {
         extern __shared__ int sums[];
-        __shared__ uint64_t red[2][NT / 64];
+        __shared__ uint32_t red[3][NT / 64];
+        __shared__ int place[2];
         int *st = sums, *go = sums + a.R + 1, *bo = sums + 2 * (a.R + 1);
         const int tid = threadIdx.x;
         const int64_t head = a.ends[0], tail = a.ends[1];
         const int64_t left = tail - head;
         const int avail = left < 0 ? 0 : left > a.N ? a.N : int(left);
-        const PagesStep s{a, st, go, bo, a.old_lens, a.new_lens, avail, ring_at(head, a.N), ring_at(tail, a.N)};
-        if (tid == 0) st[0] = go[0] = bo[0] = 0;
+        PagesStep s{a, st, go, bo, a.old_lens, a.new_lens, avail, 0, 0};
+        if (tid == NT - 1) { // (two long divisions, beside the first waves' sums)
+            st[0] = go[0] = bo[0] = 0;
+            place[0] = ring_at(head, a.N);
+            place[1] = ring_at(tail, a.N);
+        }
         // the sums: first as if the maps held every token, again without those that do not fit where they do not
         for (bool again = false;; again = true) {
-            uint64_t tokens = 0, pages = 0; // pages: taken in the low half, given back in the high half
+            uint32_t carry[3] = {0, 0, 0}; // tokens, pages taken, pages given back (fewer than 2^31, as the table's)
             for (int b = 0; b < a.R; b += NT) {
                 const int i = b + tid;
                 int o = 0, n = 0;
                 if (i < a.R) s.lens(i, o, n);
                 const bool fits = n <= (a.W << a.sh) && (!again || i >= a.R || st[i + 1] <= a.T);
                 const int d = pages_of(n, a.sh) - pages_of(o, a.sh);
-                uint64_t te = uint64_t(max(n - o, 0)), pe = d >= 0 ? (fits ? uint64_t(d) : 0) : uint64_t(-d) << 32;
-                group_prefix_u64<NT>(te, pe, tokens, pages, red);
+                uint32_t u[3] = {uint32_t(max(n - o, 0)), d > 0 && fits ? uint32_t(d) : 0u, uint32_t(max(-d, 0))};
+                group_prefix<NT>(u, carry, red, min(NT / 64, (a.R - b + 63) / 64));
                 if (i < a.R) {
-                    st[i + 1] = int(te <= uint64_t(a.T) ? te : uint64_t(a.T) + 1);
-                    go[i + 1] = int(uint32_t(pe));
-                    bo[i + 1] = int(pe >> 32);
+                    st[i + 1] = int(min(u[0], uint32_t(a.T) + 1));
+                    go[i + 1] = int(u[1]);
+                    bo[i + 1] = int(u[2]);
                 }
             }
             __syncthreads();
-            if (again || tokens <= uint64_t(a.T)) break;
+            if (again || carry[0] <= uint32_t(a.T)) break;
         }
-        if constexpr (ALONE) {
-            s.items(tid, NT);
-        } else {
-            const int n3 = 3 * (a.R + 1);
-            for (int i = tid; i < n3; i += NT) a.sums[i] = sums[i];
-            for (int i = tid; i < a.R; i += NT) {
-                a.sums[n3 + i] = a.old_lens[i];
-                a.sums[n3 + a.R + i] = a.new_lens[i];
-            }
-            if (tid == 0) {
-                int *e = a.sums + n3 + 2 * a.R;
-                e[0] = s.avail;
-                e[1] = s.h0;
-                e[2] = s.t0;
-            }
-        }
+        s.h0 = place[0];
+        s.t0 = place[1];
+        if (a.what & kPagesItems) s.items(blockIdx.x * NT + tid, gridDim.x * NT);
+        if (!(a.what & kPagesEnd) || blockIdx.x != 0) return;
         __syncthreads(); // the lengths may be updated in place: every thread is done with them
         for (int i = tid; i < a.R; i += NT) {
             int o, n;
@@ -233,17 +243,6 @@ namespace mg
             a.ends_out[0] = head + used;
             a.ends_out[1] = tail + bo[a.R];
         }
-    }
-
-    __global__ __launch_bounds__(256) void k_kv_pages_items(PagesArgs a)
-    {
-        extern __shared__ int sums[];
-        const int n1 = a.R + 1;
-        for (int i = threadIdx.x; i < 3 * n1; i += 256) sums[i] = a.sums[i];
-        const int *lens = a.sums + 3 * n1, *e = lens + 2 * a.R;
-        const PagesStep s{a, sums, sums + n1, sums + 2 * n1, lens, lens + a.R, e[0], e[1], e[2]};
-        __syncthreads();
-        s.items(blockIdx.x * 256 + threadIdx.x, gridDim.x * 256);
     }
 
     void launch_kv_pages(mg_ctx *c, int32_t *table, int64_t ldt, int64_t requests, int64_t max_pages,
@@ -262,20 +261,22 @@ namespace mg
         need(ring && ends && ends_out, "kv_pages: NULL tensor");
         if (ldt == 0) ldt = max_pages;
         need(ldt >= max_pages, "kv_pages: row stride smaller than a row");
-        const PagesArgs a{table,    old_lens, new_lens, ring, ends, lens, ends_out, starts, slots, pos, static_cast<int *>(c->work),
-                          ldt, int(requests), int(max_pages), int(num_pages), int(tokens), sh};
+        PagesArgs a{table, old_lens, new_lens, ring, ends, lens, ends_out, starts, slots, pos,
+                    ldt, int(requests), int(max_pages), int(num_pages), int(tokens), sh, 0};
         const size_t lds = 3 * size_t(requests + 1) * sizeof(int);
-        const int64_t room = c->work_bytes / int64_t(sizeof(int));
-        if (tokens <= kPagesAlone || 5 * requests + 6 > room) {
-            hipLaunchKernelGGL((k_kv_pages<1024, true>), dim3(1), dim3(1024), lds, c->stream, a);
+        auto go = [&](int what, int64_t groups) {
+            a.what = what;
+            hipLaunchKernelGGL((k_kv_pages<1024>), dim3(unsigned(groups)), dim3(1024), lds, c->stream, a);
             check_launch("k_kv_pages");
-            return;
+        };
+        const int64_t most = 2 * int64_t(c->num_cus), all = (tokens + kPagesGroup - 1) / kPagesGroup;
+        const int64_t groups = all < 1 ? 1 : all < most ? all : most;
+        const bool in_place = lens == old_lens || lens == new_lens || ends_out == ends;
+        if (!in_place || tokens <= kPagesAlone) {
+            go(kPagesItems | kPagesEnd, in_place ? 1 : groups);
+        } else {
+            go(kPagesItems, groups);
+            go(kPagesEnd, 1);
         }
-        hipLaunchKernelGGL((k_kv_pages<1024, false>), dim3(1), dim3(1024), lds, c->stream, a);
-        check_launch("k_kv_pages");
-        // a token a thread, at most a few rounds of work-groups
-        const int64_t most = 8 * int64_t(c->num_cus), groups = (tokens + 255) / 256;
-        hipLaunchKernelGGL(k_kv_pages_items, dim3(unsigned(groups < most ? groups : most)), dim3(256), lds, c->stream, a);
-        check_launch("k_kv_pages_items");
     }
 } // namespace mg

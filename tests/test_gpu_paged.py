@@ -657,7 +657,7 @@ def test_decode_small_workspaces(prims):
 
 
 def test_pages_small_workspace(prims):
-    """a large step without room for its sums: one work-group does it"""
+    """a large step needs no room in the workspace"""
     import mgprims
     rng = np.random.default_rng(12)
     p = mgprims.Prims(0, workspace_bytes=64)
@@ -667,10 +667,28 @@ def test_pages_small_workspace(prims):
     assert sum(new) > 4096
     run_pages(p, table, old, new, 16, ring, ends, sum(new) + 3)
     run_pages(prims, table, old, new, 16, ring, ends, sum(new) + 3, in_place=True)
-    # too few pages and maps that end early, in the form of two launches
+    # too few pages and maps that end early
     run_pages(prims, table, old, new, 16, ring, [ends[0], ends[0] + 200], sum(new))
     run_pages(prims, table, old, new, 16, ring, ends, 5000)
     p.close()
+
+
+@pytest.mark.parametrize("R", (1, 63, 200, 1024, 1030, 4096))
+@pytest.mark.parametrize("tokens", (1024, 1025, 4096, 4097, 9001))
+def test_pages_step_sizes(prims, R, tokens):
+    """around the sizes where a step takes more work-groups or, in place, two launches: maps with room to spare,
+    maps that end early (requests behind the end only shrink) and too few pages"""
+    rng = np.random.default_rng(R + tokens)
+    ps, most = 16, 2 * tokens // R + 2
+    W = (most + 40) // ps + 2
+    old = [int(x) for x in rng.integers(0, 40, R)]
+    new = [o + int(x) if rng.random() < 0.8 else int(x) // 4 for o, x in zip(old, rng.integers(0, most, R))]
+    takes = sum(max(0, PO.pages_of(n, ps) - PO.pages_of(o, ps)) for o, n in zip(old, new))
+    table, ring, ends = pages_state(rng, R, W, ps, old, takes + 3, head=7)
+    for in_place in (False, True):
+        for t, e in ((max(tokens, sum(max(0, n - o) for o, n in zip(old, new))), ends), (tokens, ends),
+                     (tokens, [ends[0], ends[0] + takes // 2])):
+            run_pages(prims, table, old, new, ps, ring, e, t, in_place=in_place)
 
 
 @pytest.mark.parametrize("q8", (False, True))
