@@ -590,19 +590,22 @@ namespace mg
             const int place = s == 0 ? cut.z : 2 * (cut.w + s - 1);
             return (int64_t(place) * a.vh + v) * a.hw;
         };
-        // every part's maximum, sum and outputs at once where a thread has at most P of them, else in two passes
-        constexpr int P = 4;
-        float pm[P], pl[P], top = -__builtin_huge_valf(), sum = 0.0f;
-        Vec<float, 4> px[P], acc{{0.0f, 0.0f, 0.0f, 0.0f}};
-        const bool few = nt <= P * SG;
-        if (few) {
+        // P parts' maxima, sums and outputs are in flight at once (5 requests of 77 parts: 6.4 us with four, 5.2 with eight),
+        // joined with those before them as scores are
+        constexpr int P = E <= 16 ? 8 : 4;
+        constexpr float kLow = -__builtin_huge_valf();
+        float top = kLow, sum = 0.0f;
+        Vec<float, 4> acc{{0.0f, 0.0f, 0.0f, 0.0f}};
+        for (int s0 = sg; s0 < nt && live; s0 += P * SG) {
+            float pm[P], pl[P], t = top;
+            Vec<float, 4> px[P];
 #pragma unroll
             for (int k = 0; k < P; ++k) {
-                const int s = sg + k * SG;
-                pm[k] = -__builtin_huge_valf();
+                const int s = s0 + k * SG;
+                pm[k] = kLow;
                 pl[k] = 0.0f;
                 px[k] = Vec<float, 4>{{0.0f, 0.0f, 0.0f, 0.0f}};
-                if (s < nt && live) {
+                if (s < nt) {
                     const int64_t r = row(s);
                     pm[k] = ml[2 * (r + hh)];
                     pl[k] = ml[2 * (r + hh) + 1];
@@ -610,34 +613,33 @@ namespace mg
                 }
             }
 #pragma unroll
-            for (int k = 0; k < P; ++k) top = __builtin_fmaxf(top, pm[k]);
-        } else if (live) {
-            for (int s = sg; s < nt; s += SG) top = __builtin_fmaxf(top, ml[2 * (row(s) + hh)]);
+            for (int k = 0; k < P; ++k) t = __builtin_fmaxf(t, pm[k]);
+            const float ref = t == kLow ? 0.0f : t, f = __builtin_amdgcn_exp2f(top - ref);
+            sum *= f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc.v[i] *= f;
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                const float w = __builtin_amdgcn_exp2f(pm[k] - ref);
+                sum = __builtin_fmaf(w, pl[k], sum);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc.v[i] = __builtin_fmaf(w, px[k].v[i], acc.v[i]);
+            }
+            top = t;
         }
         tops[sg][e] = top;
         __syncthreads();
+        float all = top;
 #pragma unroll
-        for (int s = 0; s < SG; ++s) top = __builtin_fmaxf(top, tops[s][e]);
-        const float ref = top == -__builtin_huge_valf() ? 0.0f : top;
-        auto add = [&](float m, float l, const Vec<float, 4> &x) {
-            const float f = __builtin_amdgcn_exp2f(m - ref);
-            sum = __builtin_fmaf(f, l, sum);
+        for (int s = 0; s < SG; ++s) all = __builtin_fmaxf(all, tops[s][e]);
+        const float f = __builtin_amdgcn_exp2f(top - (all == kLow ? 0.0f : all));
+        sums[sg][e] = sum * f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc.v[i] = __builtin_fmaf(f, x.v[i], acc.v[i]);
-        };
-        if (few) {
-#pragma unroll
-            for (int k = 0; k < P; ++k) add(pm[k], pl[k], px[k]);
-        } else if (live) {
-            for (int s = sg; s < nt; s += SG) {
-                const int64_t r = row(s);
-                add(ml[2 * (r + hh)], ml[2 * (r + hh) + 1], *reinterpret_cast<const Vec<float, 4> *>(a.part + r * D + i0));
-            }
-        }
-        sums[sg][e] = sum;
-        accs[sg][e] = acc;
+        for (int i = 0; i < 4; ++i) accs[sg][e].v[i] = acc.v[i] * f;
         __syncthreads();
         if (sg != 0 || !live) return;
+        sum = sums[0][e];
+        acc = accs[0][e];
 #pragma unroll
         for (int s = 1; s < SG; ++s) {
             sum += sums[s][e];
@@ -727,8 +729,14 @@ namespace mg
                 hipLaunchKernelGGL(kern, grid, dim3(256), 0, c->stream, a, int(D));
                 check_launch("k_attn_paged_join");
             };
-            // few requests over many teams: threads over the teams; else over the outputs
-            teams / who >= 8 ? join(k_attn_paged_join<SO, 16>, 16) : join(k_attn_paged_join<SO, 64>, 64);
+            // few requests over many teams: threads over the teams; else over the outputs (one request of 131072 keys,
+            // 32/2 heads, 256 teams, 4 / 16: 31.3 us, 32.7; 8/1 heads, 512 teams: 21.7, 27.8; two of 60000, 32/2 heads, 128
+            // teams each: 31.4, 29.9)
+            const int64_t parts = teams / who;
+            if (parts >= 256)
+                join(k_attn_paged_join<SO, 4>, 4);
+            else
+                parts >= 8 ? join(k_attn_paged_join<SO, 16>, 16) : join(k_attn_paged_join<SO, 64>, 64);
         };
         if (dt_out == F32)
             dt == BF16 ? sized(SBf16{}, SF32{}) : sized(SF16{}, SF32{});

@@ -382,6 +382,15 @@ def test_decode_long(prims, dt, q8):
     decode_case(prims, [9001], 5, 1, 64, 128, dt, q8)
 
 
+@pytest.mark.parametrize("dt,q8", FORMS)
+def test_decode_many_parts(prims, dt, q8):
+    """requests of hundreds of partial results: alone, next to few short ones, next to many"""
+    decode_case(prims, [40000], 8, 1, 128, 16, dt, q8)
+    decode_case(prims, [100000], 2, 1, 64, 64, dt, q8, out="same")
+    decode_case(prims, [30000, 5, 0], 4, 1, 128, 32, dt, q8)
+    decode_case(prims, [9] * 40 + [30000] + [7] * 60, 3, 1, 64, 16, dt, q8)
+
+
 def test_decode_many_short(prims):
     """more requests than work-groups, all short"""
     rng = np.random.default_rng(8)
