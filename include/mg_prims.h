@@ -272,9 +272,9 @@ int mg_attn_decode(mg_ctx *ctx, const uint16_t *q, const uint16_t *k_cache, cons
  * -1. Negative lengths count as 0, old ones past the row's capacity as that. A
  * table entry outside the pool gives slot -1. At most 4096 requests, 2^30 tokens
  * and fewer than 2^31 table entries and pages; everything
- * stays on the device, so a decode loop can be captured (these calls, as others,
- * use the context's workspace: graphs captured from one context are replayed one
- * after another). No tensor may overlap another but as said. */
+ * stays on the device, so a decode loop can be captured (the attention below, as
+ * other calls, uses the context's workspace: graphs captured from one context are
+ * replayed one after another). No tensor may overlap another but as said. */
 int mg_kv_pages(mg_ctx *ctx, int32_t *page_table, int64_t ldt, int64_t requests, int64_t max_pages,
                 const int32_t *old_lens, const int32_t *new_lens, int64_t page_size, int32_t *free_ring,
                 int64_t num_pages, const int64_t *ends, int32_t *lens, int64_t *ends_out, int32_t *starts,

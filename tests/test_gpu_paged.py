@@ -700,6 +700,26 @@ def test_pages_step_sizes(prims, R, tokens):
             run_pages(prims, table, old, new, ps, ring, e, t, in_place=in_place)
 
 
+@pytest.mark.parametrize("tokens", (700, 6000))
+@pytest.mark.parametrize("lens_is,ends_in_place", (("new", False), ("new", True), ("apart", True), ("old", False)))
+def test_pages_what_is_in_place(prims, tokens, lens_is, ends_in_place):
+    """each of the outputs that may replace its input, alone and together"""
+    rng = np.random.default_rng(tokens)
+    R, ps = 60, 16
+    old = [int(x) for x in rng.integers(0, 40, R)]
+    new = [o + tokens // R if i % 5 else 0 for i, o in enumerate(old)]
+    W = max(new) // ps + 2
+    table, ring, ends = pages_state(rng, R, W, ps, old, R * W, head=3)
+    t, dold, dnew, dring, dends = i32(table), i32(old), i32(new), i32(ring), i64(ends)
+    lens = {"new": dnew, "old": dold, "apart": i32([-5] * R)}[lens_is]
+    eout = dends if ends_in_place else i64([-5, -5])
+    starts, slots, pos = i32([-5] * (R + 1)), i64([-5] * tokens), i64([-5] * tokens)
+    prims.kv_pages(t, dold, dnew, ps, dring, dends, lens, eout, starts, slots, pos)
+    want = PO.kv_pages(table.tolist(), old, new, ps, ring.tolist(), ends, tokens)
+    for g, w in zip((t, dring, lens, eout, starts, slots, pos), want):
+        assert np.array_equal(g.cpu().numpy(), np.asarray(w).reshape(tuple(g.shape)))
+
+
 @pytest.mark.parametrize("q8", (False, True))
 def test_append_many_tokens(prims, q8):
     """many work-groups, q's rows and k's, a wave of both kinds"""
