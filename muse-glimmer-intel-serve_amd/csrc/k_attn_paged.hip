@@ -590,22 +590,20 @@ namespace mg
             const int place = s == 0 ? cut.z : 2 * (cut.w + s - 1);
             return (int64_t(place) * a.vh + v) * a.hw;
         };
-        // P parts' maxima, sums and outputs are in flight at once (5 requests of 77 parts: 6.4 us with four, 5.2 with eight),
-        // joined with those before them as scores are
+        // P parts' maxima, sums and outputs are in flight at once (5 requests of 77 parts: 6.4 us with four, 4.8 with
+        // eight); a thread with more takes them in batches, joined as scores are
         constexpr int P = E <= 16 ? 8 : 4;
         constexpr float kLow = -__builtin_huge_valf();
-        float top = kLow, sum = 0.0f;
-        Vec<float, 4> acc{{0.0f, 0.0f, 0.0f, 0.0f}};
-        for (int s0 = sg; s0 < nt && live; s0 += P * SG) {
-            float pm[P], pl[P], t = top;
-            Vec<float, 4> px[P];
+        float pm[P], pl[P], top = kLow, sum = 0.0f;
+        Vec<float, 4> px[P], acc{{0.0f, 0.0f, 0.0f, 0.0f}};
+        auto load = [&](int s0) {
 #pragma unroll
             for (int k = 0; k < P; ++k) {
                 const int s = s0 + k * SG;
                 pm[k] = kLow;
                 pl[k] = 0.0f;
                 px[k] = Vec<float, 4>{{0.0f, 0.0f, 0.0f, 0.0f}};
-                if (s < nt) {
+                if (s < nt && live) {
                     const int64_t r = row(s);
                     pm[k] = ml[2 * (r + hh)];
                     pl[k] = ml[2 * (r + hh) + 1];
@@ -613,29 +611,45 @@ namespace mg
                 }
             }
 #pragma unroll
-            for (int k = 0; k < P; ++k) t = __builtin_fmaxf(t, pm[k]);
-            const float ref = t == kLow ? 0.0f : t, f = __builtin_amdgcn_exp2f(top - ref);
+            for (int k = 0; k < P; ++k) top = __builtin_fmaxf(top, pm[k]);
+        };
+        auto add = [&](float ref) {
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                const float f = __builtin_amdgcn_exp2f(pm[k] - ref);
+                sum = __builtin_fmaf(f, pl[k], sum);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc.v[i] = __builtin_fmaf(f, px[k].v[i], acc.v[i]);
+            }
+        };
+        auto scale = [&](float f) {
             sum *= f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc.v[i] *= f;
-#pragma unroll
-            for (int k = 0; k < P; ++k) {
-                const float w = __builtin_amdgcn_exp2f(pm[k] - ref);
-                sum = __builtin_fmaf(w, pl[k], sum);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) acc.v[i] = __builtin_fmaf(w, px[k].v[i], acc.v[i]);
+        };
+        auto ref_of = [&](float t) { return t == kLow ? 0.0f : t; };
+        const bool few = nt <= P * SG; // one batch: weighed by the maximum of all threads at once
+        load(sg);
+        if (!few) {
+            add(ref_of(top));
+            for (int s0 = sg + P * SG; s0 < nt; s0 += P * SG) {
+                const float was = top;
+                load(s0);
+                scale(__builtin_amdgcn_exp2f(was - ref_of(top)));
+                add(ref_of(top));
             }
-            top = t;
         }
         tops[sg][e] = top;
         __syncthreads();
         float all = top;
 #pragma unroll
         for (int s = 0; s < SG; ++s) all = __builtin_fmaxf(all, tops[s][e]);
-        const float f = __builtin_amdgcn_exp2f(top - (all == kLow ? 0.0f : all));
-        sums[sg][e] = sum * f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) accs[sg][e].v[i] = acc.v[i] * f;
+        if (few)
+            add(ref_of(all));
+        else
+            scale(__builtin_amdgcn_exp2f(top - ref_of(all)));
+        sums[sg][e] = sum;
+        accs[sg][e] = acc;
         __syncthreads();
         if (sg != 0 || !live) return;
         sum = sums[0][e];
