@@ -34,7 +34,8 @@
 // is one bit a key, and rows of masked keys are never loaded: what they hold
 // (NaN too) cannot reach the sums.
 //   f16: weights are kept at 2^12 p, so that the low part of a weight down to
-// 2^-26 of the largest is a normal number; sum and output carry the factor.
+// 2^-26 of the largest is a normal number; sum and output carry the factor. It
+// multiplies the weight: beside a maximum past 2^26 an exponent would lose it.
 //   Q8_0: quants become bf16, or f16 beside f16 queries, on their way from LDS,
 // exactly (8 bits); a K block's scale multiplies its 32-dim part of the score, a
 // V block's its weights before they are split, so no value is rounded to 16 bits.
@@ -83,7 +84,7 @@ namespace mg
     struct Mm<SBf16>
     {
         using x8 = bf16x8;
-        static constexpr float up = 0.0f; // log2 of the weights' factor
+        static constexpr float up = 1.0f; // the weights' factor
         static MG_DEV f32x4 mma(x8 a, x8 b, f32x4 c) { return mfma_bf16(a, b, c); }
         static MG_DEV uint32_t pack(float a, float b) // (bf_pack, without its copies of values that live on)
         {
@@ -98,7 +99,7 @@ namespace mg
     struct Mm<SF16>
     {
         using x8 = f16x8;
-        static constexpr float up = 12.0f;
+        static constexpr float up = 0x1p12f;
         static MG_DEV f32x4 mma(x8 a, x8 b, f32x4 c) { return mfma_f16(a, b, c); }
         static MG_DEV uint32_t pack(float a, float b)
         {
@@ -444,7 +445,7 @@ namespace mg
                 // weights: element 4t + r of lane (head n, c) is key 16 t + 4c + r
                 float p[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f(sc[e >> 2][e & 3] - (mref - M::up));
+                for (int e = 0; e < 8; ++e) p[e] = M::up * __builtin_amdgcn_exp2f(sc[e >> 2][e & 3] - mref);
                 if (__builtin_amdgcn_ballot_w64(mn != m) != 0) {
                     // some head's running max moved: rescale its sum and its O row
                     // (rows are heads 4c + r; their factors come from lanes 4c + r)

@@ -1,0 +1,87 @@
+"""GPU: paged decode attention where scores and weights reach the ends of their
+range, against 64 bits. The inputs make every score exact (or nearly so), so that
+a bound counts the weights and sums alone.
+"""
+import numpy as np
+import pytest
+
+import oracle as O
+from test_gpu_paged import DEV, FORMS, i32
+from util import BF16, to_dev
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0**-24  # half a step of f32, relative
+
+
+def pool(x, dt, q8, quants=None):
+    """x [pages, ps, heads, D] f64 of values that the storage type holds, or Q8_0: quants of that shape, x their
+    scales [.., D / 32] -> (cache, scales, values in f64)"""
+    import torch
+    if not q8:
+        b = O.from_f64(x, dt)
+        return to_dev(b, dt), None, O.to_f64(b, dt)
+    d = x.astype(np.float16)
+    vals = quants.astype(np.float64).reshape(*d.shape, 32) * d.astype(np.float64)[..., None]
+    return torch.from_numpy(quants.astype(np.int8)).to(DEV), torch.from_numpy(d).to(DEV), vals.reshape(quants.shape)
+
+
+def random_values(rng, shape, dt, q8):
+    if not q8:
+        return pool(rng.standard_normal(shape), dt, False)
+    return pool(rng.uniform(0.001, 0.03, (*shape[:3], shape[3] // 32)), dt, True, rng.integers(-127, 128, shape))
+
+
+def softmax_rows(s, V):
+    """softmax(s) V and softmax(s) |V| in f64: s [heads, keys], V [keys, D]"""
+    with np.errstate(invalid="ignore"):
+        p = np.exp(s - s.max(1, keepdims=True))
+    p /= p.sum(1, keepdims=True)
+    return p @ V, p @ np.abs(V)
+
+
+@pytest.mark.parametrize("dt,q8", FORMS)
+@pytest.mark.parametrize("D,n", ((128, 50), (64, 700)))
+@pytest.mark.parametrize("same", (False, True))
+def test_finite_scores_of_any_magnitude(prims, dt, q8, D, n, same):
+    """scores of 2^24 to 2^30 of either sign. A request's keys are of two kinds, t in every dim and t / 2, and q
+    holds a power of two: every product and partial sum of a score is a whole multiple of 2^-2 below 2^24 of its
+    last bit, so scores are exact, equal within a kind, and far enough apart between the kinds that one kind
+    weighs nothing. Weights are then 0 and 1: an output is its kind's mean, off by its sum of n terms (n / 32 + 128
+    additions meet one), the quotient and the scaling (4) and half a step of a 16-bit output."""
+    import torch
+    rng = np.random.default_rng(D + n)
+    R, ps = 24, 16
+    W = -(-n // ps)
+    N = R * W
+    table = rng.permutation(N).reshape(R, W)
+    t = 2048.0 + 85 * np.arange(R)
+    t = np.floor(t / 16) * 16 if dt == BF16 else np.floor(t / 2) * 2  # 8 and 11 bits
+    kind = rng.integers(0, 2, (R, W * ps))
+    kind[:, 0], kind[:, 1] = 0, 1
+    k = np.zeros((N, ps, 1, D))
+    k[table] = (t[:, None] / (1 + kind)).reshape(R, W, ps, 1, 1)
+    if q8:  # quants 64 and 32 of scales t / 64
+        quants = np.zeros((N, ps, 1, D))
+        quants[table] = (64 // (1 + kind)).reshape(R, W, ps, 1, 1)
+        d = np.zeros((N, ps, 1, D // 32))
+        d[table] = (t / 64)[:, None, None, None, None]
+        kc, kd, K = pool(d, dt, True, quants)
+    else:
+        kc, kd, K = pool(k, dt, False)
+    assert np.array_equal(K, k)
+    vc, vd, V = random_values(rng, (N, ps, 1, D), dt, q8)
+    gains = np.array([2048.0, -2048.0, 4096.0, -1024.0, 16384.0, -512.0])
+    q = np.broadcast_to(gains[None, :, None], (R, len(gains), D))
+    dq = to_dev(O.from_f64(np.ascontiguousarray(q), dt), dt)
+    scaling = D**-0.5
+    out = torch.full(q.shape, 7.0, dtype=dq.dtype if same else torch.float32, device=DEV)
+    prims.attn_decode_paged(dq, kc, vc, i32(table), i32([n] * R), scaling, 0, kd, vd, out)
+    got = out.double().cpu().numpy()
+    half = (2.0**-8 if dt == BF16 else 2.0**-11) if same else 0.0
+    for r in range(R):
+        key = np.arange(n)
+        rows = [x[table[r, key // ps], key % ps, 0] for x in (K, V)]
+        ref, mag = softmax_rows(q[r] @ rows[0].T * scaling, rows[1])
+        bound = (n / 32 + 132) * U * mag + half * np.abs(ref) + (2.0**-24 if same else 0.0)
+        assert np.all(np.abs(got[r] - ref) <= bound), (r, t[r], got[r, :, 0].tolist(), ref[:, 0].tolist())
