@@ -25,17 +25,21 @@
 // across the end of a request, and written to LDS;
 // S^T = K Q^T and O += P V run on the matrix cores (16 query heads of the
 // group, zero-padded, as columns), the weights entering as a high and a low
-// 16-bit part (three for f32 outputs), so each is within 2^-16 of p relative.
-// Online softmax in f32 on scores scaled by log2(e).
+// 16-bit part (three of bf16 for f32 outputs), so each is within 2^-16 of p relative
+// down to 2^-100 of the largest. Online softmax in f32 on scores scaled by log2(e).
 //   Pages: lane l holds the slot of key l of the step (its table entry was
 // requested a step before); a load instruction covers 4 to 16 rows, which lie
 // in one page where the page is that large, so one readlane gives their base;
 // else, or where a key is masked, each row's slot comes by a shuffle. The mask
 // is one bit a key, and rows of masked keys are never loaded: what they hold
 // (NaN too) cannot reach the sums.
-//   f16: weights are kept at 2^12 p, so that the low part of a weight down to
-// 2^-26 of the largest is a normal number; sum and output carry the factor. It
-// multiplies the weight: beside a maximum past 2^26 an exponent would lose it.
+//   f16: two parts of 2^15 p are within 2^-19 of p down to p = 2^-21, where the low part
+// ends at f16's smallest step; below it few bits would be left of a weight, which are all
+// that counts behind a key that takes nearly everything and whose value is near zero. A
+// step that holds a smaller weight takes its product in bf16, a value as the exact sum of
+// two bf16 ones. (All steps in bf16: 32 windowed requests 22.3 us for 21.1, 250 short
+// ones 75.2 for 70.6.) The factor multiplies the weight: beside a maximum past 2^26 an
+// exponent would lose it.
 //   Q8_0: quants become bf16, or f16 beside f16 queries, on their way from LDS,
 // exactly (8 bits); a K block's scale multiplies its 32-dim part of the score, a
 // V block's its weights before they are split, so no value is rounded to 16 bits.
@@ -84,7 +88,6 @@ namespace mg
     struct Mm<SBf16>
     {
         using x8 = bf16x8;
-        static constexpr float up = 1.0f; // the weights' factor
         static MG_DEV f32x4 mma(x8 a, x8 b, f32x4 c) { return mfma_bf16(a, b, c); }
         static MG_DEV uint32_t pack(float a, float b) // (bf_pack, without its copies of values that live on)
         {
@@ -99,7 +102,6 @@ namespace mg
     struct Mm<SF16>
     {
         using x8 = f16x8;
-        static constexpr float up = 0x1p12f;
         static MG_DEV f32x4 mma(x8 a, x8 b, f32x4 c) { return mfma_f16(a, b, c); }
         static MG_DEV uint32_t pack(float a, float b)
         {
@@ -115,9 +117,9 @@ namespace mg
     {
         return __builtin_bit_cast(X8, *reinterpret_cast<const Vec<uint32_t, 4> *>(p));
     }
-    // two weights as sums of NP 16-bit parts, each the rest's nearest, as the pair `at` of NP operands
+    // two values as sums of NP 16-bit parts, each the rest's nearest, as the pair `at` of NP operands
     template <class M, int NP>
-    MG_DEV void split_weights(float p0, float p1, Vec<uint32_t, 4> (&w)[NP], int at)
+    MG_DEV void split(float p0, float p1, Vec<uint32_t, 4> (&w)[NP], int at)
     {
 #pragma unroll
         for (int k = 0; k < NP; ++k) {
@@ -236,13 +238,15 @@ namespace mg
         constexpr int SO4 = D + 4;                // row stride of a wave's output in LDS (floats)
         constexpr int WB = 32 * (SK + SV);        // LDS bytes of a wave's K and V
         static_assert(16 * SO4 * 4 <= WB, "a wave's output takes the place of its K and V");
-        using MS = Mm<S>;                               // the scores' product, at q's type
-        using M = Mm<std::conditional_t<Q8, SBf16, S>>; // the outputs'
-        using x8 = typename M::x8;
+        using MS = Mm<S>; // the scores' product, at q's type
         using raw = typename SO::raw;
-        // parts of a weight: two bf16 ones leave 2^-17 of it at most, 1.5e-6 of an output (2-norm), which f32
-        // outputs would show (three: 3e-7) and 16-bit ones do not; two f16 ones 2^-22
-        constexpr int NP = SO::dt == F32 && std::is_same_v<M, Mm<SBf16>> ? 3 : 2;
+        // f16 values: the output's product in f16 where a step's weights allow, else in bf16
+        constexpr bool F = S::dt == F16 && !Q8;
+        constexpr float up = F ? 0x1p15f : 1.0f; // the weights' factor
+        constexpr float kSmall = 0x1p-6f;        // a weight below 2^-21, with its factor
+        // bf16 parts of a weight: two leave 2^-17 of it at most, 1.5e-6 of an output (2-norm), which f32
+        // outputs would show (three: 3e-7) and 16-bit ones do not
+        constexpr int NPB = SO::dt == F32 ? 3 : 2;
         constexpr float kLow = -__builtin_huge_valf();
         __shared__ __align__(16) char lds[4][WB];
         __shared__ __align__(16) float scl[Q8 ? 4 : 1][2][KB][32];
@@ -425,7 +429,7 @@ namespace mg
                         }
                     } else {
 #pragma unroll
-                        for (int i = 0; i < KB; ++i) st = MS::mma(__builtin_bit_cast(x8, kt[t][i]), qop[i], st);
+                        for (int i = 0; i < KB; ++i) st = MS::mma(__builtin_bit_cast(typename MS::x8, kt[t][i]), qop[i], st);
                     }
 #pragma unroll
                     for (int r = 0; r < 4; ++r) sc[t][r] = st[r] * a.scale2;
@@ -445,7 +449,7 @@ namespace mg
                 // weights: element 4t + r of lane (head n, c) is key 16 t + 4c + r
                 float p[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) p[e] = M::up * __builtin_amdgcn_exp2f(sc[e >> 2][e & 3] - mref);
+                for (int e = 0; e < 8; ++e) p[e] = up * __builtin_amdgcn_exp2f(sc[e >> 2][e & 3] - mref);
                 if (__builtin_amdgcn_ballot_w64(mn != m) != 0) {
                     // some head's running max moved: rescale its sum and its O row
                     // (rows are heads 4c + r; their factors come from lanes 4c + r)
@@ -465,34 +469,62 @@ namespace mg
                 // of dim 16 s + n, through the transposing read
                 const char *vr = Q8 ? sv + (16 * (n >> 3) + 4 * c + (n >> 1 & 3)) * SV + 8 * (n & 1)
                                     : sv + (4 * c + (n >> 2)) * SV + 8 * (n & 3);
-                Vec<uint32_t, 4> w[NP];
+                auto outputs = [&](auto in_f16) {
+                    using M = Mm<std::conditional_t<decltype(in_f16)::value, SF16, SBf16>>;
+                    using x8 = typename M::x8;
+                    constexpr int NP = decltype(in_f16)::value ? 2 : NPB; // parts of a weight
+                    constexpr int NV = F && !decltype(in_f16)::value ? 2 : 1; // parts of a value: f16's 11 bits are 8 and 3
+                    Vec<uint32_t, 4> w[NP];
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    if constexpr (Q8) {
-                        if (t % 2 == 0) {
-                            const float *d = scl[wv][1][t / 2] + 4 * c;
-                            const Vec<float, 4> d0 = *reinterpret_cast<const Vec<float, 4> *>(d);
-                            const Vec<float, 4> d1 = *reinterpret_cast<const Vec<float, 4> *>(d + 16);
+                    for (int t = 0; t < NT; ++t) {
+                        if constexpr (Q8) {
+                            if (t % 2 == 0) {
+                                const float *d = scl[wv][1][t / 2] + 4 * c;
+                                const Vec<float, 4> d0 = *reinterpret_cast<const Vec<float, 4> *>(d);
+                                const Vec<float, 4> d1 = *reinterpret_cast<const Vec<float, 4> *>(d + 16);
 #pragma unroll
-                            for (int e = 0; e < 4; e += 2) {
-                                split_weights<M, NP>(p[e] * d0.v[e], p[e + 1] * d0.v[e + 1], w, e / 2);
-                                split_weights<M, NP>(p[4 + e] * d1.v[e], p[5 + e] * d1.v[e + 1], w, 2 + e / 2);
+                                for (int e = 0; e < 4; e += 2) {
+                                    split<M, NP>(p[e] * d0.v[e], p[e + 1] * d0.v[e + 1], w, e / 2);
+                                    split<M, NP>(p[4 + e] * d1.v[e], p[5 + e] * d1.v[e + 1], w, 2 + e / 2);
+                                }
+                            }
+                        } else if (t == 0) {
+#pragma unroll
+                            for (int e = 0; e < 8; e += 2) split<M, NP>(p[e], p[e + 1], w, e / 2);
+                        }
+                        Vec<uint32_t, 4> vb[NV];
+                        if constexpr (Q8) {
+                            vb[0] = __builtin_bit_cast(Vec<uint32_t, 4>, q8_bf16(lds_read_tr8(vr + 16 * t)));
+                        } else {
+                            const bf16x4 v0 = lds_read_tr(reinterpret_cast<const uint16_t *>(vr + 32 * t));
+                            const bf16x4 v1 = lds_read_tr(reinterpret_cast<const uint16_t *>(vr + 16 * SV + 32 * t));
+                            vb[0] = __builtin_bit_cast(Vec<uint32_t, 4>,
+                                                       bf16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
+                            if constexpr (NV == 2) {
+                                const Vec<uint32_t, 4> x = vb[0];
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    split<M, NV>(f16_f32(uint16_t(x.v[i])), f16_f32(uint16_t(x.v[i] >> 16)), vb, i);
                             }
                         }
-                    } else if (t == 0) {
+                        // (a weight's third part times a value's second, 2^-26 of their product, is left out)
 #pragma unroll
-                        for (int e = 0; e < 8; e += 2) split_weights<M, NP>(p[e], p[e + 1], w, e / 2);
-                    }
-                    x8 vb;
-                    if constexpr (Q8) {
-                        vb = q8_bf16(lds_read_tr8(vr + 16 * t));
-                    } else {
-                        const bf16x4 v0 = lds_read_tr(reinterpret_cast<const uint16_t *>(vr + 32 * t));
-                        const bf16x4 v1 = lds_read_tr(reinterpret_cast<const uint16_t *>(vr + 16 * SV + 32 * t));
-                        vb = __builtin_bit_cast(x8, bf16x8{v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]});
-                    }
+                        for (int k = 0; k < NP; ++k)
 #pragma unroll
-                    for (int k = 0; k < NP; ++k) o[t] = M::mma(__builtin_bit_cast(x8, w[k]), vb, o[t]);
+                            for (int i = 0; i < NV && k + i < 3; ++i)
+                                o[t] = M::mma(__builtin_bit_cast(x8, w[k]), __builtin_bit_cast(x8, vb[i]), o[t]);
+                    }
+                };
+                if constexpr (F) {
+                    uint32_t least = 0xffffffffu; // of the weights' bits, less 1: a zero weight (a masked key's) is none
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) least = min(least, __builtin_bit_cast(uint32_t, p[e]) - 1u);
+                    if (__builtin_amdgcn_ballot_w64(least < __builtin_bit_cast(uint32_t, kSmall) - 1u) == 0)
+                        outputs(std::true_type{});
+                    else
+                        outputs(std::false_type{});
+                } else {
+                    outputs(std::false_type{});
                 }
                 wave_lds_sync(); // this step's reads are done before the next one's writes
             } while (more);

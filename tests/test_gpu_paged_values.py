@@ -85,3 +85,63 @@ def test_finite_scores_of_any_magnitude(prims, dt, q8, D, n, same):
         ref, mag = softmax_rows(q[r] @ rows[0].T * scaling, rows[1])
         bound = (n / 32 + 132) * U * mag + half * np.abs(ref) + (2.0**-24 if same else 0.0)
         assert np.all(np.abs(got[r] - ref) <= bound), (r, t[r], got[r, :, 0].tolist(), ref[:, 0].tolist())
+
+
+@pytest.mark.parametrize("dt,q8", FORMS)
+@pytest.mark.parametrize("D,n,at", ((128, 40, 0), (64, 900, 0), (128, 900, 555)))
+@pytest.mark.parametrize("same", (False, True))
+def test_small_weights_behind_one_key(prims, dt, q8, D, n, at, same):
+    """one key (at `at`) takes nearly everything, and its value is zero in half of the dims: there an output is made
+    of the other keys' weights alone, 2^-13 to 2^-100 of its own. q and k are zero but for one dim, q is a power of
+    two and the large key's score is 0, so a score s (in units of log 2) is off by the roundings of the scaling and
+    of their product, 2 U |s|, and enters the weight once: relative 2 U |s| log 2; exponential and quotient 8 U; the
+    weight's parts 2^-16; its sum (n / 32 + 128) U; half a step of a 16-bit output."""
+    import torch
+    rng = np.random.default_rng(D + n + at)
+    gaps = np.array([13, 16, 19, 21, 24, 26, 30, 34, 37, 40, 50, 64, 80, 99])  # of each request
+    R, ps = len(gaps), 16
+    W = -(-n // ps)
+    N = R * W
+    table = rng.permutation(N).reshape(R, W)
+    # the others' scores: from the gap to one unit above it, in 64 steps, over log 2 and the gain
+    key = np.arange(W * ps)
+    k0 = (gaps[:, None] - (key * 37 % 64) / 64) * 0.7
+    k0[:, at] = 0.0
+    k = np.zeros((N, ps, 1, D))
+    if q8:
+        quants = np.zeros((N, ps, 1, D))
+        d = np.zeros((N, ps, 1, D // 32))
+        quants[table, :, 0, 0] = np.where(k0 > 0, 100, 0).reshape(R, W, ps)
+        d[table, :, 0, 0] = (k0 / 100).reshape(R, W, ps)
+        kc, kd, K = pool(d, dt, True, quants)
+    else:
+        k[table, :, 0, 0] = k0.reshape(R, W, ps)
+        kc, kd, K = pool(k, dt, False)
+    if q8:
+        vq = rng.integers(-127, 128, (N, ps, 1, D))
+        vd_ = rng.uniform(0.001, 0.03, (N, ps, 1, D // 32))
+        vq[table[:, at // ps], at % ps, 0, :D // 2] = 0
+        vc, vd, V = pool(vd_, dt, True, vq)
+    else:
+        v = rng.standard_normal((N, ps, 1, D))
+        v[table[:, at // ps], at % ps, 0, :D // 2] = 0.0
+        vc, vd, V = pool(v, dt, False)
+    q = np.zeros((R, 3, D))
+    q[:, :, 0] = -1.0
+    dq = to_dev(O.from_f64(q, dt), dt)
+    out = torch.full(q.shape, 7.0, dtype=dq.dtype if same else torch.float32, device=DEV)
+    prims.attn_decode_paged(dq, kc, vc, i32(table), i32([n] * R), 1.0, 0, kd, vd, out)
+    got = out.double().cpu().numpy()
+    half = (2.0**-8 if dt == BF16 else 2.0**-11) if same else 0.0
+    tiny = 2.0**-25 if same and dt != BF16 else 0.0  # half of f16's smallest step
+    worst = []
+    for r in range(R):
+        j = np.arange(n)
+        kr, vr = (x[table[r, j // ps], j % ps, 0] for x in (K, V))
+        s = q[r] @ kr.T
+        ref, mag = softmax_rows(s, vr)
+        err = 2 * U * np.abs(s).max() + (8 + n / 32 + 128) * U + 2.0**-16
+        bound = err * mag + half * np.abs(ref) + tiny
+        assert np.abs(ref[:, :D // 2]).max() < 2.0**(-gaps[r] * 0.99 + 14)  # (these dims do hold small weights only)
+        worst.append((int(gaps[r]), float((np.abs(got[r] - ref) / np.maximum(bound, 1e-300)).max())))
+    assert all(w <= 1 for _, w in worst), worst
