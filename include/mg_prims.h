@@ -307,7 +307,10 @@ int mg_qk_norm_rope_paged(mg_ctx *ctx, void *q, int64_t q_heads, int64_t ldq, vo
  * gives zeros; a key whose page lies outside the pool is left out, as a masked
  * one; what the pool holds behind a request's length or before its window is
  * never used. An attended value that is not finite makes the outputs it enters
- * not finite (an infinite one may give NaN). head_dim 64 or 128; any number of
+ * not finite (an infinite one may give NaN), but a key whose score is -inf weighs
+ * nothing beside a larger score; scores of -inf alone give NaN. Scores and sums
+ * are f32: a score past its range is infinite, and a bf16 value past 2^127 / lens[r]
+ * may make its sum so. head_dim 64 or 128; any number of
  * query heads per kv head; at most 65535 requests, 2^31 - 1 slots in the pool and
  * tables (or windows of them) of fewer than 2^38 keys. A numerical envelope, not
  * bits: f32 sums and weights to 2^-16 relative (those down to 2^-100 of the

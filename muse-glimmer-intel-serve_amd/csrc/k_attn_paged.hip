@@ -7,7 +7,8 @@
 // [slots, kv_heads, head_dim]:
 //   s_j = (q_bh . k_j) * scaling,   out_bh = sum_j softmax(s)_j v_j.
 // A request without keys gives zeros. A key whose page is outside the pool is
-// left out, as a masked one. Q8_0 pages hold k_j and v_j as q * d, exactly.
+// left out, as a masked one. A score of -inf weighs nothing beside a larger one;
+// a request that has only such scores gives NaN, as the quotient 0 / 0 is. Q8_0 pages hold k_j and v_j as q * d, exactly.
 //
 // Division of the work (mg_paged_plan.hpp): the requests' keys form one line of
 // units, cut into equal runs; a team of work-groups, one for every KV head (and
@@ -166,6 +167,14 @@ namespace mg
         typedef int i32x2 __attribute__((ext_vector_type(2)));
         typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
         return __builtin_bit_cast(Vec<uint32_t, 2>, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2 *)(p)));
+    }
+
+    // the factor of a part whose maximum is m beside the maximum `top` >= m of all (both may be -inf)
+    MG_DEV float weight_of(float m, float top) { return m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top); }
+    // what an output is multiplied by: 1 / sum; without a score above -inf 0 where there is no key, else NaN
+    MG_DEV float inverse(float sum, float top)
+    {
+        return top > -__builtin_huge_valf() ? 1.0f / sum : sum == 0.0f ? 0.0f : __builtin_nanf("");
     }
 
     // the work-group's run [u0, u1) of its team, the request it starts in and that request's first unit p
@@ -374,6 +383,7 @@ namespace mg
 #pragma unroll
             for (int t = 0; t < NT; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             float m = kLow, l = 0.0f; // head n (replicated over c)
+            bool any = false;         // the wave has seen a key that is not masked
             int kb = cur.k0 + kPagedStep * wv;
             bool more;
             do {
@@ -400,6 +410,7 @@ namespace mg
                     slot = slot_of();
                 }
                 if (now == 0) continue;
+                any = true;
                 // K as A of S^T: lane (key n, c) holds dims 32 i + 8c.. of key 16 t + n
                 Vec<uint32_t, EPL == 16 ? 2 : 4> kt[2][KB];
 #pragma unroll
@@ -539,9 +550,11 @@ namespace mg
             // join the four waves: their outputs take the place of K and V in LDS
             l = rows4_sum(l);
             float *so = reinterpret_cast<float *>(lds[wv]);
+            // keys, but none above -inf: the sum, 0 (or NaN), says so by 1. Beside a maximum it weighs 0; where no
+            // part has one the parts' sums are added as they are, and 0 means that nothing was attended.
             if (c == 0) {
                 wm[wv][n] = m;
-                wl[wv][n] = l;
+                wl[wv][n] = any && m == kLow ? l + 1.0f : l;
             }
 #pragma unroll
             for (int t = 0; t < NT; ++t)
@@ -560,13 +573,12 @@ namespace mg
             const int hh = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (D / 16);
             if (hh < a.hw) {
                 const float top = __builtin_fmaxf(__builtin_fmaxf(wm[0][hh], wm[1][hh]), __builtin_fmaxf(wm[2][hh], wm[3][hh]));
-                const float ref = top == kLow ? 0.0f : top;
                 float sum = 0.0f, acc[D / 16];
 #pragma unroll
                 for (int e = 0; e < D / 16; ++e) acc[e] = 0.0f;
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    const float f = __builtin_amdgcn_exp2f(wm[w][hh] - ref);
+                    const float f = weight_of(wm[w][hh], top);
                     sum = __builtin_fmaf(f, wl[w][hh], sum);
                     const float *src = reinterpret_cast<const float *>(lds[w]) + hh * SO4 + d0;
 #pragma unroll
@@ -577,7 +589,7 @@ namespace mg
                     }
                 }
                 if (whole) {
-                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    const float inv = inverse(sum, top);
                     raw *dst = static_cast<raw *>(a.out) + cur.b * a.ldo + int64_t(h0 + hh) * D + d0;
 #pragma unroll
                     for (int e = 0; e < D / 16; ++e) dst[e] = SO::enc32(acc[e] * inv);
@@ -649,7 +661,7 @@ namespace mg
         auto add = [&](float ref) {
 #pragma unroll
             for (int k = 0; k < P; ++k) {
-                const float f = __builtin_amdgcn_exp2f(pm[k] - ref);
+                const float f = weight_of(pm[k], ref);
                 sum = __builtin_fmaf(f, pl[k], sum);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc.v[i] = __builtin_fmaf(f, px[k].v[i], acc.v[i]);
@@ -660,16 +672,15 @@ namespace mg
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc.v[i] *= f;
         };
-        auto ref_of = [&](float t) { return t == kLow ? 0.0f : t; };
         const bool few = nt <= P * SG; // one batch: weighed by the maximum of all threads at once
         load(sg);
         if (!few) {
-            add(ref_of(top));
+            add(top);
             for (int s0 = sg + P * SG; s0 < nt; s0 += P * SG) {
                 const float was = top;
                 load(s0);
-                scale(__builtin_amdgcn_exp2f(was - ref_of(top)));
-                add(ref_of(top));
+                scale(weight_of(was, top));
+                add(top);
             }
         }
         tops[sg][e] = top;
@@ -678,9 +689,9 @@ namespace mg
 #pragma unroll
         for (int s = 0; s < SG; ++s) all = __builtin_fmaxf(all, tops[s][e]);
         if (few)
-            add(ref_of(all));
+            add(all);
         else
-            scale(__builtin_amdgcn_exp2f(top - ref_of(all)));
+            scale(weight_of(top, all));
         sums[sg][e] = sum;
         accs[sg][e] = acc;
         __syncthreads();
@@ -693,7 +704,7 @@ namespace mg
 #pragma unroll
             for (int i = 0; i < 4; ++i) acc.v[i] += accs[s][e].v[i];
         }
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const float inv = inverse(sum, all);
         const int nsub = a.hpg / a.hw, g = v / nsub;
         const int h0 = g * a.hpg + (v - g * nsub) * a.hw;
         typename SO::raw *dst = static_cast<typename SO::raw *>(a.out) + cut.x * a.ldo + int64_t(h0) * D + i0;

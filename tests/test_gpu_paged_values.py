@@ -145,3 +145,71 @@ def test_small_weights_behind_one_key(prims, dt, q8, D, n, at, same):
         assert np.abs(ref[:, :D // 2]).max() < 2.0**(-gaps[r] * 0.99 + 14)  # (these dims do hold small weights only)
         worst.append((int(gaps[r]), float((np.abs(got[r] - ref) / np.maximum(bound, 1e-300)).max())))
     assert all(w <= 1 for _, w in worst), worst
+
+
+def infinite_keys(D, dt, q8, pages, ps, nkv, seed):
+    """a pool of ordinary keys and values, and a function that gives key (page, place) of head 1 the score -inf"""
+    import torch
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    shape = (pages, ps, nkv, D)
+    if not q8:
+        t = torch.bfloat16 if dt == BF16 else torch.float16
+        kc, vc = (torch.randn(shape, generator=g, device=DEV).to(t) for _ in range(2))
+
+        def spoil(page, place):
+            kc[page, place, 1, 3] = -float("inf")
+        return kc, vc, None, None, spoil
+    kc, vc = (torch.randint(-127, 128, shape, generator=g, device=DEV, dtype=torch.int8) for _ in range(2))
+    kd, vd = (torch.full((*shape[:3], D // 32), 0.01, dtype=torch.float16, device=DEV) for _ in range(2))
+
+    def spoil(page, place):
+        kc[page, place, 1, :32] = -5
+        kd[page, place, 1, 0] = float("inf")
+    return kc, vc, kd, vd, spoil
+
+
+@pytest.mark.parametrize("dt,q8", FORMS)
+@pytest.mark.parametrize("D,lens,teams", ((128, [40, 5, 300], None), (64, [9000, 33, 700], None), (128, [30000], None),
+                                          (64, [200] * 80, 64), (64, [3000] * 3, 64)))
+def test_scores_of_minus_infinity(prims, dt, q8, D, lens, teams):
+    """a softmax over scores of -inf alone is NaN, for that request and kv head only and however its keys are split;
+    with one finite score among them that key takes all; keys left out (bad pages) do not count, and a request with
+    such keys only gives zeros"""
+    import mgprims
+    import torch
+    ps, nkv, R = 16, 2, len(lens)
+    W = -(-max(lens) // ps)
+    kc, vc, kd, vd, spoil = infinite_keys(D, dt, q8, R * W, ps, nkv, D + R)
+    table = torch.arange(R * W, device=DEV).int().view(R, W)
+    q = torch.rand((R, 6, D), device=DEV).add_(0.25).to(torch.bfloat16 if dt == BF16 else torch.float16)
+    n = i32(lens)
+    p = mgprims.Prims(0, workspace_bytes=teams) if teams else prims  # (no room for partial results: nothing is cut)
+    run = lambda t=table, w=0: p.attn_decode_paged(q, kc, vc, t, n, 0.1, w, kd, vd)
+    base = run()
+    assert torch.isfinite(base).all()
+    r = R - 1
+    rows = slice(r * W, (r + 1) * W)
+    spoil(rows, slice(None))
+    got = run()
+    assert torch.isnan(got[r, 3:]).all()
+    got[r, 3:] = base[r, 3:]
+    assert torch.equal(got, base)
+    assert torch.isnan(run(w=3)[r, 3:]).all()
+    out_of_pool = table.clone()
+    out_of_pool[r, 0] = -1  # some left out: still NaN where others are left
+    assert torch.isnan(run(out_of_pool)[r, 3:]).all() == (lens[r] > ps)
+    out_of_pool[r] = R * W
+    assert not run(out_of_pool)[r].any()
+    # one finite key
+    at = lens[r] // 2
+    page, place = r * W + at // ps, at % ps
+    if q8:
+        kd[page, place, 1, 0] = 0.01
+        value = vc[page, place, 1].float() * vd[page, place, 1, 0].float()
+    else:
+        kc[page, place, 1, 3] = 1.0
+        value = vc[page, place, 1].float()
+    # (its weight is 1: quotient and products exact, but for a Q8_0 value's scale in two or three parts)
+    assert torch.allclose(run()[r, 3:], value.expand(3, D), rtol=2.0**-16, atol=0)
+    if teams:
+        p.close()
