@@ -6,6 +6,7 @@ import numpy as np
 import pytest
 
 import oracle as O
+import paged_oracle as PO
 from test_gpu_paged import DEV, FORMS, i32
 from util import BF16, to_dev
 
@@ -213,3 +214,45 @@ def test_scores_of_minus_infinity(prims, dt, q8, D, lens, teams):
     assert torch.allclose(run()[r, 3:], value.expand(3, D), rtol=2.0**-16, atol=0)
     if teams:
         p.close()
+
+
+@pytest.mark.parametrize("dt,q8", FORMS)
+@pytest.mark.parametrize("D,ps", ((64, 16), (128, 64), (128, 1)))
+@pytest.mark.parametrize("window", (1, 31, 100, 1000))
+@pytest.mark.parametrize("freed", ("bad", "foreign"))
+def test_nothing_before_a_window_is_used(prims, dt, q8, D, ps, window, freed):
+    """pages behind a sliding window have gone: what the window's first page holds before it is NaN, table entries
+    before it are outside the pool or pages of NaN; every request equals one of the window's own keys alone"""
+    import torch
+    rng = np.random.default_rng(D + ps + window)
+    lens = [0, 1, window, window + 1, window + 17, 333, 2077]
+    R, W = len(lens), 2077 // ps + 2
+    kept = [(max(0, n - window), n) for n in lens]
+    pages = [list(range(lo // ps, -(-n // ps))) for lo, n in kept]
+    N = sum(map(len, pages)) + 1  # the last one is nobody's
+    perm = rng.permutation(N - 1)
+    table = rng.integers(N, 2 * N, (R, W)) if freed == "bad" else np.full((R, W), N - 1)
+    used = np.zeros((N, ps), bool)
+    at = 0
+    for r, (lo, n) in enumerate(kept):
+        for pg in pages[r]:
+            table[r, pg] = perm[at]
+            j = np.arange(pg * ps, (pg + 1) * ps)
+            used[perm[at]] = (j >= lo) & (j < n)
+            at += 1
+    caches, plain = [], []
+    for _ in range(2):
+        c, d, x = random_values(rng, (N, ps, 1, D), dt, q8)
+        (d if q8 else c)[torch.from_numpy(~used).to(DEV)] = float("nan")
+        caches.append((c, d))
+        plain.append(x)
+    q = rng.standard_normal((R, 3, D))
+    dq = to_dev(O.from_f64(q, dt), dt)
+    (kc, kd), (vc, vd) = caches
+    got = prims.attn_decode_paged(dq, kc, vc, i32(table), i32(lens), 0.1, window, kd, vd).double().cpu().numpy()
+    qf = dq.double().cpu().numpy()
+    for r, (lo, n) in enumerate(kept):
+        j = np.arange(lo, n)
+        K, V = (x[table[r, j // ps], j % ps] for x in plain)  # [keys, 1, D]
+        ref, bound = PO.attn_decode(qf[r:r + 1], K[:, None], V[:, None], np.arange(len(j))[None], [len(j)], 1, 0, 0.1)
+        assert np.all(np.abs(got[r] - ref[0]) <= bound[0]), r
