@@ -66,18 +66,14 @@ namespace mg
         const int32_t *table, *lens;
         void *out;
         float *part;     // [2 teams, vh, hw, D] outputs, then [2 teams, vh, hw] maxima and sums
-        int4 *cut;       // [requests] or [teams]: what the second kernel joins (Cut)
-        int by_team;     // a Cut for each team (there are fewer than requests), not for each request
+        PagedCut *cut;   // [requests] or, by_team, [teams]: what the second kernel joins
+        int by_team;
         int64_t ldq, ldt, ldo, window;
         int R, nkv, W, sh, num_pages;
         int hpg, hw, vh; // query heads a kv head, a work-group; work-groups a team
         int teams;
         float scale2;    // scaling * log2(e)
     };
-
-    // PagedArgs::cut, for a request (or for the request that begins in a team and passes its end): x the request, y
-    // the number of its partial results (0: none), z the first one's place, w the team of the second; each team
-    // behind the first begins with the request, so its part is at 2 t
 
     typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
     MG_DEV f32x4 mfma_f16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
@@ -275,7 +271,7 @@ namespace mg
         const Run run = find_run(a, team);
         const bool notes = a.teams > 1 && v == 0 && threadIdx.x == 0; // who writes the cuts down
         if (run.u0 >= run.u1) { // the whole work-group
-            if (notes && a.by_team) a.cut[team] = int4{0, 0, 0, 0};
+            if (notes && a.by_team) a.cut[team] = PagedCut{};
             return;
         }
         const int nsub = a.hpg / a.hw, g = v / nsub;
@@ -562,14 +558,10 @@ namespace mg
                 for (int r = 0; r < 4; ++r) so[(4 * c + r) * SO4 + 16 * t + n] = o[t][r];
             __syncthreads();
             const bool whole = cur.at == 0 && cur.end == cur.units;
-            if (notes && (a.by_team ? cur.behind == 0 : cur.at == 0)) {
-                int4 cut{cur.b, 0, 2 * team + (cur.b == run.b ? 0 : 1), team + 1};
-                if (cur.at == 0 && !whole) {
-                    const int first = run.u1 - cur.behind - cur.end; // the request's first unit
-                    cut.y = team_of(run.d, first + cur.units - 1) - team + 1;
-                }
-                a.cut[a.by_team ? team : cur.b] = cut;
-            }
+            const int first = run.u1 - cur.behind - cur.end; // the request's first unit
+            if (notes && leaves_cut(a.by_team, cur.at, cur.behind))
+                a.cut[a.by_team ? team : cur.b] =
+                    cur.at == 0 ? paged_cut(run.d, team, cur.b, first, cur.units) : PagedCut{};
             const int hh = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (D / 16);
             if (hh < a.hw) {
                 const float top = __builtin_fmaxf(__builtin_fmaxf(wm[0][hh], wm[1][hh]), __builtin_fmaxf(wm[2][hh], wm[3][hh]));
@@ -594,8 +586,7 @@ namespace mg
 #pragma unroll
                     for (int e = 0; e < D / 16; ++e) dst[e] = SO::enc32(acc[e] * inv);
                 } else {
-                    const int64_t pl = 2 * int64_t(team) + (cur.b == run.b ? 0 : 1);
-                    const int64_t row = (pl * a.vh + v) * a.hw + hh;
+                    const int64_t row = (int64_t(team_place(run.d, team, first)) * a.vh + v) * a.hw + hh;
                     float *dst = a.part + row * D + d0;
 #pragma unroll
                     for (int e = 0; e < D / 16; e += 4)
@@ -623,18 +614,15 @@ namespace mg
         constexpr int SG = 256 / E;
         __shared__ float tops[SG][E], sums[SG][E];
         __shared__ Vec<float, 4> accs[SG][E];
-        const int4 cut = a.cut[blockIdx.x];
-        const int nt = cut.y;
+        const PagedCut cut = a.cut[blockIdx.x];
+        const int nt = cut.parts;
         if (nt == 0) return; // finished in its team
         const int v = blockIdx.y, e = threadIdx.x % E, sg = threadIdx.x / E;
         const int i0 = (int(blockIdx.z) * E + e) * 4; // the thread's outputs among [hw, D]
         const bool live = i0 < a.hw * D;
         const int hh = live ? i0 / D : 0; // (a work-group's outputs may be of several heads)
         const float *ml = a.part + 2 * int64_t(a.teams) * a.vh * a.hw * D;
-        auto row = [&](int s) {
-            const int place = s == 0 ? cut.z : 2 * (cut.w + s - 1);
-            return (int64_t(place) * a.vh + v) * a.hw;
-        };
+        auto row = [&](int s) { return (int64_t(cut_place(cut, s)) * a.vh + v) * a.hw; };
         // P parts' maxima, sums and outputs are in flight at once (5 requests of 77 parts: 6.4 us with four, 4.8 with
         // eight); a thread with more takes them in batches, joined as scores are
         constexpr int P = E <= 16 ? 8 : 4;
@@ -707,7 +695,7 @@ namespace mg
         const float inv = inverse(sum, all);
         const int nsub = a.hpg / a.hw, g = v / nsub;
         const int h0 = g * a.hpg + (v - g * nsub) * a.hw;
-        typename SO::raw *dst = static_cast<typename SO::raw *>(a.out) + cut.x * a.ldo + int64_t(h0) * D + i0;
+        typename SO::raw *dst = static_cast<typename SO::raw *>(a.out) + cut.request * a.ldo + int64_t(h0) * D + i0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) dst[i] = SO::enc32(acc.v[i] * inv);
     }
@@ -756,13 +744,13 @@ namespace mg
         int64_t teams = per_cu * int64_t(c->num_cus) / vh;
         teams = teams < most ? teams : most;
         // (the cuts, then the partial results' outputs, then their maxima and sums)
-        const int64_t tbytes = 2 * vh * hw * (D + 2) * int64_t(sizeof(float)) + int64_t(sizeof(int4));
+        const int64_t tbytes = 2 * vh * hw * (D + 2) * int64_t(sizeof(float)) + int64_t(sizeof(PagedCut));
         teams = teams < c->work_bytes / tbytes ? teams : c->work_bytes / tbytes;
         teams = teams > 1 ? teams : 1;
-        const bool by_team = teams < seqs; // else there is room for a cut of each request among the teams'
+        const bool by_team = cuts_by_team(teams, seqs); // else there is room for a cut of each request among the teams'
         PagedArgs a{};
         a.q = q, a.kc = kc, a.vc = vc, a.kd = kd, a.vd = vd, a.table = table, a.lens = lens, a.out = out;
-        a.cut = static_cast<int4 *>(c->work);
+        a.cut = static_cast<PagedCut *>(c->work);
         a.part = reinterpret_cast<float *>(a.cut + teams);
         a.by_team = by_team;
         a.ldq = ldq, a.ldt = ldt, a.ldo = ldo, a.window = window;
@@ -781,7 +769,7 @@ namespace mg
             else
                 D == 128 ? go(k_attn_paged<S, SO, false, 4>) : go(k_attn_paged<S, SO, false, 2>);
             if (teams == 1) return; // nothing is cut
-            const int64_t who = by_team ? teams - 1 : seqs; // (the last team's end cuts nothing)
+            const int64_t who = cuts_kept(teams, seqs);
             auto join = [&](auto kern, int e) {
                 const dim3 grid{unsigned(who), unsigned(vh), unsigned((hw * D + 4 * e - 1) / (4 * e))};
                 hipLaunchKernelGGL(kern, grid, dim3(256), 0, c->stream, a, int(D));

@@ -66,4 +66,26 @@ namespace mg
     }
     // where team t leaves its partial result of the request whose first unit is p
     MG_HD int team_place(const PagedTeams &d, int t, int p) { return 2 * t + (team_first(d, t) < p ? 1 : 0); }
+
+    // What the join of a request reads: how many partial results it has (0: finished in its team), the place of the
+    // first and the team of the second. Every team behind the first begins with the request.
+    struct alignas(16) PagedCut
+    {
+        int request, parts, first, second;
+    };
+    // the request of `units` units from unit p on, which begins in team t
+    MG_HD PagedCut paged_cut(const PagedTeams &d, int t, int request, int p, int units)
+    {
+        const int behind = team_of(d, p + units - 1) - t;
+        return PagedCut{request, behind > 0 ? behind + 1 : 0, team_place(d, t, p), t + 1};
+    }
+    // the place of a request's partial result s < parts
+    MG_HD int cut_place(const PagedCut &c, int s) { return s == 0 ? c.first : 2 * (c.second + s - 1); }
+
+    // Notes are kept for each request by the team it begins in, or, of fewer teams than requests, for each team
+    // but the last by the team itself: of its last part, which only the team's end can cut.
+    MG_HD bool cuts_by_team(int64_t teams, int64_t requests) { return teams < requests; }
+    MG_HD int64_t cuts_kept(int64_t teams, int64_t requests) { return cuts_by_team(teams, requests) ? teams - 1 : requests; }
+    // whether a team's part from its request's unit `at` on, with `behind` units of the team behind it, leaves a note
+    MG_HD bool leaves_cut(bool by_team, int at, int behind) { return by_team ? behind == 0 : at == 0; }
 } // namespace mg
