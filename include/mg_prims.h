@@ -162,7 +162,8 @@ int mg_rope(mg_ctx *ctx, void *q, int64_t q_heads, int64_t ldq, void *k, int64_t
  *   the caches are [cache_slots, k_heads, head_dim] (the ring of k_kv_append);
  *   two tokens of one call that map to one slot race, as in the reference.
  * Each step rounds to `dtype` exactly as mg_rmsnorm_rows, mg_scale and mg_rope
- * do, so the result is bit-identical to running them in sequence
+ * do, so the result is bit-identical to running them in sequence, but for the
+ * sign of an f16 NaN
  * (MG_F64 | MG_F32_COMPAT: the QK-norm takes the f32 chain, 801-803).
  * ldq/ldk/ldv: token strides in elements (0 = heads*head_dim). */
 int mg_qk_norm_rope(mg_ctx *ctx, void *q, int64_t q_heads, int64_t ldq, void *k, int64_t k_heads,
@@ -274,7 +275,9 @@ int mg_attn_decode(mg_ctx *ctx, const uint16_t *q, const uint16_t *k_cache, cons
  * and fewer than 2^31 table entries and pages; everything
  * stays on the device, so a decode loop can be captured (the attention below, as
  * other calls, uses the context's workspace: graphs captured from one context are
- * replayed one after another). No tensor may overlap another but as said. */
+ * replayed one after another). No tensor may overlap another but as said.
+ * Time follows the tokens, except where few tokens come with many pages given
+ * back or taken: about a microsecond a thousand pages then. */
 int mg_kv_pages(mg_ctx *ctx, int32_t *page_table, int64_t ldt, int64_t requests, int64_t max_pages,
                 const int32_t *old_lens, const int32_t *new_lens, int64_t page_size, int32_t *free_ring,
                 int64_t num_pages, const int64_t *ends, int32_t *lens, int64_t *ends_out, int32_t *starts,

@@ -46,12 +46,12 @@
 // V block's its weights before they are split, so no value is rounded to 16 bits.
 //
 // What bounds it: HBM where requests are long. 8 requests of 131072 keys (40/8
-// heads of 128, bf16): 646 us, 6.65 TB/s of the 7.04 that a plain read reaches; 64
-// ragged ones of up to 8000: 157, 6.1; 250 of up to 700: 68, 5.1 (waves wait 62 % of
+// heads of 128, bf16): 657 us, 6.5 TB/s of the 7.04 that a plain read reaches; 64
+// ragged ones of up to 8000: 156, 6.2; 250 of up to 700: 67, 5.1 (waves wait 61 % of
 // their cycles: a request's last step and the waves' meeting leave little in flight).
 // About 6 us of each is launch, sums and the first step's chain of table entry, rows
 // and products; the join adds 4 to 6. Q8_0: 5 of 100003 keys (32/2 heads) 56 us, 4.8
-// TB/s; 580 vector instructions a step and wave keep the SIMDs 58 % busy and three
+// TB/s; 550 vector instructions a step and wave keep the SIMDs 57 % busy and three
 // waves each do not cover the rest of the step's chain.
 #include "mg_device.hpp"
 #include "mg_internal.hpp"
@@ -229,6 +229,8 @@ namespace mg
         return r;
     }
 
+    // (Q8_0 with 168 registers for three waves a SIMD: f16 queries with f32 outputs over head_dim 128 keep 12 bytes a
+    // lane in scratch, and take 62.8 us where bf16's, without, take 62.3)
     template <class S, class SO, bool Q8, int KB> // KB = head_dim / 32
     __global__ __launch_bounds__(256, Q8 ? 3 : 2) void k_attn_paged(PagedArgs a)
     {

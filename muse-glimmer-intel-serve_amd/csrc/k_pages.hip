@@ -27,10 +27,14 @@
 // requests, 94 000 tokens 13.3 -> 7.3 us a call, 200 requests, 520 000 tokens 11.2 -> 7.3),
 // and the first also writes the new lengths and counters. Where those replace their
 // old values, which the others still read, they are left to a second launch of one
-// work-group, from 4096 tokens on (10.1 us, what one work-group takes at 4300).
+// work-group, from 4096 tokens on (10.4 us, what one work-group takes at 4000).
 //
-// Latency bounds it: 4.4 us of kernel for a decode step of 48 requests, 6.7 and 7.2 for the two
-// above: a launch, the sums, then chains of a bisection and two or three dependent loads.
+// Latency bounds it: traced 4.8 us (median) for a decode step of 48 requests, in place or not, 7.7
+// and 8.2 for the two above, of which a stream of calls hides 0.5 to 1: a launch, the sums, then
+// chains of a bisection and two or three dependent loads. The work-groups follow the tokens alone:
+// pages are taken and given back by as many, so one of them takes a step of few tokens that ends
+// long requests, at 0.5 (few requests to bisect) to 1.1 us a thousand pages: 8 requests of 131072
+// tokens in pages of 16 38 us, 256 of 4096 61, 256 of 131072 2.3 ms.
 #include "mg_device.hpp"
 #include "mg_internal.hpp"
 
