@@ -316,7 +316,7 @@ int mg_qk_norm_rope_paged(mg_ctx *ctx, void *q, int64_t q_heads, int64_t ldq, vo
  * may make its sum so. head_dim 64 or 128; any number of
  * query heads per kv head; at most 65535 requests, 2^31 - 1 slots in the pool and
  * tables (or windows of them) of fewer than 2^38 keys. A numerical envelope, not
- * bits: f32 sums and weights to 2^-16 relative (those down to 2^-100 of the
+ * bits: f32 sums and weights to 2^-16 relative (those down to 2^-90 of the
  * largest), keys split over work-groups and joined, the split depending on the
  * batch's lengths. */
 int mg_attn_decode_paged(mg_ctx *ctx, const void *q, int64_t ldq, const void *k_cache, const void *v_cache,

@@ -8,7 +8,8 @@
 //   s_j = (q_bh . k_j) * scaling,   out_bh = sum_j softmax(s)_j v_j.
 // A request without keys gives zeros. A key whose page is outside the pool is
 // left out, as a masked one. A score of -inf weighs nothing beside a larger one;
-// a request that has only such scores gives NaN, as the quotient 0 / 0 is. Q8_0 pages hold k_j and v_j as q * d, exactly.
+// a request that has only such scores gives NaN, as the quotient 0 / 0 is. Q8_0
+// pages hold k_j and v_j as q * d, exactly.
 //
 // Division of the work (mg_paged_plan.hpp): the requests' keys form one line of
 // units, cut into equal runs; a team of work-groups, one for every KV head (and
@@ -27,7 +28,8 @@
 // S^T = K Q^T and O += P V run on the matrix cores (16 query heads of the
 // group, zero-padded, as columns), the weights entering as a high and a low
 // 16-bit part (three of bf16 for f32 outputs), so each is within 2^-16 of p relative
-// down to 2^-100 of the largest. Online softmax in f32 on scores scaled by log2(e).
+// down to 2^-90 of the largest (a Q8_0 scale may take 2^-24 of bf16's range, a low
+// part 2^-17). Online softmax in f32 on scores scaled by log2(e).
 //   Pages: lane l holds the slot of key l of the step (its table entry was
 // requested a step before); a load instruction covers 4 to 16 rows, which lie
 // in one page where the page is that large, so one readlane gives their base;
