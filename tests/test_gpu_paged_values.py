@@ -256,3 +256,54 @@ def test_nothing_before_a_window_is_used(prims, dt, q8, D, ps, window, freed):
         K, V = (x[table[r, j // ps], j % ps] for x in plain)  # [keys, 1, D]
         ref, bound = PO.attn_decode(qf[r:r + 1], K[:, None], V[:, None], np.arange(len(j))[None], [len(j)], 1, 0, 0.1)
         assert np.all(np.abs(got[r] - ref[0]) <= bound[0]), r
+
+
+@pytest.mark.parametrize("q8", (False, True))
+@pytest.mark.parametrize("T", (1, 5, 70))
+def test_append_without_query_heads(prims, q8, T):
+    """k and v alone: as with q heads beside them"""
+    import torch
+    g = torch.Generator(device=DEV).manual_seed(T)
+    k, v = (torch.randn((T, 3, 128), generator=g, device=DEV).bfloat16() for _ in range(2))
+    slots = torch.randperm(80, generator=g, device=DEV)[:T]
+    res = []
+    for heads in (0, 2):
+        q, kk = torch.ones((T, heads, 128), dtype=torch.bfloat16, device=DEV), k.clone()
+        kc, vc = (torch.zeros((10, 8, 3, 128), dtype=torch.int8 if q8 else torch.bfloat16, device=DEV) for _ in range(2))
+        kd, vd = (torch.zeros((10, 8, 3, 4), dtype=torch.float16, device=DEV) if q8 else None for _ in range(2))
+        prims.qk_norm_rope_paged(q, kk, v, 1e-6, 1.0, None, None, slots, slots, kc, vc, kd, vd)
+        res.append([t for t in (kk, kc, vc, kd, vd) if t is not None])
+    assert all(torch.equal(a, b) for a, b in zip(*res)) and res[0][1].any()
+
+
+@pytest.mark.parametrize("dt,q8", FORMS)
+@pytest.mark.parametrize("nq,nkv,ps,window,scaling", ((17, 1, 16, 0, 0.088), (46, 2, 16, 2**40, -0.088), (4, 2, 1 << 20, 70, 0.0)))
+def test_decode_corners(prims, dt, q8, nq, nkv, ps, window, scaling):
+    """groups of 17 and 23 query heads, scalings of zero and below, windows past 32 bits, the largest pages"""
+    rng = np.random.default_rng(nq)
+    lens, D = [0, 130, 33, 1], 64
+    N, W = (4, 1) if ps > 1000 else (40, 9)
+    if ps > 1000:  # (the first 160 keys of each page are filled, and are all that the oracle sees)
+        import torch
+        shape = (N, ps, nkv, D)
+        c = [torch.zeros(shape, dtype=torch.int8 if q8 else torch.bfloat16 if dt == BF16 else torch.float16, device=DEV)
+             for _ in range(2)]
+        d = [torch.zeros((*shape[:3], D // 32), dtype=torch.float16, device=DEV) if q8 else None for _ in range(2)]
+        plain = []
+        for cc, dd in zip(c, d):
+            x, s, vals = random_values(rng, (N, 160, nkv, D), dt, q8)
+            cc[:, :160] = x
+            if q8:
+                dd[:, :160] = s
+            plain.append(vals)
+        (kc, vc), (kd, vd), (K, V) = c, d, plain
+    else:
+        (kc, kd, K), (vc, vd, V) = (random_values(rng, (N, ps, nkv, D), dt, q8) for _ in range(2))
+    table = np.stack([rng.permutation(N)[:W] for _ in lens])
+    q = rng.standard_normal((len(lens), nq, D))
+    dq = to_dev(O.from_f64(q, dt), dt)
+    got = prims.attn_decode_paged(dq, kc, vc, i32(table), i32(lens), scaling, window, kd, vd).double().cpu().numpy()
+    # (the oracle's bound takes a scaling's magnitude: the sign goes into q)
+    qf = dq.double().cpu().numpy() * (-1.0 if scaling < 0 else 1.0)
+    ref, bound = PO.attn_decode(qf, K, V, table, lens, min(ps, 160), window, abs(scaling))
+    assert np.all(np.abs(got - ref) <= bound)
