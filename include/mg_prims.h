@@ -342,6 +342,44 @@ int mg_quantize_q8_0(mg_ctx *ctx, const uint16_t *w, int64_t rows, int64_t in, i
 int mg_gemv_q8_0(mg_ctx *ctx, const int8_t *qs, const uint16_t *d, const uint16_t *x, int64_t batch, int64_t rows,
                  int64_t in, int64_t ldx, float *y, int64_t ldy, int blockdot);
 
+/* ---- MXFP4: rows in 4.25 bits an element. NO COUNTERPART in the reference,
+ * whose smallest format is Q8_0. The OCP microscaling format: 32 consecutive
+ * elements of a row share the power of two 2^(s - 127) of one byte s (e8m0; 255
+ * is NaN: the whole block is), each is an e2m1 code: 0 .5 1 1.5 2 3 4 6 by its
+ * low three bits, the sign in bit 3. qs uint8 [rows, in / 2], element 2 i of a row
+ * in the low four bits of byte i; scales uint8 [rows, in / 32]; `in` a multiple of
+ * 32. A value past the type it is read at is infinite, one below it rounds.
+ *
+ * Quantizer: x [rows, in] at dtype (MG_BF16, MG_F16 or MG_F32; row stride ldx, 0 =
+ * in) -> s = floor(log2 amax) - 2 + 127 within [0, 254] (amax 0: 0), codes the
+ * nearest of x / 2^(s - 127), ties to the even code, past 6: 6 (an amax of 6 to 8
+ * scales loses up to a quarter, the format's own rule). A block that holds an
+ * infinity or a NaN: s = 255. x 16-byte, qs 4-byte aligned, ldx of whole 16 bytes. */
+int mg_quantize_mxfp4(mg_ctx *ctx, const void *x, int64_t ldx, int64_t rows, int64_t in, int dtype, uint8_t *qs,
+                      uint8_t *scales);
+
+/* out [rows, in] = rnd(code * 2^(s - 127)) at dtype_out (MG_BF16, MG_F16 or MG_F32),
+ * one rounding; a block of scale 255 gives NaN. out 16-byte, qs 4-byte aligned. */
+int mg_dequant_mxfp4(mg_ctx *ctx, const uint8_t *qs, const uint8_t *scales, void *out, int64_t rows, int64_t in,
+                     int dtype_out);
+
+/* y[b, o] = sum_i W[o, i] * x[b, i] for b < batch (1..64), W [rows, in] in MXFP4
+ * (qs, scales), x [batch, in] at dtype MG_BF16 or MG_F16 (row stride ldx, 0 = in),
+ * y at dtype_out, MG_F32 or dtype (row stride ldy, 0 = rows). Every product is of
+ * the exact values; f32 sums, in an order that depends on batch and sizes: a row's
+ * bits may differ between batches. qs and x 16-byte aligned, ldx % 8 == 0. (Longer
+ * batches: quantize the activations and call mg_gemm_mxfp4, or dequantize the
+ * weight for a 16-bit product.) */
+int mg_gemv_mxfp4(mg_ctx *ctx, const uint8_t *qs, const uint8_t *scales, const void *x, int64_t batch, int64_t rows,
+                  int64_t in, int64_t ldx, void *y, int64_t ldy, int dtype, int dtype_out);
+
+/* y[t, o] = sum_i W[o, i] * A[t, i], both MXFP4: activations A [tokens, in] (a_qs,
+ * a_scales), weight W [rows, in] (qs, scales) -> y [tokens, rows] at dtype_out
+ * (MG_F32, MG_BF16 or MG_F16; row stride ldy, 0 = rows). Exact products, f32 sums in
+ * an order that depends on the sizes, one rounding. a_qs and qs 16-byte aligned. */
+int mg_gemm_mxfp4(mg_ctx *ctx, const uint8_t *a_qs, const uint8_t *a_scales, int64_t tokens, const uint8_t *qs,
+                  const uint8_t *scales, int64_t rows, int64_t in, void *y, int64_t ldy, int dtype_out);
+
 /* HBM stream probe: NO COUNTERPART in the reference; a measurement aid that
  * moves `bytes` (a multiple of 16) through the primitives' access pattern
  * (16-byte non-temporal loads and stores, one-shot grid) with no arithmetic:

@@ -394,6 +394,42 @@ int mg_gemv_q8_0(mg_ctx *ctx, const int8_t *qs, const uint16_t *d, const uint16_
     });
 }
 
+int mg_quantize_mxfp4(mg_ctx *ctx, const void *x, int64_t ldx, int64_t rows, int64_t in, int dtype, uint8_t *qs,
+                      uint8_t *scales)
+{
+    MG_GUARD(-1, {
+        mg::launch_quantize_mxfp4(ctx_of(ctx), x, ldx, rows, in, dtype, qs, scales);
+        return 0;
+    });
+}
+
+int mg_dequant_mxfp4(mg_ctx *ctx, const uint8_t *qs, const uint8_t *scales, void *out, int64_t rows, int64_t in,
+                     int dtype_out)
+{
+    MG_GUARD(-1, {
+        mg::launch_dequant_mxfp4(ctx_of(ctx), qs, scales, out, rows, in, dtype_out);
+        return 0;
+    });
+}
+
+int mg_gemv_mxfp4(mg_ctx *ctx, const uint8_t *qs, const uint8_t *scales, const void *x, int64_t batch, int64_t rows,
+                  int64_t in, int64_t ldx, void *y, int64_t ldy, int dtype, int dtype_out)
+{
+    MG_GUARD(-1, {
+        mg::launch_gemv_mxfp4(ctx_of(ctx), qs, scales, x, ldx, batch, rows, in, y, ldy, dtype, dtype_out);
+        return 0;
+    });
+}
+
+int mg_gemm_mxfp4(mg_ctx *ctx, const uint8_t *a_qs, const uint8_t *a_scales, int64_t tokens, const uint8_t *qs,
+                  const uint8_t *scales, int64_t rows, int64_t in, void *y, int64_t ldy, int dtype_out)
+{
+    MG_GUARD(-1, {
+        mg::launch_gemm_mxfp4(ctx_of(ctx), a_qs, a_scales, tokens, qs, scales, rows, in, y, ldy, dtype_out);
+        return 0;
+    });
+}
+
 int mg_attn_prefill(mg_ctx *ctx, const uint16_t *q, int64_t ldq, const uint16_t *k_cache, const uint16_t *v_cache,
                     int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim, int64_t cache_slots,
                     int64_t pos0, int64_t window, double scaling, float *out, int64_t ldo)

@@ -130,6 +130,15 @@ namespace mg
                                   int64_t max_pages, const int32_t *lens, int64_t seqs, int64_t nq, int64_t nkv,
                                   int64_t D, int64_t page_size, int64_t num_pages, int64_t window, double scaling,
                                   void *out, int64_t ldo, int dt, int dt_out);
+    // k_mxfp4.hip
+    void launch_quantize_mxfp4(mg_ctx *c, const void *x, int64_t ldx, int64_t rows, int64_t in, int dt, uint8_t *qs,
+                               uint8_t *s);
+    void launch_dequant_mxfp4(mg_ctx *c, const uint8_t *qs, const uint8_t *s, void *out, int64_t rows, int64_t in,
+                              int dt);
+    void launch_gemv_mxfp4(mg_ctx *c, const uint8_t *qs, const uint8_t *s, const void *x, int64_t ldx, int64_t batch,
+                           int64_t rows, int64_t in, void *y, int64_t ldy, int dt, int dt_out);
+    void launch_gemm_mxfp4(mg_ctx *c, const uint8_t *aq, const uint8_t *as, int64_t tokens, const uint8_t *qs,
+                           const uint8_t *s, int64_t rows, int64_t in, void *y, int64_t ldy, int dt_out);
     void launch_vocab(mg_ctx *c, const void *logits, int64_t ld, int64_t rows, int64_t V, int dt_in, int64_t K,
                       double *lse, int64_t *amax, int64_t *top_idx, float *top_val, bool tail_on, double mult,
                       double cap, void *logits_out);

@@ -1,0 +1,143 @@
+// MXFP4 on the device: gfx950's conversions of e2m1 codes with a power-of-two
+// scale, and products of codes on the matrix cores. A conversion's scale operand
+// is an f32 whose exponent field alone counts: the e8m0 byte shifted there. All
+// are exact or round once, to nearest even, for every scale (2^-127 and NaN, byte
+// 255, among them), with subnormals; a quantized value past 6 becomes 6.
+#pragma once
+
+#include "mg_device.hpp"
+
+namespace mg
+{
+    constexpr int kMxFp4 = 16; // among the storage formats' dt: codes with scales
+    struct SMxFp4
+    {
+        static constexpr int dt = kMxFp4;
+    };
+
+    typedef _Float16 mxf16x8 __attribute__((ext_vector_type(8)));
+    typedef __bf16 mxbf16x2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 mxf16x2 __attribute__((ext_vector_type(2)));
+
+    MG_DEV float mx_scale(uint32_t s) { return __builtin_bit_cast(float, s << 23); }
+
+    // the scale byte of a block whose largest magnitude has the f32 bits `amax`
+    MG_DEV uint32_t mx_scale_byte(uint32_t amax)
+    {
+        const uint32_t e = amax >> 23;
+        return e == 255u ? 255u : e > 2u ? e - 2u : 0u;
+    }
+    MG_DEV uint32_t mx_quad_max(uint32_t v)
+    {
+        v = max(v, dpp_mov<0xB1, 0xf>(v, v)); // quad_perm [1,0,3,2]
+        v = max(v, dpp_mov<0x4E, 0xf>(v, v)); // quad_perm [2,3,0,1]
+        return v;
+    }
+
+    // eight elements on their way to codes; amax() gives f32 bits (an infinity or a NaN: the largest)
+    template <class S>
+    struct Mx8
+    {
+        Vec<uint32_t, S::dt == F32 ? 8 : 4> v;
+        MG_DEV uint32_t amax() const
+        {
+            uint32_t m = 0;
+            if constexpr (S::dt == F32) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) m = max(m, v.v[i] & 0x7fffffffu);
+                return m;
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) m = pk_max_u16(m, v.v[i] & 0x7fff7fffu);
+                m = max(m & 0xffffu, m >> 16);
+                return S::dt == BF16 ? m << 16 : __builtin_bit_cast(uint32_t, f16_f32(uint16_t(m)));
+            }
+        }
+        MG_DEV uint32_t codes(uint32_t s) const
+        {
+            const float f = mx_scale(s);
+            uint32_t q = 0;
+            if constexpr (S::dt == F32) {
+                auto at = [&](int i) { return __builtin_bit_cast(float, v.v[i]); };
+                q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, at(0), at(1), f, 0);
+                q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, at(2), at(3), f, 1);
+                q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, at(4), at(5), f, 2);
+                q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(q, at(6), at(7), f, 3);
+            } else if constexpr (S::dt == BF16) {
+                auto at = [&](int i) { return __builtin_bit_cast(mxbf16x2, v.v[i]); };
+                q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, at(0), f, 0);
+                q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, at(1), f, 1);
+                q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, at(2), f, 2);
+                q = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(q, at(3), f, 3);
+            } else {
+                auto at = [&](int i) { return __builtin_bit_cast(mxf16x2, v.v[i]); };
+                q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, at(0), f, 0);
+                q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, at(1), f, 1);
+                q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, at(2), f, 2);
+                q = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(q, at(3), f, 3);
+            }
+            return q;
+        }
+    };
+    template <class S>
+    MG_DEV Mx8<S> mx_load8(const typename S::raw *p)
+    {
+        Mx8<S> x;
+        if constexpr (S::dt == F32) {
+            const Vec<uint32_t, 4> a = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(p));
+            const Vec<uint32_t, 4> b = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(p) + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x.v.v[i] = a.v[i], x.v.v[4 + i] = b.v[i];
+        } else {
+            x.v = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(p));
+        }
+        return x;
+    }
+
+    // eight codes as bf16 or f16 pairs, as f32 (a NaN scale gives the format's one NaN)
+    MG_DEV Vec<uint32_t, 4> mx_bf16(uint32_t q, float f)
+    {
+        return Vec<uint32_t, 4>{{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, f, 0)),
+                                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, f, 1)),
+                                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, f, 2)),
+                                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, f, 3))}};
+    }
+    MG_DEV Vec<uint32_t, 4> mx_f16(uint32_t q, float f)
+    {
+        return Vec<uint32_t, 4>{{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, f, 0)),
+                                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, f, 1)),
+                                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, f, 2)),
+                                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, f, 3))}};
+    }
+    template <class SO>
+    MG_DEV void mx_store8(typename SO::raw *out, uint32_t q, uint32_t s)
+    {
+        const float f = mx_scale(s);
+        if constexpr (SO::dt == F32) {
+            typedef float f32x2 __attribute__((ext_vector_type(2)));
+            f32x2 v[4];
+            v[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, f, 0);
+            v[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, f, 1);
+            v[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, f, 2);
+            v[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, f, 3);
+            st16_stream<float, 4>(out, Vec<float, 4>{{v[0][0], v[0][1], v[1][0], v[1][1]}});
+            st16_stream<float, 4>(out + 4, Vec<float, 4>{{v[2][0], v[2][1], v[3][0], v[3][1]}});
+        } else {
+            Vec<uint32_t, 4> w = SO::dt == BF16 ? mx_bf16(q, f) : mx_f16(q, f);
+            if (s == 255u) // the library's NaN (the conversion's has a sign)
+                w = SO::dt == BF16 ? Vec<uint32_t, 4>{{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u}}
+                                   : Vec<uint32_t, 4>{{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u}};
+            st16_stream<uint32_t, 4>(reinterpret_cast<uint32_t *>(out), w);
+        }
+    }
+
+    // f32 sums of 16 x 16 products over 128 codes each: lane l = 16 c + n holds block c (32 codes, 16 bytes) of
+    // row n of A (column n of B) and its scale byte; C as the other 16 x 16 products'
+    MG_DEV f32x4 mfma_mxfp4(Vec<uint32_t, 4> a, uint32_t sa, Vec<uint32_t, 4> b, uint32_t sb, f32x4 c)
+    {
+        typedef int i32x8 __attribute__((ext_vector_type(8)));
+        const i32x8 av = {int(a.v[0]), int(a.v[1]), int(a.v[2]), int(a.v[3]), 0, 0, 0, 0};
+        const i32x8 bv = {int(b.v[0]), int(b.v[1]), int(b.v[2]), int(b.v[3]), 0, 0, 0, 0};
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(av, bv, c, 4, 4, 0, int(sa), 0, int(sb));
+    }
+} // namespace mg

@@ -71,6 +71,10 @@ _SIGS = {
     "mg_sample_rows": ([_P, _P, _I, _I, _I, _P, _I, _D, _D, _D, _P, _P, _P], _INT),
     "mg_vocab_reduce_tail": ([_P, _P, _I, _I, _I, _INT, _D, _D, _I, _P, _P, _P, _P, _P], _INT),
     "mg_vocab_reduce_noalloc": ([_P, _P, _I, _I, _I, _INT, _I, _P, _P, _P, _P], _INT),
+    "mg_quantize_mxfp4": ([_P, _P, _I, _I, _I, _INT, _P, _P], _INT),
+    "mg_dequant_mxfp4": ([_P, _P, _P, _P, _I, _I, _INT], _INT),
+    "mg_gemv_mxfp4": ([_P, _P, _P, _P, _I, _I, _I, _I, _P, _I, _INT, _INT], _INT),
+    "mg_gemm_mxfp4": ([_P, _P, _P, _I, _P, _P, _I, _I, _P, _I, _INT], _INT),
     "mg_probe_stream": ([_P, _INT, _P, _P, _P, _P, _I], _INT),
     "mg_npy_info": ([ctypes.c_char_p, ctypes.c_char_p, _P, _INT, ctypes.POINTER(_INT)], _INT),
     "mg_npy_load": ([_P, ctypes.c_char_p, _P, _I, _INT], _INT),
@@ -136,6 +140,8 @@ def _ptr(t):
 class Prims:
     """A libmgprims context bound to one device and stream."""
 
+    _u8 = None  # torch.uint8, once torch is imported
+
     def __init__(self, device: int = 0, stream=None, workspace_bytes: int = 0):
         import torch
         self.lib = load_library()
@@ -147,6 +153,7 @@ class Prims:
         self.device = device
         # what the calls of a decode step look up
         self._i32, self._i64, self._i8, self._f16 = torch.int32, torch.int64, torch.int8, torch.float16
+        self._u8 = torch.uint8
         self._codes = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32}
 
     def _check(self, rc):
@@ -581,6 +588,72 @@ class Prims:
             raise MgError(f"gemv_q8_0: x must be [B, {n_in}] and y [B, {rows}]")
         self._check(self.lib.mg_gemv_q8_0(self.h, _ptr(qs), _ptr(d), _ptr(x), B, rows, n_in, ldx, _ptr(y), ldy,
                                           int(blockdot)))
+
+    # -------------------------------------------------------------- MXFP4
+    # rows in 4.25 bits an element: two e2m1 codes a byte (element 2 i in the low four bits of byte i), a power of
+    # two for every 32 of a row (e8m0)
+    def _mx(self, name, qs, s):
+        """(rows, in) of contiguous uint8 codes [rows, in / 2] and scales [rows, in / 32]"""
+        if qs.dtype != self._u8 or s.dtype != self._u8 or qs.dim() != 2 or s.dim() != 2:
+            raise MgError(f"{name}: codes and scales must be 2-d uint8, got {qs.dtype} {tuple(qs.shape)} and {s.dtype} "
+                          f"{tuple(s.shape)}")
+        rows, n = qs.shape[0], 2 * qs.shape[1]
+        if n % 32 != 0 or tuple(s.shape) != (rows, n // 32):
+            raise MgError(f"{name}: codes {tuple(qs.shape)} need rows of whole 32s and scales {(rows, n // 32)}, got "
+                          f"{tuple(s.shape)}")
+        if not (qs.is_contiguous() and s.is_contiguous()):
+            raise MgError(f"{name}: codes and scales must be contiguous")
+        return rows, n
+
+    def _mx_rows(self, name, t, shape):
+        """(row stride, dtype code) of a 16-bit or f32 [rows, n] tensor with unit inner stride, rows not overlapping"""
+        code = self._codes.get(t.dtype)
+        if code is None or t.shape != shape:
+            raise MgError(f"{name}: expected a 16-bit or f32 tensor of {tuple(shape)}, got {t.dtype} {tuple(t.shape)}")
+        ld, inner = t.stride()
+        if inner != 1 and shape[1] > 1 or shape[0] > 1 and ld < shape[1]:
+            raise MgError(f"{name}: rows must have unit inner stride and not overlap")
+        return (ld if shape[0] > 1 else shape[1]), code
+
+    def quantize_mxfp4(self, x, qs, s):
+        """x [rows, in] bf16, f16 or f32 -> codes qs uint8 [rows, in / 2] and scales s uint8 [rows, in / 32]
+        (mg_quantize_mxfp4: a power of two from each block's amax, codes to nearest even)."""
+        self._here(x, qs, s)
+        rows, n = self._mx("quantize_mxfp4", qs, s)
+        ld, code = self._mx_rows("quantize_mxfp4", x, (rows, n))
+        self._check(self.lib.mg_quantize_mxfp4(self.h, x.data_ptr(), ld, rows, n, code, qs.data_ptr(), s.data_ptr()))
+
+    def dequant_mxfp4(self, qs, s, out):
+        """What codes and scales stand for, out [rows, in] bf16, f16 or f32, contiguous (mg_dequant_mxfp4)."""
+        self._here(qs, s, out)
+        rows, n = self._mx("dequant_mxfp4", qs, s)
+        ld, code = self._mx_rows("dequant_mxfp4", out, (rows, n))
+        if ld != n:
+            raise MgError("dequant_mxfp4: out must be contiguous")
+        self._check(self.lib.mg_dequant_mxfp4(self.h, qs.data_ptr(), s.data_ptr(), out.data_ptr(), rows, n, code))
+
+    def gemv_mxfp4(self, qs, s, x, y):
+        """y[b, o] = sum_i W[o, i] x[b, i] over an MXFP4 weight [rows, in] (mg_gemv_mxfp4): x [B, in] bf16 or f16,
+        B in 1..64, y [B, rows] float32 or x's dtype."""
+        self._here(qs, s, x, y)
+        rows, n = self._mx("gemv_mxfp4", qs, s)
+        B = x.shape[0] if x.dim() == 2 else 0
+        ldx, code = self._mx_rows("gemv_mxfp4", x, (B, n))
+        ldy, ocode = self._mx_rows("gemv_mxfp4", y, (B, rows))
+        self._check(self.lib.mg_gemv_mxfp4(self.h, qs.data_ptr(), s.data_ptr(), x.data_ptr(), B, rows, n, ldx,
+                                           y.data_ptr(), ldy, code, ocode))
+
+    def gemm_mxfp4(self, a_qs, a_s, qs, s, y):
+        """y[t, o] = sum_i W[o, i] A[t, i], both MXFP4 (mg_gemm_mxfp4): activations [T, in], weight [rows, in] ->
+        y [T, rows] float32, bf16 or f16."""
+        self._here(a_qs, a_s, qs, s, y)
+        T, n = self._mx("gemm_mxfp4", a_qs, a_s)
+        rows, wn = self._mx("gemm_mxfp4", qs, s)
+        if wn != n:
+            raise MgError(f"gemm_mxfp4: activations of {n} and weight rows of {wn} elements differ")
+        ldy, code = self._mx_rows("gemm_mxfp4", y, (T, rows))
+        self._check(self.lib.mg_gemm_mxfp4(self.h, a_qs.data_ptr(), a_s.data_ptr(), T, qs.data_ptr(), s.data_ptr(), rows,
+                                           n, y.data_ptr(), ldy, code))
 
     # -------------------------------------------------------------- vocab
     def _vocab_outs(self, name, rows, K, lse, argmax, top_idx, top_val):
