@@ -380,6 +380,27 @@ int mg_gemv_mxfp4(mg_ctx *ctx, const uint8_t *qs, const uint8_t *scales, const v
 int mg_gemm_mxfp4(mg_ctx *ctx, const uint8_t *a_qs, const uint8_t *a_scales, int64_t tokens, const uint8_t *qs,
                   const uint8_t *scales, int64_t rows, int64_t in, void *y, int64_t ldy, int dtype_out);
 
+/* mg_qk_norm_rope_paged into MXFP4 pages: k_cache and v_cache uint8 [num_pages,
+ * page_size, kv_heads, head_dim / 2] codes, k_scale and v_scale uint8 [.., head_dim
+ * / 32], by mg_quantize_mxfp4's rule (the k row as stored at dtype). q and k bit for
+ * bit as there; head_dim 64, 128 or 256, all rows and the caches 16-byte aligned. */
+int mg_qk_norm_rope_paged_mxfp4(mg_ctx *ctx, void *q, int64_t q_heads, int64_t ldq, void *k, int64_t k_heads,
+                                int64_t ldk, const void *v, int64_t ldv, int64_t tokens, int64_t head_dim, double eps,
+                                double qk_scale, const void *cos_t, const void *sin_t, int64_t table_rows,
+                                const int64_t *positions, const int64_t *slot_map, uint8_t *k_cache, uint8_t *v_cache,
+                                uint8_t *k_scale, uint8_t *v_scale, int64_t cache_slots, int dtype);
+
+/* mg_attn_decode_paged over MXFP4 pages, each k and v exactly code * 2^(s - 127);
+ * all else as there, the scales 8-byte aligned. An attended block of scale 255 makes
+ * the outputs it enters NaN (a key's: all of its request's for its query heads; a
+ * value's: those of the block's 32 dims). Weights count with their V block's scale:
+ * a product of the two keeps 2^-16 of itself down to 2^-118 and is lost below 2^-126. */
+int mg_attn_decode_paged_mxfp4(mg_ctx *ctx, const void *q, int64_t ldq, const uint8_t *k_cache, const uint8_t *v_cache,
+                               const uint8_t *k_scale, const uint8_t *v_scale, const int32_t *page_table, int64_t ldt,
+                               int64_t max_pages, const int32_t *lens, int64_t requests, int64_t q_heads,
+                               int64_t kv_heads, int64_t head_dim, int64_t page_size, int64_t num_pages, int64_t window,
+                               double scaling, void *out, int64_t ldo, int dtype, int dtype_out);
+
 /* HBM stream probe: NO COUNTERPART in the reference; a measurement aid that
  * moves `bytes` (a multiple of 16) through the primitives' access pattern
  * (16-byte non-temporal loads and stores, one-shot grid) with no arithmetic:

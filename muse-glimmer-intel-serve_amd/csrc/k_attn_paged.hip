@@ -55,28 +55,10 @@
 // and products; the join adds 4 to 6. Q8_0: 5 of 100003 keys (32/2 heads) 56 us, 4.8
 // TB/s; 550 vector instructions a step and wave keep the SIMDs 57 % busy and three
 // waves each do not cover the rest of the step's chain.
-#include "mg_device.hpp"
-#include "mg_internal.hpp"
-#include "mg_paged_plan.hpp"
+#include "mg_attn_paged.hpp"
 
 namespace mg
 {
-    struct PagedArgs
-    {
-        const void *q, *kc, *vc;
-        const uint16_t *kd, *vd;
-        const int32_t *table, *lens;
-        void *out;
-        float *part;     // [2 teams, vh, hw, D] outputs, then [2 teams, vh, hw] maxima and sums
-        PagedCut *cut;   // [requests] or, by_team, [teams]: what the second kernel joins
-        int by_team;
-        int64_t ldq, ldt, ldo, window;
-        int R, nkv, W, sh, num_pages;
-        int hpg, hw, vh; // query heads a kv head, a work-group; work-groups a team
-        int teams;
-        float scale2;    // scaling * log2(e)
-    };
-
     typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
     MG_DEV f32x4 mfma_f16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
@@ -165,70 +147,6 @@ namespace mg
         typedef int i32x2 __attribute__((ext_vector_type(2)));
         typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
         return __builtin_bit_cast(Vec<uint32_t, 2>, __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2 *)(p)));
-    }
-
-    // the factor of a part whose maximum is m beside the maximum `top` >= m of all (both may be -inf)
-    MG_DEV float weight_of(float m, float top) { return m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top); }
-    // what an output is multiplied by: 1 / sum; without a score above -inf 0 where there is no key, else NaN
-    MG_DEV float inverse(float sum, float top)
-    {
-        return top > -__builtin_huge_valf() ? 1.0f / sum : sum == 0.0f ? 0.0f : __builtin_nanf("");
-    }
-
-    // the work-group's run [u0, u1) of its team, the request it starts in and that request's first unit p
-    struct Run
-    {
-        PagedTeams d;
-        int u0, u1, p, b;
-    };
-    MG_DEV Run find_run(const PagedArgs &a, int team)
-    {
-        const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-        if (a.R <= 64) {
-            // each wave by itself, a request a lane
-            const int own = lane < a.R ? paged_span(a.lens[lane], a.W << a.sh, a.window).units : 0;
-            const int pre = wave_prefix_sum(own);
-            Run r;
-            r.d = paged_teams(__builtin_amdgcn_readlane(pre, 63), a.teams);
-            r.u0 = r.u1 = r.p = r.b = 0;
-            if (team >= r.d.teams) return r;
-            r.u0 = team_first(r.d, team);
-            r.u1 = team_first(r.d, team + 1);
-            r.b = wave_count(pre <= r.u0); // the requests that end before it
-            r.p = r.b > 0 ? __builtin_amdgcn_readlane(pre, r.b - 1) : 0;
-            return r;
-        }
-        __shared__ int red[4], found[2];
-        const int per = (a.R + 255) / 256, b0 = tid * per, b1 = min(b0 + per, a.R);
-        const int cap = a.W << a.sh;
-        int mine = 0;
-        for (int b = b0; b < b1; ++b) mine += paged_span(a.lens[b], cap, a.window).units;
-        int pre = wave_prefix_sum(mine);
-        if (lane == 63) red[wv] = pre;
-        __syncthreads();
-        for (int w = 0; w < wv; ++w) pre += red[w];
-        Run r;
-        // (uniform values read from LDS go to scalar registers)
-        r.d = paged_teams(__builtin_amdgcn_readfirstlane(red[0] + red[1] + red[2] + red[3]), a.teams);
-        int p = pre - mine; // the thread's first unit
-        r.u0 = r.u1 = 0;
-        if (team >= r.d.teams) return r;
-        r.u0 = team_first(r.d, team);
-        r.u1 = team_first(r.d, team + 1);
-        if (r.u0 >= p && r.u0 < pre) {
-            int b = b0;
-            for (;; ++b) {
-                const int u = paged_span(a.lens[b], cap, a.window).units;
-                if (r.u0 < p + u) break;
-                p += u;
-            }
-            found[0] = p;
-            found[1] = b;
-        }
-        __syncthreads();
-        r.p = __builtin_amdgcn_readfirstlane(found[0]);
-        r.b = __builtin_amdgcn_readfirstlane(found[1]);
-        return r;
     }
 
     // (Q8_0 with 168 registers for three waves a SIMD: f16 queries with f32 outputs over head_dim 128 keep 12 bytes a
@@ -704,11 +622,10 @@ namespace mg
         for (int i = 0; i < 4; ++i) dst[i] = SO::enc32(acc.v[i] * inv);
     }
 
-    void launch_attn_decode_paged(mg_ctx *c, const void *q, int64_t ldq, const void *kc, const void *vc,
-                                  const uint16_t *kd, const uint16_t *vd, const int32_t *table, int64_t ldt,
-                                  int64_t max_pages, const int32_t *lens, int64_t seqs, int64_t nq, int64_t nkv,
-                                  int64_t D, int64_t page_size, int64_t num_pages, int64_t window, double scaling,
-                                  void *out, int64_t ldo, int dt, int dt_out)
+    PagedArgs paged_args(const void *q, int64_t ldq, const void *kc, const void *vc, const void *kd, const void *vd,
+                         const int32_t *table, int64_t ldt, int64_t max_pages, const int32_t *lens, int64_t seqs, int64_t nq,
+                         int64_t nkv, int64_t D, int64_t page_size, int64_t num_pages, int64_t window, double scaling,
+                         void *out, int64_t ldo, int dt, int dt_out)
     {
         const int sh = page_shift(page_size, "attn_decode_paged");
         need(seqs >= 0 && nq > 0 && nkv > 0 && nq % nkv == 0,
@@ -730,39 +647,80 @@ namespace mg
         need(reinterpret_cast<uintptr_t>(kd) % 8 == 0 && reinterpret_cast<uintptr_t>(vd) % 8 == 0,
              "attn_decode_paged: scales must be 8-byte aligned");
         need(seqs <= 65535, "attn_decode_paged: at most 65535 requests");
-        if (seqs == 0) return;
+        PagedArgs a{};
+        if (seqs == 0) return a;
         need(q && kc && vc && table && lens && out, "attn_decode_paged: NULL tensor");
         // a wave serves up to 16 query heads (the matrix cores' 16 columns); larger
         // groups split over work-groups of the largest divisor <= 16
         const int64_t hpg = nq / nkv;
         int64_t hw = hpg;
         while (hw > 16 || hpg % hw != 0) --hw;
-        const int64_t vh = nkv * (hpg / hw);
-        // Teams for 2 to 4 work-groups a CU: as many as its registers take, but three, not four, for 16-bit rows of
-        // 64 (10 requests of 100003 keys 351 us, four 372, two 358; Q8_0: four 69, three 72, two 81 at 64 ragged
-        // requests of up to 8000). Not more than there can be units, nor than the workspace has room for.
-        const int per_cu = kd ? (D == 128 ? 3 : 4) : (D == 128 ? 2 : 3);
-        const int64_t span = window > 0 && window < max_pages << sh ? window + kPagedStep : max_pages << sh;
-        const int64_t most = seqs * (span / kPagedUnit + 1);
-        need(most < (int64_t(1) << 31), "attn_decode_paged: the table must stand for fewer than 2^38 keys");
-        int64_t teams = per_cu * int64_t(c->num_cus) / vh;
-        teams = teams < most ? teams : most;
-        // (the cuts, then the partial results' outputs, then their maxima and sums)
-        const int64_t tbytes = 2 * vh * hw * (D + 2) * int64_t(sizeof(float)) + int64_t(sizeof(PagedCut));
-        teams = teams < c->work_bytes / tbytes ? teams : c->work_bytes / tbytes;
-        teams = teams > 1 ? teams : 1;
-        const bool by_team = cuts_by_team(teams, seqs); // else there is room for a cut of each request among the teams'
-        PagedArgs a{};
-        a.q = q, a.kc = kc, a.vc = vc, a.kd = kd, a.vd = vd, a.table = table, a.lens = lens, a.out = out;
-        a.cut = static_cast<PagedCut *>(c->work);
-        a.part = reinterpret_cast<float *>(a.cut + teams);
-        a.by_team = by_team;
+        a.q = q, a.kc = kc, a.vc = vc, a.table = table, a.lens = lens, a.out = out;
         a.ldq = ldq, a.ldt = ldt, a.ldo = ldo, a.window = window;
         a.R = int(seqs), a.nkv = int(nkv), a.W = int(max_pages), a.sh = sh, a.num_pages = int(num_pages);
-        a.hpg = int(hpg), a.hw = int(hw), a.vh = int(vh), a.teams = int(teams);
+        a.hpg = int(hpg), a.hw = int(hw), a.vh = int(nkv * (hpg / hw));
         a.scale2 = float(double(float(scaling)) * 1.4426950408889634);
+        return a;
+    }
+
+    void paged_divide(mg_ctx *c, PagedArgs &a, int64_t D, int per_cu, int step)
+    {
+        const int64_t tokens = int64_t(a.W) << a.sh, unit = 4 * step;
+        const int64_t span = a.window > 0 && a.window < tokens ? a.window + step : tokens;
+        const int64_t most = a.R * (span / unit + 1);
+        need(most < (int64_t(1) << 31), "attn_decode_paged: the table must stand for fewer than 2^38 keys");
+        // not more teams than there can be units, nor than the workspace has room for
+        int64_t teams = per_cu * int64_t(c->num_cus) / a.vh;
+        teams = teams < most ? teams : most;
+        // (the cuts, then the partial results' outputs, then their maxima and sums)
+        const int64_t tbytes = 2 * int64_t(a.vh) * a.hw * (D + 2) * int64_t(sizeof(float)) + int64_t(sizeof(PagedCut));
+        teams = teams < c->work_bytes / tbytes ? teams : c->work_bytes / tbytes;
+        teams = teams > 1 ? teams : 1;
+        a.by_team = cuts_by_team(teams, a.R); // else there is room for a cut of each request among the teams'
+        a.cut = static_cast<PagedCut *>(c->work);
+        a.part = reinterpret_cast<float *>(a.cut + teams);
+        a.teams = int(teams);
+    }
+
+    void paged_join(mg_ctx *c, const PagedArgs &a, int64_t D, int dt_out)
+    {
+        if (a.teams == 1) return; // nothing is cut
+        const int64_t who = cuts_kept(a.teams, a.R);
+        auto join = [&](auto kern, int e) {
+            const dim3 grid{unsigned(who), unsigned(a.vh), unsigned((a.hw * D + 4 * e - 1) / (4 * e))};
+            hipLaunchKernelGGL(kern, grid, dim3(256), 0, c->stream, a, int(D));
+            check_launch("k_attn_paged_join");
+        };
+        // few requests over many teams: threads over the teams; else over the outputs (one request of 131072 keys,
+        // 32/2 heads, 256 teams, 4 / 16: 31.3 us, 32.7; 8/1 heads, 512 teams: 21.7, 27.8; two of 60000, 32/2 heads, 128
+        // teams each: 31.4, 29.9)
+        const int64_t parts = a.teams / who;
+        auto to = [&](auto so) {
+            using SO = decltype(so);
+            if (parts >= 256)
+                join(k_attn_paged_join<SO, 4>, 4);
+            else
+                parts >= 8 ? join(k_attn_paged_join<SO, 16>, 16) : join(k_attn_paged_join<SO, 64>, 64);
+        };
+        dt_out == F32 ? to(SF32{}) : dt_out == BF16 ? to(SBf16{}) : to(SF16{});
+    }
+
+    void launch_attn_decode_paged(mg_ctx *c, const void *q, int64_t ldq, const void *kc, const void *vc,
+                                  const uint16_t *kd, const uint16_t *vd, const int32_t *table, int64_t ldt,
+                                  int64_t max_pages, const int32_t *lens, int64_t seqs, int64_t nq, int64_t nkv,
+                                  int64_t D, int64_t page_size, int64_t num_pages, int64_t window, double scaling,
+                                  void *out, int64_t ldo, int dt, int dt_out)
+    {
+        PagedArgs a = paged_args(q, ldq, kc, vc, kd, vd, table, ldt, max_pages, lens, seqs, nq, nkv, D, page_size,
+                                 num_pages, window, scaling, out, ldo, dt, dt_out);
+        if (a.R == 0) return;
+        a.kd = kd, a.vd = vd;
+        // Teams for 2 to 4 work-groups a CU: as many as its registers take, but three, not four, for 16-bit rows of
+        // 64 (10 requests of 100003 keys 351 us, four 372, two 358; Q8_0: four 69, three 72, two 81 at 64 ragged
+        // requests of up to 8000).
+        paged_divide(c, a, D, kd ? (D == 128 ? 3 : 4) : (D == 128 ? 2 : 3), kPagedStep);
         auto go = [&](auto kern) {
-            hipLaunchKernelGGL(kern, dim3(unsigned(teams * vh)), dim3(256), 0, c->stream, a);
+            hipLaunchKernelGGL(kern, dim3(unsigned(a.teams * a.vh)), dim3(256), 0, c->stream, a);
             check_launch("k_attn_paged");
         };
         auto sized = [&](auto s, auto so) {
@@ -772,25 +730,11 @@ namespace mg
                 D == 128 ? go(k_attn_paged<S, SO, true, 4>) : go(k_attn_paged<S, SO, true, 2>);
             else
                 D == 128 ? go(k_attn_paged<S, SO, false, 4>) : go(k_attn_paged<S, SO, false, 2>);
-            if (teams == 1) return; // nothing is cut
-            const int64_t who = cuts_kept(teams, seqs);
-            auto join = [&](auto kern, int e) {
-                const dim3 grid{unsigned(who), unsigned(vh), unsigned((hw * D + 4 * e - 1) / (4 * e))};
-                hipLaunchKernelGGL(kern, grid, dim3(256), 0, c->stream, a, int(D));
-                check_launch("k_attn_paged_join");
-            };
-            // few requests over many teams: threads over the teams; else over the outputs (one request of 131072 keys,
-            // 32/2 heads, 256 teams, 4 / 16: 31.3 us, 32.7; 8/1 heads, 512 teams: 21.7, 27.8; two of 60000, 32/2 heads, 128
-            // teams each: 31.4, 29.9)
-            const int64_t parts = teams / who;
-            if (parts >= 256)
-                join(k_attn_paged_join<SO, 4>, 4);
-            else
-                parts >= 8 ? join(k_attn_paged_join<SO, 16>, 16) : join(k_attn_paged_join<SO, 64>, 64);
         };
         if (dt_out == F32)
             dt == BF16 ? sized(SBf16{}, SF32{}) : sized(SF16{}, SF32{});
         else
             dt == BF16 ? sized(SBf16{}, SBf16{}) : sized(SF16{}, SF16{});
+        paged_join(c, a, D, dt_out);
     }
 } // namespace mg

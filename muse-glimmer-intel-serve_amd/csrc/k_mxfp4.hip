@@ -64,14 +64,6 @@ namespace mg
         uint32_t s;
     };
 
-    // f16 pairs of a word as sums of two bf16 pairs: 11 bits are 8 and 3 (an infinity or a NaN is its high part)
-    MG_DEV void mx_halves(uint32_t w, uint32_t &hi, uint32_t &lo)
-    {
-        const float a = f16_f32(uint16_t(w)), b = f16_f32(uint16_t(w >> 16));
-        hi = bf_pack(a, b);
-        lo = bf_pack(__builtin_isfinite(a) ? a - bf_lo(hi) : 0.0f, __builtin_isfinite(b) ? b - bf_hi(hi) : 0.0f);
-    }
-
     // One chunk's products. 16-bit activations: the codes become bf16, exactly. Beside
     // f16 activations they become f16 where that is exact too (scales of 2^-23 to
     // 2^13, blocks of zeros, NaN), else the activations are split into two bf16 parts.

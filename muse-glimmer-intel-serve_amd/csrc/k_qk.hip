@@ -8,8 +8,9 @@
 //   q        = rnd(q * qk_scale)      q only; qk_scale an f32 value outside f64
 //   q, k     = apply_rope(., table row pos)   when a table is given
 //   k_cache[pos % slots, g, :] = k,  v_cache[pos % slots, g, :] = v
-// or, for a paged cache, the same rows at slot slot_map[t], kept as they are or
-// as Q8_0 (32 elements to an f16 scale, the rule of k_quantize_q8_0).
+// or, for a paged cache, the same rows at slot slot_map[t], kept as they are, as
+// Q8_0 (32 elements to an f16 scale, the rule of k_quantize_q8_0) or as MXFP4 (32
+// to a power of two, the rule of k_quantize_mxfp4).
 // Each step materializes at storage exactly as the separate primitives do, so
 // the result is bit-identical to running mg_rmsnorm_rows, mg_scale, mg_rope and
 // the two cache copies one after the other.
@@ -27,6 +28,7 @@
 
 #include "mg_device.hpp"
 #include "mg_internal.hpp"
+#include "mg_mxfp4.hpp"
 
 namespace mg
 {
@@ -35,8 +37,8 @@ namespace mg
     constexpr int kQkPieces = 1;   // k_qk_pairs: 8-element pieces per lane in each half of a row
 
     // where a token's k and v go: the ring slot of its position, or slot_map's slot
-    // (one outside the cache: nowhere), as stored rows or as Q8_0
-    enum : int { kKvRing = 0, kKvSlots = 1, kKvSlotsQ8 = 2 };
+    // (one outside the cache: nowhere), as stored rows, as Q8_0 or as MXFP4
+    enum : int { kKvRing = 0, kKvSlots = 1, kKvSlotsQ8 = 2, kKvSlotsMx = 3 };
 
     struct QkArgs
     {
@@ -44,7 +46,7 @@ namespace mg
         int D;
         double eps;
         const int64_t *slot_map;
-        uint16_t *kd, *vd; // Q8_0 scales
+        void *kd, *vd; // scales: Q8_0's f16, MXFP4's bytes
     };
 
     // eight elements of a head row as Q8_0, the four lanes of a quad holding a block's 32:
@@ -67,6 +69,16 @@ namespace mg
         for (int e = 0; e < 8; ++e) q |= uint64_t(uint8_t(int8_t(int(__builtin_roundf(x[e] * id))))) << (8 * e);
         *reinterpret_cast<uint64_t *>(qs + at) = q;
         if (at % 32 == 0) d[at / 32] = __builtin_bit_cast(uint16_t, static_cast<_Float16>(dd));
+    }
+
+    // the same as MXFP4: eight codes a lane
+    template <class S>
+    MG_DEV void st_mx(const Vec<typename S::raw, 8> &v, uint8_t *qs, uint8_t *d, int64_t at)
+    {
+        const Mx8<S> x{__builtin_bit_cast(Vec<uint32_t, 4>, v)};
+        const uint32_t s = mx_scale_byte(mx_quad_max(x.amax()));
+        *reinterpret_cast<uint32_t *>(qs + at / 2) = x.codes(s);
+        if (at % 32 == 0) d[at / 32] = uint8_t(s);
     }
 
     template <class S, int VEC, bool C, int KV>
@@ -298,10 +310,10 @@ namespace mg
         const int j = lane & (TPR - 1);
         const bool live = r < rows;
         const int64_t rc = live ? r : rows - 1; // addresses of a dead lane stay in bounds
-        // Rows go token by token, its q and its k heads; for Q8_0 q's first and then k's, so that a wave's rows are
+        // Rows go token by token, its q and its k heads; for Q8_0 and MXFP4 q's first and then k's, so that a wave's rows are
         // of one kind (but for one wave) and only k's pay for the quantizer: 2000 tokens of 32/2 heads 14.5 -> 12.1 us (f16 14.7 -> 13.1)
         const int64_t qrows = a.T * a.nq;
-        const bool by_kind = KV == kKvSlotsQ8, second = by_kind && rc >= qrows;
+        const bool by_kind = KV >= kKvSlotsQ8, second = by_kind && rc >= qrows;
         const int64_t rk = second ? rc - qrows : rc, per = !by_kind ? heads : second ? a.nkv : a.nq;
         const int64_t t = rows <= int64_t(0xffffffff) ? int64_t(uint32_t(rk) / uint32_t(per)) : rk / per;
         const int hr = int(rk - t * per);
@@ -501,10 +513,21 @@ namespace mg
             if constexpr (KV == kKvSlotsQ8) {
                 static_assert(NV == 1 && TPR >= 4, "a quad holds a block of 32");
                 int8_t *kq = reinterpret_cast<int8_t *>(kc), *vq = reinterpret_cast<int8_t *>(vc);
-                st_q8<S>(lo[0], kq, a.kd, o);
-                st_q8<S>(hi[0], kq, a.kd, o + half);
-                st_q8<S>(vlo[0], vq, a.vd, o);
-                st_q8<S>(vhi[0], vq, a.vd, o + half);
+                uint16_t *kd = static_cast<uint16_t *>(a.kd), *vd = static_cast<uint16_t *>(a.vd);
+                st_q8<S>(lo[0], kq, kd, o);
+                st_q8<S>(hi[0], kq, kd, o + half);
+                st_q8<S>(vlo[0], vq, vd, o);
+                st_q8<S>(vhi[0], vq, vd, o + half);
+                return;
+            }
+            if constexpr (KV == kKvSlotsMx) {
+                static_assert(NV == 1 && TPR >= 4, "a quad holds a block of 32");
+                uint8_t *kq = reinterpret_cast<uint8_t *>(kc), *vq = reinterpret_cast<uint8_t *>(vc);
+                uint8_t *kd = static_cast<uint8_t *>(a.kd), *vd = static_cast<uint8_t *>(a.vd);
+                st_mx<S>(lo[0], kq, kd, o);
+                st_mx<S>(hi[0], kq, kd, o + half);
+                st_mx<S>(vlo[0], vq, vd, o);
+                st_mx<S>(vhi[0], vq, vd, o + half);
                 return;
             }
 #pragma unroll
@@ -563,6 +586,8 @@ namespace mg
         }
         if constexpr (KV == kKvSlotsQ8) {
             fail("qk_norm_rope_paged: Q8_0 pages need head_dim 64, 128 or 256 and 16-byte aligned rows");
+        } else if constexpr (KV == kKvSlotsMx) {
+            fail("qk_norm_rope_paged: MXFP4 pages need head_dim 64, 128 or 256 and 16-byte aligned rows");
         } else {
             if (vec)
                 go(k_qk_norm_rope<S, V16, C, KV>);
@@ -606,7 +631,7 @@ namespace mg
     void launch_qk_norm_rope_paged(mg_ctx *c, void *q, int64_t nq, int64_t ldq, void *k, int64_t nkv, int64_t ldk,
                                    const void *v, int64_t ldv, int64_t T, int64_t D, double eps, double qk_scale,
                                    const void *co, const void *si, int64_t table_rows, const int64_t *pos,
-                                   const int64_t *slot_map, void *kc, void *vc, uint16_t *kd, uint16_t *vd,
+                                   const int64_t *slot_map, void *kc, void *vc, void *kd, void *vd, bool mx,
                                    int64_t slots, int dt)
     {
         need(D > 0 && D % 2 == 0 && D <= 512, "qk_norm_rope_paged: head_dim must be even and <= 512");
@@ -616,6 +641,7 @@ namespace mg
         need((co == nullptr) == (si == nullptr), "qk_norm_rope_paged: give both cos and sin, or neither");
         need(co == nullptr || table_rows > 0, "qk_norm_rope_paged: empty rope table");
         need((kd == nullptr) == (vd == nullptr), "qk_norm_rope_paged: give both k_scale and v_scale, or neither");
+        need(!mx || kd, "qk_norm_rope_paged: MXFP4 pages need their scales");
         need(slots > 0, "qk_norm_rope_paged: empty cache");
         need(dt == BF16 || dt == F16, "qk_norm_rope_paged: dtype must be bf16 or f16");
         if (ldq == 0) ldq = nq * D;
@@ -624,11 +650,14 @@ namespace mg
         need(ldq >= nq * D && ldk >= nkv * D && ldv >= nkv * D,
              "qk_norm_rope_paged: token stride smaller than heads*head_dim");
         const QkArgs a{nq, nkv, ldq, ldk, ldv, T, table_rows, 0, slots, int(D), eps, slot_map, kd, vd};
-        if (dt == BF16)
-            kd ? launch_qk_t<SBf16, false, kKvSlotsQ8>(c, q, k, v, a, qk_scale, co, si, pos, kc, vc)
-               : launch_qk_t<SBf16, false, kKvSlots>(c, q, k, v, a, qk_scale, co, si, pos, kc, vc);
-        else
-            kd ? launch_qk_t<SF16, false, kKvSlotsQ8>(c, q, k, v, a, qk_scale, co, si, pos, kc, vc)
-               : launch_qk_t<SF16, false, kKvSlots>(c, q, k, v, a, qk_scale, co, si, pos, kc, vc);
+        auto go = [&](auto st) {
+            using S = decltype(st);
+            if (mx)
+                launch_qk_t<S, false, kKvSlotsMx>(c, q, k, v, a, qk_scale, co, si, pos, kc, vc);
+            else
+                kd ? launch_qk_t<S, false, kKvSlotsQ8>(c, q, k, v, a, qk_scale, co, si, pos, kc, vc)
+                   : launch_qk_t<S, false, kKvSlots>(c, q, k, v, a, qk_scale, co, si, pos, kc, vc);
+        };
+        dt == BF16 ? go(SBf16{}) : go(SF16{});
     }
 } // namespace mg

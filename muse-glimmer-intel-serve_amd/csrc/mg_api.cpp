@@ -473,7 +473,35 @@ int mg_qk_norm_rope_paged(mg_ctx *ctx, void *q, int64_t q_heads, int64_t ldq, vo
     MG_GUARD(-1, {
         mg::launch_qk_norm_rope_paged(ctx_of(ctx), q, q_heads, ldq, k, k_heads, ldk, v, ldv, tokens, head_dim, eps,
                                       qk_scale, cos_t, sin_t, table_rows, positions, slot_map, k_cache, v_cache,
-                                      k_scale, v_scale, cache_slots, dtype);
+                                      k_scale, v_scale, false, cache_slots, dtype);
+        return 0;
+    });
+}
+
+int mg_qk_norm_rope_paged_mxfp4(mg_ctx *ctx, void *q, int64_t q_heads, int64_t ldq, void *k, int64_t k_heads,
+                                int64_t ldk, const void *v, int64_t ldv, int64_t tokens, int64_t head_dim, double eps,
+                                double qk_scale, const void *cos_t, const void *sin_t, int64_t table_rows,
+                                const int64_t *positions, const int64_t *slot_map, uint8_t *k_cache, uint8_t *v_cache,
+                                uint8_t *k_scale, uint8_t *v_scale, int64_t cache_slots, int dtype)
+{
+    MG_GUARD(-1, {
+        mg::launch_qk_norm_rope_paged(ctx_of(ctx), q, q_heads, ldq, k, k_heads, ldk, v, ldv, tokens, head_dim, eps,
+                                      qk_scale, cos_t, sin_t, table_rows, positions, slot_map, k_cache, v_cache,
+                                      k_scale, v_scale, true, cache_slots, dtype);
+        return 0;
+    });
+}
+
+int mg_attn_decode_paged_mxfp4(mg_ctx *ctx, const void *q, int64_t ldq, const uint8_t *k_cache, const uint8_t *v_cache,
+                               const uint8_t *k_scale, const uint8_t *v_scale, const int32_t *page_table, int64_t ldt,
+                               int64_t max_pages, const int32_t *lens, int64_t requests, int64_t q_heads,
+                               int64_t kv_heads, int64_t head_dim, int64_t page_size, int64_t num_pages, int64_t window,
+                               double scaling, void *out, int64_t ldo, int dtype, int dtype_out)
+{
+    MG_GUARD(-1, {
+        mg::launch_attn_decode_mxfp4(ctx_of(ctx), q, ldq, k_cache, v_cache, k_scale, v_scale, page_table, ldt, max_pages,
+                                     lens, requests, q_heads, kv_heads, head_dim, page_size, num_pages, window, scaling,
+                                     out, ldo, dtype, dtype_out);
         return 0;
     });
 }

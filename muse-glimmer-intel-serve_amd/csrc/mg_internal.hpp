@@ -123,7 +123,7 @@ namespace mg
     void launch_qk_norm_rope_paged(mg_ctx *c, void *q, int64_t nq, int64_t ldq, void *k, int64_t nkv, int64_t ldk,
                                    const void *v, int64_t ldv, int64_t T, int64_t D, double eps, double qk_scale,
                                    const void *co, const void *si, int64_t table_rows, const int64_t *pos,
-                                   const int64_t *slot_map, void *kc, void *vc, uint16_t *kd, uint16_t *vd,
+                                   const int64_t *slot_map, void *kc, void *vc, void *kd, void *vd, bool mx,
                                    int64_t slots, int dt);
     void launch_attn_decode_paged(mg_ctx *c, const void *q, int64_t ldq, const void *kc, const void *vc,
                                   const uint16_t *kd, const uint16_t *vd, const int32_t *table, int64_t ldt,
@@ -139,6 +139,12 @@ namespace mg
                            int64_t rows, int64_t in, void *y, int64_t ldy, int dt, int dt_out);
     void launch_gemm_mxfp4(mg_ctx *c, const uint8_t *aq, const uint8_t *as, int64_t tokens, const uint8_t *qs,
                            const uint8_t *s, int64_t rows, int64_t in, void *y, int64_t ldy, int dt_out);
+    // k_attn_mxfp4.hip
+    void launch_attn_decode_mxfp4(mg_ctx *c, const void *q, int64_t ldq, const uint8_t *kc, const uint8_t *vc,
+                                  const uint8_t *ks, const uint8_t *vs, const int32_t *table, int64_t ldt,
+                                  int64_t max_pages, const int32_t *lens, int64_t seqs, int64_t nq, int64_t nkv,
+                                  int64_t D, int64_t page_size, int64_t num_pages, int64_t window, double scaling,
+                                  void *out, int64_t ldo, int dt, int dt_out);
     void launch_vocab(mg_ctx *c, const void *logits, int64_t ld, int64_t rows, int64_t V, int dt_in, int64_t K,
                       double *lse, int64_t *amax, int64_t *top_idx, float *top_val, bool tail_on, double mult,
                       double cap, void *logits_out);

@@ -109,6 +109,14 @@ namespace mg
                                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, f, 2)),
                                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, f, 3))}};
     }
+    // f16 pairs of a word as sums of two bf16 pairs: 11 bits are 8 and 3 (an infinity or a NaN is its high part)
+    MG_DEV void mx_halves(uint32_t w, uint32_t &hi, uint32_t &lo)
+    {
+        const float a = f16_f32(uint16_t(w)), b = f16_f32(uint16_t(w >> 16));
+        hi = bf_pack(a, b);
+        lo = bf_pack(__builtin_isfinite(a) ? a - bf_lo(hi) : 0.0f, __builtin_isfinite(b) ? b - bf_hi(hi) : 0.0f);
+    }
+
     template <class SO>
     MG_DEV void mx_store8(typename SO::raw *out, uint32_t q, uint32_t s)
     {
@@ -129,6 +137,15 @@ namespace mg
                                    : Vec<uint32_t, 4>{{0x7e007e00u, 0x7e007e00u, 0x7e007e00u, 0x7e007e00u}};
             st16_stream<uint32_t, 4>(reinterpret_cast<uint32_t *>(out), w);
         }
+    }
+
+    // ds_read_b64_tr_b4: within each 16-lane group, lane i receives four-bit element i of the 8-byte pieces
+    // addressed by lanes 0 .. 15, lane j's in place j
+    MG_DEV Vec<uint32_t, 2> lds_read_tr4(const char *p)
+    {
+        typedef int i32x2 __attribute__((ext_vector_type(2)));
+        typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
+        return __builtin_bit_cast(Vec<uint32_t, 2>, __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2 *)(p)));
     }
 
     // f32 sums of 16 x 16 products over 128 codes each: lane l = 16 c + n holds block c (32 codes, 16 bytes) of

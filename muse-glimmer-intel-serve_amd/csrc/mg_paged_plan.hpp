@@ -1,8 +1,8 @@
 // How decode attention over a paged cache divides its keys among work-groups:
 // plain arithmetic, the same on the host (its host test) and on the device.
 //
-// A request's attended keys [lo, n) are cut into units of 128 keys from `base`,
-// lo rounded down to a step of 32 (a request without keys has one empty unit,
+// A request's attended keys [lo, n) are cut into units of 128 keys (256 of a
+// 4-bit cache) from `base`, lo rounded down to a step of 32 (64) (a request without keys has one empty unit,
 // so that somebody writes its zeros). The units of all requests form one line
 // of T; it is cut into `teams` equal runs, whatever requests they cross, and
 // each team has a work-group for every group of query heads. A request inside
@@ -29,14 +29,16 @@ namespace mg
         int lo, n, base, units;
     };
 
-    // `cap`: the tokens a table row can hold
+    // `cap`: the tokens a table row can hold; STEP: the keys a wave takes at once, a unit four of them
+    template <int STEP = kPagedStep>
     MG_HD PagedSpan paged_span(int len, int cap, int64_t window)
     {
+        constexpr int U = 4 * STEP;
         PagedSpan s;
         s.n = len < 0 ? 0 : len > cap ? cap : len;
         s.lo = window > 0 && s.n > window ? int(s.n - window) : 0;
-        s.base = s.lo / kPagedStep * kPagedStep;
-        const int u = (s.n - s.base) / kPagedUnit + ((s.n - s.base) % kPagedUnit != 0);
+        s.base = s.lo / STEP * STEP;
+        const int u = (s.n - s.base) / U + ((s.n - s.base) % U != 0);
         s.units = u > 0 ? u : 1;
         return s;
     }

@@ -67,6 +67,10 @@ _SIGS = {
                                _I, _INT], _INT),
     "mg_attn_decode_paged": ([_P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _D, _P, _I, _INT,
                               _INT], _INT),
+    "mg_qk_norm_rope_paged_mxfp4": ([_P, _P, _I, _I, _P, _I, _I, _P, _I, _I, _I, _D, _D, _P, _P, _I, _P, _P, _P, _P, _P,
+                                     _P, _I, _INT], _INT),
+    "mg_attn_decode_paged_mxfp4": ([_P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _P, _I, _I, _I, _I, _I, _I, _I, _D, _P, _I,
+                                    _INT, _INT], _INT),
     "mg_sample_dist": ([_P, _P, _P, _P, _P, _I, _I, _D, _D, _D, _P, _P, _P], _INT),
     "mg_sample_rows": ([_P, _P, _I, _I, _I, _P, _I, _D, _D, _D, _P, _P, _P], _INT),
     "mg_vocab_reduce_tail": ([_P, _P, _I, _I, _I, _INT, _D, _D, _I, _P, _P, _P, _P, _P], _INT),
@@ -440,9 +444,14 @@ class Prims:
         return shape, (ld if shape[0] > 1 else n), code
 
     def _pool(self, name, k_cache, v_cache, k_scale, v_scale, dtype, heads, dim):
-        """shape of a pool [num_pages, page_size, Hk, D] at dtype, or int8 with f16 scales [.., D / 32]
-        (heads None: any number)"""
+        """(num_pages, page_size, Hk, whether it is MXFP4) of a pool [num_pages, page_size, Hk, D] at dtype, int8 with
+        f16 scales [.., D / 32] or uint8 codes [.., D / 2] with uint8 scales [.., D / 32] (heads None: any number)"""
         shape = k_cache.shape
+        mx = k_cache.dtype == self._u8
+        if mx:
+            if dim % 32 != 0:
+                raise MgError(f"{name}: MXFP4 pages hold rows of whole 32s, got head_dim {dim}")
+            dim //= 2
         if len(shape) != 4 or shape[3] != dim or heads is not None and shape[2] != heads:
             raise MgError(f"{name}: caches must be [num_pages, page_size, {heads or 'heads'}, {dim}], got {tuple(shape)}")
         if v_cache.shape != shape:
@@ -451,15 +460,17 @@ class Prims:
             raise MgError(f"{name}: caches must be contiguous")
         if (k_scale is None) != (v_scale is None):
             raise MgError(f"{name}: give both k_scale and v_scale, or neither")
-        want = dtype if k_scale is None else self._i8
+        if mx and k_scale is None:
+            raise MgError(f"{name}: uint8 pools are MXFP4 codes and need k_scale and v_scale")
+        want = self._u8 if mx else dtype if k_scale is None else self._i8
         if k_cache.dtype != want or v_cache.dtype != want:
             raise MgError(f"{name}: caches of {k_cache.dtype} and {v_cache.dtype}, {want} needed")
         if k_scale is not None:
-            want = (*shape[:3], dim // 32)
+            want, kind = (*shape[:3], dim // (16 if mx else 32)), self._u8 if mx else self._f16
             for t in (k_scale, v_scale):
-                if t.dtype != self._f16 or t.shape != want or not t.is_contiguous():
-                    raise MgError(f"{name}: scales must be contiguous float16 {want}, got {t.dtype} {tuple(t.shape)}")
-        return shape
+                if t.dtype != kind or t.shape != want or not t.is_contiguous():
+                    raise MgError(f"{name}: scales must be contiguous {kind} {want}, got {t.dtype} {tuple(t.shape)}")
+        return shape[0], shape[1], shape[2], mx
 
     def kv_pages(self, page_table, old_lens, new_lens, page_size, free_ring, ends, lens, ends_out, starts=None,
                  slot_map=None, positions=None):
@@ -485,8 +496,8 @@ class Prims:
                            k_scale=None, v_scale=None):
         """qk_norm_rope with the append through a slot map (mg_qk_norm_rope_paged): k and v of token t go
         to slot slot_map[t] of the pool k_cache / v_cache [num_pages, page_size, Hk, D] (a slot outside it:
-        nowhere), at q's dtype or, with k_scale / v_scale [num_pages, page_size, Hk, D / 32] f16, as int8
-        Q8_0. positions [T] pick the rows of cos / sin (None: no rotation)."""
+        nowhere), at q's dtype or, with k_scale / v_scale [num_pages, page_size, Hk, D / 32], as Q8_0 (int8
+        pools, f16 scales) or MXFP4 (uint8 pools [.., D / 2], uint8 scales; mg_qk_norm_rope_paged_mxfp4). positions [T] pick the rows of cos / sin (None: no rotation)."""
         name, dtype = "qk_norm_rope_paged", q.dtype
         self._here(q, k, v, k_cache, v_cache, slot_map, positions, cos, sin, k_scale, v_scale)
         (T, qh, D), ldq, code = self._token_rows(name, q)
@@ -496,14 +507,14 @@ class Prims:
             raise MgError(f"{name}: k and v must be {dtype} [{T}, kv heads, {D}], got {k.dtype} {tuple(kshape)} and "
                           f"{v.dtype} {tuple(vshape)}")
         kh = kshape[1]
-        pages, page_size, _, _ = self._pool(name, k_cache, v_cache, k_scale, v_scale, dtype, kh, D)
+        pages, page_size, _, mx = self._pool(name, k_cache, v_cache, k_scale, v_scale, dtype, kh, D)
         rows = 0
         if cos is not None or sin is not None:
             if cos is None or sin is None or cos.dtype != dtype or sin.dtype != dtype or cos.shape != sin.shape or \
                     cos.dim() != 2 or cos.shape[1] != D // 2 or not (cos.is_contiguous() and sin.is_contiguous()):
                 raise MgError(f"{name}: cos and sin must be contiguous {dtype} [positions, {D // 2}], or both None")
             rows = cos.shape[0]
-        self._check(self.lib.mg_qk_norm_rope_paged(
+        self._check((self.lib.mg_qk_norm_rope_paged_mxfp4 if mx else self.lib.mg_qk_norm_rope_paged)(
             self.h, q.data_ptr(), qh, ldq, k.data_ptr(), kh, ldk, v.data_ptr(), ldv, T, D, eps, qk_scale,
             cos.data_ptr() if rows else None, sin.data_ptr() if rows else None, rows,
             self._ints(name, self._i64, T, positions), self._ints(name, self._i64, T, slot_map), k_cache.data_ptr(),
@@ -513,8 +524,9 @@ class Prims:
     def attn_decode_paged(self, q, k_cache, v_cache, page_table, lens, scaling, window=0, k_scale=None, v_scale=None,
                           out=None):
         """One new token's attention for each of R requests over a paged KV cache (mg_attn_decode_paged):
-        q [R, Hq, D] bf16 or f16; pool [num_pages, page_size, Hk, D] at q's dtype, or int8 Q8_0 with scales
-        [.., D / 32] f16; page_table [R, W] int32, lens [R] int32 keys of each (the new token's among them)
+        q [R, Hq, D] bf16 or f16; pool [num_pages, page_size, Hk, D] at q's dtype, int8 Q8_0 with scales
+        [.., D / 32] f16, or MXFP4, uint8 codes [.., D / 2] with uint8 scales [.., D / 32]
+        (mg_attn_decode_paged_mxfp4); page_table [R, W] int32, lens [R] int32 keys of each (the new token's among them)
         -> out [R, Hq, D], float32 (default) or q's dtype. A request without keys gives zeros."""
         name = "attn_decode_paged"
         if out is None:
@@ -526,9 +538,9 @@ class Prims:
         if oshape != shape:
             raise MgError(f"{name}: shape {tuple(shape)} and {tuple(oshape)} differ")
         R, hq, D = shape
-        pages, page_size, hk, _ = self._pool(name, k_cache, v_cache, k_scale, v_scale, q.dtype, None, D)
+        pages, page_size, hk, mx = self._pool(name, k_cache, v_cache, k_scale, v_scale, q.dtype, None, D)
         ldt, W = self._page_table(name, page_table, R)
-        self._check(self.lib.mg_attn_decode_paged(
+        self._check((self.lib.mg_attn_decode_paged_mxfp4 if mx else self.lib.mg_attn_decode_paged)(
             self.h, q.data_ptr(), ldq, k_cache.data_ptr(), v_cache.data_ptr(),
             None if k_scale is None else k_scale.data_ptr(), None if v_scale is None else v_scale.data_ptr(),
             page_table.data_ptr(), ldt, W, self._ints(name, self._i32, R, lens), R, hq, hk, D, page_size, pages, window,
