@@ -24,7 +24,7 @@ ARCH = "gfx950"
 
 SOURCES = ["mg_api.cpp", "mg_npy.cpp", "k_norm.hip", "k_elementwise.hip", "k_rope.hip", "k_qk.hip", "k_softmax.hip", "k_softmax64.hip",
            "k_q8.hip", "k_vocab.hip", "k_sample.hip", "k_attn.hip", "k_attn_prefill.hip", "k_pages.hip",
-           "k_attn_paged.hip", "k_mxfp4.hip", "k_attn_mxfp4.hip", "k_probe.hip"]
+           "k_attn_paged.hip", "k_mxfp4.hip", "k_mxfp4_gemv.hip", "k_mxfp4_gemm.hip", "k_attn_mxfp4.hip", "k_probe.hip"]
 
 FLAGS = [
     "-x", "hip", f"--offload-arch={ARCH}", "-O3", "-fPIC", "-std=c++17",

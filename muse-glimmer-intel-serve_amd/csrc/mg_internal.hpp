@@ -139,6 +139,10 @@ namespace mg
                            int64_t rows, int64_t in, void *y, int64_t ldy, int dt, int dt_out);
     void launch_gemm_mxfp4(mg_ctx *c, const uint8_t *aq, const uint8_t *as, int64_t tokens, const uint8_t *qs,
                            const uint8_t *s, int64_t rows, int64_t in, void *y, int64_t ldy, int dt_out);
+    // k_mxfp4_gemm.hip: large products; whether it took the call
+    bool launch_mxfp4_tiles(mg_ctx *c, const uint8_t *aq, const uint8_t *as, int64_t tokens, const uint8_t *qs,
+                            const uint8_t *s, int64_t rows, int64_t in, void *y, int64_t ldy, int dt_out);
+    void join_splits(mg_ctx *c, const float *part, int ns, void *y, int64_t ldy, int64_t rows, int64_t T, int dt_out);
     // k_attn_mxfp4.hip
     void launch_attn_decode_mxfp4(mg_ctx *c, const void *q, int64_t ldq, const uint8_t *kc, const uint8_t *vc,
                                   const uint8_t *ks, const uint8_t *vs, const int32_t *table, int64_t ldt,

@@ -5,6 +5,8 @@
 // 255, among them), with subnormals; a quantized value past 6 becomes 6.
 #pragma once
 
+#include <type_traits>
+
 #include "mg_device.hpp"
 
 namespace mg
@@ -147,6 +149,39 @@ namespace mg
         typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
         return __builtin_bit_cast(Vec<uint32_t, 2>, __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2 *)(p)));
     }
+
+    // f(0), f(1) .. of compile-time numbers
+    template <int I, int N, class F>
+    MG_DEV void each(F f)
+    {
+        if constexpr (I < N) {
+            f(std::integral_constant<int, I>{});
+            each<I + 1, N>(f);
+        }
+    }
+
+    // 64 lanes' 16 bytes (or one, as a word) from base + off, each lane its own, to LDS at `to` + 16 (or 4) * lane.
+    // (The compiler's own form would make every LDS read wait for all of them; here the kernel counts.)
+    template <int BYTES = 16>
+    MG_DEV void lds_load(const uint8_t *base, uint32_t off, uint32_t to)
+    {
+        // (uniform, but the compiler keeps some selections of them in vector registers)
+        const uint64_t b = reinterpret_cast<uint64_t>(base);
+        const uint64_t sb = uint64_t(uint32_t(__builtin_amdgcn_readfirstlane(int(b >> 32)))) << 32 |
+                            uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(b))));
+        to = uint32_t(__builtin_amdgcn_readfirstlane(int(to)));
+        if constexpr (BYTES == 16)
+            __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(sb) : "memory");
+        else
+            __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, %2" ::"s"(to), "v"(off), "s"(sb) : "memory");
+    }
+    // the same from any address of each lane
+    MG_DEV void lds_load_at(const uint8_t *p, uint32_t to)
+    {
+        to = uint32_t(__builtin_amdgcn_readfirstlane(int(to)));
+        __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(p) : "memory");
+    }
+    MG_DEV uint32_t lds_address(const char *p) { return uint32_t(uintptr_t((__attribute__((address_space(3))) const char *)p)); }
 
     // f32 sums of 16 x 16 products over 128 codes each: lane l = 16 c + n holds block c (32 codes, 16 bytes) of
     // row n of A (column n of B) and its scale byte; C as the other 16 x 16 products'
