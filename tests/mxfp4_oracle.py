@@ -34,7 +34,8 @@ def quantize(x):
 
 def product(w, x):
     """y = x w^T in 64 bits and its bound: every product is exact; a term passes one addition a matrix instruction
-    of its wave (in / 128 of them: a wave takes every fourth chunk of 128 or fewer, in four instructions or one) and
-    those of the waves' join, at most 24, each addition off by at most a step (2^-23) of the sum of magnitudes."""
+    of its accumulator's (of 64 elements or more each, or of 32 with two accumulators taking turns: in / 64 of them) and
+    those of accumulators', waves' and parts' joins, at most 24, each addition off by at most a step (2^-23) of the sum
+    of magnitudes."""
     y, mag = x @ w.T, np.abs(x) @ np.abs(w).T
-    return y, (w.shape[1] / 128 + 25) * 2.0**-23 * mag
+    return y, (w.shape[1] / 64 + 25) * 2.0**-23 * mag
