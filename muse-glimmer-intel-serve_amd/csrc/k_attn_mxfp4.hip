@@ -25,7 +25,11 @@
 
 namespace mg
 {
-    constexpr int kMxStep = 64; // keys a wave takes at once
+    template <class T>
+    MG_DEV T uniform_load(const T *p) // through scalar registers: p is the same in every lane
+    {
+        return *reinterpret_cast<const __attribute__((address_space(4))) T *>(reinterpret_cast<uintptr_t>(p));
+    }
 
     // each half less d's, not below 0
     MG_DEV uint32_t pk_subsat_u16(uint32_t a, uint32_t d)
@@ -39,57 +43,72 @@ namespace mg
         return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);
     }
 
-    template <class S, class SO, int KB> // KB = head_dim / 32
+    // KB = head_dim / 32; HP: kv heads a wave takes, two with up to eight query heads each
+    template <class S, class SO, int KB, int HP>
     __global__ __launch_bounds__(256, 2) void k_attn_mxfp4(PagedArgs a)
     {
         constexpr int D = 32 * KB, NT = 2 * KB; // NT output tiles of 16 dims
-        constexpr int U = 4 * kMxStep;
+        constexpr int KS = 64 / HP, U = 4 * KS; // keys of a step, of a unit
         constexpr int RB = D / 2;               // bytes of a row
         constexpr int LPR = RB / 16;            // lanes a row
         constexpr int RPI = 64 / LPR;           // rows a load instruction covers
-        constexpr int NLD = kMxStep / RPI;
-        constexpr int KW = D / 32;              // a lane's words of a key: 32 / 4 (or 16 / 4) dims of 8
-        // LDS rows: padded against bank conflicts, and every 16 of them by another 64 bytes (a K read takes rows
-        // 16 a + b)
-        constexpr int SR = RB + 16, SG = 16 * SR + 64;
-        constexpr int WB = 4 * SG;              // LDS bytes of a wave's K or V
-        constexpr int SO4 = D + 4;              // row stride of a wave's output in LDS (floats)
-        static_assert(16 * SO4 * 4 <= 2 * WB, "a wave's output takes the place of its K and V");
+        constexpr int NLD = 64 / RPI;
+        constexpr int OPS = 2 * NLD + 3;        // loads of a step: its rows, its scales, another's table entries
+        constexpr int KW = D / 32;              // a lane's words of a key: D / 4 dims
+        constexpr int WB = 64 * RB;             // LDS bytes of a step's K or V
+        constexpr int NV = 16 / HP;             // a lane's keys of its query head
         using raw = typename SO::raw;
         constexpr bool QF16 = S::dt == F16;
         constexpr int NP = SO::dt == F32 ? 3 : 2; // bf16 parts of a weight
         constexpr float kLow = -__builtin_huge_valf();
-        using KV = std::conditional_t<KB == 4, uint32_t, uint16_t>; // a key's scales
-        __shared__ __align__(16) char lds[4][2 * WB];
-        __shared__ __align__(16) uint16_t vsc[4][KB][kMxStep]; // (254 - s) << 7 of a key's V blocks, 0x8000 for NaN
+        static_assert(2 * WB >= 16 * 64 * 4, "64 dims of a wave's output take the place of a step");
+        __shared__ __align__(16) char lds[4][2][2 * WB];       // K and V of two steps
+        __shared__ uint32_t scales[4][2][2][64];               // of two steps, K's and V's, a row's a word
+        __shared__ int32_t entries[4][2][64];                  // of two steps
+        __shared__ __align__(16) uint16_t vsc[4][KB][64];      // exponents to take from weights, for a row's V blocks
         __shared__ float wm[4][16], wl[4][16];
+        __shared__ uint32_t place[4];                          // of a wave's output
         const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-        // runs of eight work-groups (a key's heads) on one XCD: two heads' rows share a 128-byte line, eight heads' scales one
+        // runs of eight work-groups on one XCD: a key's heads share lines of rows and scales
         constexpr int G = 8;
         int wg = blockIdx.x;
         if (wg < int(gridDim.x) / (8 * G) * (8 * G)) {
             const int xcd = wg % 8, turn = wg / 8;
             wg = turn / G * (8 * G) + xcd * G + turn % G;
         }
-        const int team = wg / a.vh, v = wg - team * a.vh;
-        const Run run = find_run<kMxStep>(a, team);
+        const int wgs = a.vh / HP, team = wg / wgs, v = wg - team * wgs;
+        const Run run = find_run<KS>(a, team);
         const bool notes = a.teams > 1 && v == 0 && threadIdx.x == 0; // who writes the cuts down
         if (run.u0 >= run.u1) { // the whole work-group
             if (notes && a.by_team) a.cut[team] = PagedCut{};
             return;
         }
-        const int nsub = a.hpg / a.hw, g = v / nsub;
-        const int h0 = g * a.hpg + (v - g * nsub) * a.hw;
+        const int nsub = a.hpg / a.hw, g0 = v / nsub * HP, sub = v % nsub;
         const int n = lane & 15, c = lane >> 4;
-        char *sk = lds[wv], *sv = sk + WB;
-        const int pc = lane % LPR, pr = lane / LPR;
+        // of column `col` of 16: the kv head, the query head's place in its group and among all
+        auto kv_of = [&](int col) { return g0 + (HP == 2 ? col >> 3 : 0); };
+        auto place_of = [](int col) { return HP == 2 ? col & 7 : col; };
+        auto head_of = [&](int col) { return kv_of(col) * a.hpg + sub * a.hw + place_of(col); };
+        // In LDS a step is 64 rows, a key's two heads one behind the other. A lane's values of it: (e, j), e the head
+        // (or 8 keys' half of 16), j the key, which are this row.
+        auto row_of = [](int cc, int e, int j) { return HP == 1 ? 16 * cc + 8 * e + j : 16 * cc + 2 * j + e; };
+        // A row's 16-byte pieces lie in turned order, so that 16 rows' reads of one piece meet no bank twice or, K's of
+        // a pair, few: rows with equal row % 4 differ in one of these.
+        auto turned = [](int row) { return LPR == 4 ? ((row >> 2) ^ (row >> 4)) & 3 : ((row >> 3) ^ (row >> 4)) & 1; };
+        const int pr = lane / LPR;
         const int64_t rowb = int64_t(a.nkv) * RB; // bytes between slots
-        const char *kg = static_cast<const char *>(a.kc) + int64_t(g) * RB;
-        const char *vg = static_cast<const char *>(a.vc) + int64_t(g) * RB;
-        const KV *ksg = reinterpret_cast<const KV *>(a.kd) + g, *vsg = reinterpret_cast<const KV *>(a.vd) + g;
-        const uint32_t lane_off = uint32_t(pr * rowb) + 16 * pc; // (checked on the host: below 2^32)
+        const uint8_t *kg = static_cast<const uint8_t *>(a.kc) + int64_t(g0) * RB;
+        const uint8_t *vg = static_cast<const uint8_t *>(a.vc) + int64_t(g0) * RB;
+        const int sg = (g0 + (HP == 2 ? lane & 1 : 0)) * KB; // of the lane's row's scales, from their slot's
+        // of load i's row `pr`: (row >> 4 is i more there, or the same)
+        const uint32_t lane_piece = 16 * ((lane % LPR) ^ turned(pr));
+        auto piece = [&](int i) { return LPR == 4 ? lane_piece ^ 16u * i : lane_piece; };
+        const uint32_t lane_row = uint32_t(pr / HP * rowb) + pr % HP * RB; // (checked on the host: below 2^32)
         const int cap = a.W << a.sh, psm = (1 << a.sh) - 1;
-        auto at_row = [](int row) { return row * SR + (row >> 4) * 64; };
+        // The scaling comes with the weights' exponent, as a positive number: a negative one turns the queries' signs, and
+        // at zero they are zeros (infinities and NaN stay, for their product with zero is NaN).
+        const float scale2 = a.scale2 == 0.0f ? 1.0f : __builtin_fabsf(a.scale2);
+        const uint32_t flip = a.scale2 < 0.0f ? 0x80008000u : 0u;
 
         // a part of a request in the run: units [at, end), attended keys [klo, khi), and the
         // units of the run behind it
@@ -98,7 +117,7 @@ namespace mg
             int b, at, end, units, k0, klo, khi, behind;
         };
         auto part_of = [&](int b, int at, int left) {
-            const PagedSpan sp = paged_span<kMxStep>(__builtin_amdgcn_readfirstlane(a.lens[b]), cap, a.window);
+            const PagedSpan sp = paged_span<KS>(uniform_load(a.lens + __builtin_amdgcn_readfirstlane(b)), cap, a.window);
             Part s;
             s.b = b;
             s.at = at;
@@ -113,70 +132,108 @@ namespace mg
         };
         Part cur = part_of(run.b, run.u0 - run.p, run.u1 - run.u0);
 
-        // the step whose table entries are read next: every wave takes a step of each part, which may be empty
+        // Steps are asked for in this order: their table entries four ahead, their rows and scales two ahead. All of that
+        // goes to LDS, so that the kernel alone counts what is under way: a wait in the middle for an older load would be
+        // a wait for the younger ones' rows, too.
         Part ahead = cur;
-        int akb = cur.k0 + kMxStep * wv;
+        int akb = cur.k0 + KS * wv;
         bool more_ahead = true;
-        auto advance = [&]() {
+        auto advance = [&]() { // every wave takes a step of each part, which may be empty
             akb += U;
             if (akb < ahead.khi) return;
             more_ahead = ahead.behind > 0;
             if (!more_ahead) return;
             ahead = part_of(ahead.b + 1, 0, ahead.behind);
-            akb = ahead.k0 + kMxStep * wv;
+            akb = ahead.k0 + KS * wv;
         };
-        // the slot of key akb + lane, or -1
-        auto slot_of = [&]() {
-            const int key = akb + lane;
-            if (!more_ahead || key < ahead.klo || key >= ahead.khi) return -1;
-            const int page = a.table[ahead.b * a.ldt + (key >> a.sh)];
-            return page >= 0 && page < a.num_pages ? (page << a.sh) + (key & psm) : -1;
+        struct Ask
+        {
+            int kb;
+            uint64_t rows; // those of attended keys
+            bool is;
         };
-        Vec<uint32_t, 4> stk[NLD], stv[NLD];
-        uint32_t ssk, ssv; // scales of key `lane`
-        auto stage = [&](int slot, uint64_t seen) {
-            ssk = ssv = 0;
-            if (slot >= 0) {
-                ssk = ksg[int64_t(slot) * a.nkv];
-                ssv = vsg[int64_t(slot) * a.nkv];
+        auto ask = [&](int par) { // the entries of step akb's keys, a row each
+            Ask s;
+            s.is = more_ahead;
+            s.kb = akb;
+            s.rows = 0;
+            const int32_t *p = a.lens;
+            if (more_ahead) {
+                const int key = akb + lane / HP;
+                s.rows = __builtin_amdgcn_ballot_w64(key >= ahead.klo && key < ahead.khi);
+                const int in = key < ahead.klo ? ahead.klo : key < ahead.khi ? key : ahead.khi - 1;
+                if (s.rows != 0) p = a.table + (ahead.b * a.ldt + (in >> a.sh));
+                advance();
             }
-            if (seen == ~uint64_t(0) && psm + 1 >= RPI) {
+            lds_load_at<4>(p, lds_address(reinterpret_cast<const char *>(entries[wv][par])));
+            return s;
+        };
+        Ask next0 = ask(0), next1 = ask(1);
+        // Asks for step next0's rows and scales, into the place `par`, and for the entries of the step two behind it.
+        // Returns the rows that are there; those that are not may stay what they were or be others: any finite codes.
+        bool full = false; // all OPS loads
+        auto stage = [&](int par) {
+            const int32_t entry = entries[wv][par][lane];
+            const bool there = (next0.rows >> lane & 1) != 0 && entry >= 0 && entry < a.num_pages;
+            const int slot = there ? (entry << a.sh) + ((next0.kb + lane / HP) & psm) : -1;
+            const uint64_t seen = __builtin_amdgcn_ballot_w64(there);
+            const uint32_t to = lds_address(lds[wv][par]);
+            full = seen != 0;
+            if (full) {
+                const int f = __builtin_ctzll(seen), first = __builtin_amdgcn_readlane(slot, f);
+                if ((psm + 1) * HP >= RPI) {
+                    // a load's keys lie in one page: from the first that is there (of the step, if the load has none)
 #pragma unroll
-                for (int i = 0; i < NLD; ++i) {
-                    int64_t o = __builtin_amdgcn_readlane(slot, RPI * i) * rowb;
-                    __asm__("" : "+s"(o)); // the rows' base stays in scalar registers, the lane's offset in one
-                    const char *kp = kg + o, *vp = vg + o;
-                    stk[i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(kp + lane_off));
-                    stv[i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(vp + lane_off));
-                }
-                return;
-            }
+                    for (int i = 0; i < NLD; ++i) {
+                        const uint64_t bits = seen >> (RPI * i) & ((uint64_t(1) << RPI) - 1);
+                        const int r = bits != 0 ? RPI * i + __builtin_ctzll(bits) : f;
+                        const int64_t o = (__builtin_amdgcn_readlane(slot, r) - r % RPI / HP) * rowb;
+                        const uint32_t off = lane_row + piece(i);
+                        lds_load(kg + o, off, to + 1024 * i);
+                        lds_load(vg + o, off, to + WB + 1024 * i);
+                    }
+                } else {
 #pragma unroll
-            for (int i = 0; i < NLD; ++i) {
-                const int s = __shfl(slot, pr + RPI * i, 64);
-                stk[i] = Vec<uint32_t, 4>{{0u, 0u, 0u, 0u}};
-                stv[i] = stk[i];
-                if (s >= 0) {
-                    const int64_t o = s * rowb + 16 * pc;
-                    stk[i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(kg + o));
-                    stv[i] = ld16_stream<uint32_t, 4>(reinterpret_cast<const uint32_t *>(vg + o));
+                    for (int i = 0; i < NLD; ++i) {
+                        int s = __shfl(slot, pr + RPI * i, 64);
+                        s = s >= 0 ? s : first;
+                        const int64_t o = s * rowb + (pr % HP * RB + piece(i));
+                        lds_load_at(kg + o, to + 1024 * i);
+                        lds_load_at(vg + o, to + WB + 1024 * i);
+                    }
                 }
+                const int64_t o = int64_t(there ? slot : first) * (a.nkv * KB) + sg;
+                const uint32_t ts = lds_address(reinterpret_cast<const char *>(scales[wv][par][0]));
+                lds_load_at<KB>(reinterpret_cast<const uint8_t *>(a.kd) + o, ts);
+                lds_load_at<KB>(reinterpret_cast<const uint8_t *>(a.vd) + o, ts + 256);
             }
+            __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // the entries are read
+            next0 = next1;
+            if (next0.is) next1 = ask(par);
+            else full = false;
+            return seen;
         };
-        int slot = slot_of();
-        uint64_t seen = __builtin_amdgcn_ballot_w64(slot >= 0); // keys of the staged step, one bit each
-        stage(slot, seen);
-        advance();
-        slot = slot_of();
+        __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        uint64_t now = stage(0), then = 0; // rows that are there, of the step that is next and of the one behind it
+        if (next0.is) then = stage(1);
+        else full = false;
 
         // B of S^T: lane (head n, c) holds q[n][c D / 4 + 8 i ..], zero for padding heads; f16 as two bf16 parts
         bf16x8 qop[QF16 ? 2 : 1][KW];
         auto load_q = [&](int b) {
 #pragma unroll
             for (int i = 0; i < KW; ++i) {
-                const uint16_t *qp = static_cast<const uint16_t *>(a.q) + b * a.ldq + int64_t(h0 + n) * D + c * (D / 4) + 8 * i;
+                const uint16_t *qp = static_cast<const uint16_t *>(a.q) + b * a.ldq + int64_t(head_of(n)) * D + c * (D / 4) + 8 * i;
                 Vec<uint32_t, 4> w{{0u, 0u, 0u, 0u}};
-                if (n < a.hw) w = *reinterpret_cast<const Vec<uint32_t, 4> *>(qp);
+                if (place_of(n) < a.hw) w = *reinterpret_cast<const Vec<uint32_t, 4> *>(qp);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) w.v[k] ^= flip;
+                if (a.scale2 == 0.0f) {
+                    constexpr uint32_t top = QF16 ? 0x7c00u : 0x7f80u; // the exponent of what is not finite
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        w.v[k] &= ((w.v[k] & top) == top ? 0xffffu : 0u) | ((w.v[k] >> 16 & top) == top ? 0xffff0000u : 0u);
+                }
                 if constexpr (QF16) {
                     Vec<uint32_t, 4> hi, lo;
 #pragma unroll
@@ -189,104 +246,146 @@ namespace mg
             }
         };
         load_q(cur.b);
+        int par = 0;
         for (;;) {
-            f32x4 o[NT];
+            f32x4 o[HP][NT];
 #pragma unroll
-            for (int t = 0; t < NT; ++t) o[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            float m = kLow, l = 0.0f; // head n (replicated over c)
-            bool any = false;         // the wave has seen a key that is not masked
-            int kb = cur.k0 + kMxStep * wv;
+            for (int e = 0; e < HP; ++e)
+#pragma unroll
+                for (int t = 0; t < NT; ++t) o[e][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            float m = kLow, l = 0.0f; // of head n (replicated over c)
+            bool any = false;   // the wave has seen a key that is not masked
+            uint32_t nan_v = 0; // V blocks that hold a NaN, a bit each, a head's eight
+            int kb = cur.k0 + KS * wv;
             bool more;
             do {
                 kb += U;
                 more = kb < cur.khi;
-                const uint64_t now = seen;
-                uint32_t ks[4]; // the scales of this lane's key of each tile
-                bool nan_v = false;
+                if (full)
+                    __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(OPS) : "memory"); // but for the next step's
+                else
+                    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                // the step's operands, all at once: its place takes another one's
+                Vec<uint32_t, KW> kw[4]; // row 4 a + b of tile 2 e + t is value (e, 4 t + b) of lanes c = a
+                float kf[4];             // the scales of this lane's row of each tile
+                Vec<uint32_t, 2> vx[NT];
+                bool raised = false;
                 if (now != 0) {
+                    const char *sk = lds[wv][par], *sv = sk + WB;
 #pragma unroll
-                    for (int i = 0; i < NLD; ++i) {
-                        const int row = at_row(pr + RPI * i);
-                        *reinterpret_cast<Vec<uint32_t, 4> *>(sk + row + 16 * pc) = stk[i];
-                        *reinterpret_cast<Vec<uint32_t, 4> *>(sv + row + 16 * pc) = stv[i];
+                    for (int t = 0; t < 4; ++t) {
+                        const int row = row_of(n >> 2, t >> 1, 4 * (t & 1) + (n & 3)), at = 4 * KW * c;
+                        kw[t] = *reinterpret_cast<const Vec<uint32_t, KW> *>(sk + row * RB + (at & 15) + ((at & ~15) ^ 16 * turned(row)));
+                        kf[t] = mx_scale(reinterpret_cast<const uint8_t *>(&scales[wv][par][0][row])[KB == 4 ? c : c >> 1]);
                     }
-                    bool bad = false;
+                    const int vrow = row_of(c, n >> 3, n & 7);
 #pragma unroll
-                    for (int i = 0; i < KB; ++i) {
-                        const uint32_t s = ssv >> (8 * i) & 0xffu;
-                        bad |= s == 255u;
-                        vsc[wv][i][lane] = s == 255u ? uint16_t(0x8000) : uint16_t((254u - s) << 7);
+                    for (int t = 0; t < NT; ++t)
+                        vx[t] = lds_read_tr4(sv + vrow * RB + 8 * (t & 1) + ((8 * (t & ~1)) ^ 16 * turned(vrow)));
+                    const uint32_t ssv = scales[wv][par][1][lane];
+                    // V blocks' scales; past 127 anywhere they are taken from 254 and the weights by 2^127 higher, and
+                    // a NaN is among those
+                    raised = (__builtin_amdgcn_ballot_w64((ssv & 0x80808080u) != 0) & now) != 0;
+                    const uint32_t from = raised ? 0x00fe00feu : 0x007f007fu;
+                    const int at = HP == 1 ? lane : (lane & 48) + 8 * (lane & 1) + (lane & 15) / 2;
+                    const uint32_t even = KB == 4 ? ssv & 0x00ff00ffu : (ssv & 0xffu) | (ssv & 0xff00u) << 8;
+                    const uint32_t d0 = pk_subsat_u16(from, even) << 7;
+                    vsc[wv][0][at] = uint16_t(d0);
+                    vsc[wv][KB / 2][at] = uint16_t(d0 >> 16);
+                    if constexpr (KB == 4) {
+                        const uint32_t d1 = pk_subsat_u16(from, ssv >> 8 & 0x00ff00ffu) << 7;
+                        vsc[wv][1][at] = uint16_t(d1);
+                        vsc[wv][3][at] = uint16_t(d1 >> 16);
                     }
-                    nan_v = __builtin_amdgcn_ballot_w64(bad) != 0;
+                    if (raised) {
 #pragma unroll
-                    for (int t = 0; t < 4; ++t)
-                        ks[t] = uint32_t(__shfl(int(ssk), 16 * (n >> 2) + 4 * t + (n & 3), 64)) >> (KB == 4 ? 8 * c : 8 * (c >> 1)) & 0xffu;
+                        for (int e = 0; e < HP; ++e) {
+                            const uint64_t of = HP == 1 ? now : now & (0x5555555555555555u << e);
+#pragma unroll
+                            for (int i = 0; i < KB; ++i)
+                                if ((__builtin_amdgcn_ballot_w64((ssv >> (8 * i) & 0xffu) == 255u) & of) != 0) nan_v |= 1u << (8 * e + i);
+                        }
+                    }
                     wave_lds_sync();
+                    __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // (loads into LDS keep no order with its reads)
                 }
-                // the next step's rows and the table entries of the one behind it are requested now
-                if (more_ahead) {
-                    seen = __builtin_amdgcn_ballot_w64(slot >= 0);
-                    stage(slot, seen);
-                    advance();
-                    slot = slot_of();
+                const uint64_t rows = now;
+                const int mine = par;
+                now = then;
+                then = 0;
+                par ^= 1;
+                if (more) { // (else its place takes the outputs first)
+                    full = false;
+                    if (next0.is) then = stage(mine);
                 }
-                if (now == 0) continue;
-                any = true;
-                // scores of keys 16 c + 4 t + r for head n
-                float sc[4][4], mx = kLow;
+                if (rows == 0) continue;
+                // scores of values (e, 4 t + r) for head n, without their scaling
+                f32x4 sc[4];
 #pragma unroll
-                for (int t = 0; t < 4; ++t) {
-                    const Vec<uint32_t, KW> kw =
-                        *reinterpret_cast<const Vec<uint32_t, KW> *>(sk + at_row(16 * (n >> 2) + 4 * t + (n & 3)) + 4 * KW * c);
-                    f32x4 st = {0.0f, 0.0f, 0.0f, 0.0f};
-                    const float f = mx_scale(ks[t]);
+                for (int t = 0; t < 4; ++t) sc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                    for (int i = 0; i < KW; ++i) {
-                        const bf16x8 k = __builtin_bit_cast(bf16x8, mx_bf16(kw.v[i], f));
-                        if constexpr (QF16) st = mfma_bf16(k, qop[1][i], st);
-                        st = mfma_bf16(k, qop[0][i], st);
+                for (int i = 0; i < KW; ++i)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        const bf16x8 k = __builtin_bit_cast(bf16x8, mx_bf16(kw[t].v[i], kf[t]));
+                        if constexpr (QF16) sc[t] = mfma_bf16(k, qop[1][i], sc[t]);
+                        sc[t] = mfma_bf16(k, qop[0][i], sc[t]);
                     }
+                // a pair's: lanes of columns below 8 take the first head's
+                float p[NV], mx = kLow;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) sc[t][r] = st[r] * a.scale2;
-                    if (now != ~uint64_t(0)) {
-                        const uint32_t bits = uint32_t(now >> (16 * c + 4 * t));
+                for (int i = 0; i < NV; ++i)
+                    p[i] = HP == 1 || n < 8 ? sc[i >> 2][i & 3] : sc[(2 + (i >> 2)) & 3][i & 3];
+                if (rows != ~uint64_t(0)) {
+                    const uint32_t bits = uint32_t(rows >> (16 * c)) & 0xffffu;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) sc[t][r] = (bits >> r & 1) != 0 ? sc[t][r] : kLow;
-                    }
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) mx = __builtin_fmaxf(mx, sc[t][r]);
+                    for (int i = 0; i < NV; ++i) p[i] = (bits >> (HP * i) & 1) != 0 ? p[i] : kLow;
                 }
+#pragma unroll
+                for (int i = 0; i < NV; ++i) mx = __builtin_fmaxf(mx, p[i]);
                 mx = rows4_max(mx);
-                const float mn = __builtin_fmaxf(m, mx);
+                // no less than any score times its scaling, unrounded
+                const float top = mx * scale2;
+                mx = mx == kLow ? kLow : __builtin_fmaf(__builtin_fabsf(top), 0x1p-23f, top);
+                // The reference moves when a score passes it by 8 (weights are then up to 2^8; to 1 where 2^127 is still to
+                // come), which most steps do not see.
+                const bool moves = mx > m + (raised ? 0.0f : 8.0f);
+                const float mn = moves ? mx : m;
                 // no score above -inf yet: a zero reference, so that -inf scores weigh 0
                 // and only NaN ones reach the sum
                 const float mref = mn == kLow ? 0.0f : mn;
-                // weights: element 4 t + r of lane (head n, c) is key 16 c + 4 t + r
-                float p[16];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) p[e] = __builtin_amdgcn_exp2f(sc[e >> 2][e & 3] - mref);
-                if (__builtin_amdgcn_ballot_w64(mn != m) != 0) {
-                    // some head's running max moved: rescale its sum and its O row
+                for (int i = 0; i < NV; ++i) p[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[i], scale2, -mref));
+                if (any && __builtin_amdgcn_ballot_w64(moves) != 0) {
+                    // some head's reference moved: rescale its sum and its O row
                     // (rows are heads 4c + r; their factors come from lanes 4c + r)
-                    const float corr = __builtin_amdgcn_exp2f(m - mref); // first step: 2^-inf = 0
+                    const float corr = __builtin_amdgcn_exp2f(m - mref); // from -inf: 0
                     l *= corr;
                     float cr[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) cr[r] = __shfl(corr, 4 * c + r, 64);
 #pragma unroll
-                    for (int t = 0; t < NT; ++t)
+                    for (int e = 0; e < HP; ++e)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) o[t][r] *= cr[r];
+                        for (int t = 0; t < NT; ++t)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) o[e][t][r] *= cr[r];
                 }
                 m = mn;
+                any = true;
 #pragma unroll
-                for (int e = 0; e < 16; e += 8)
-                    l += ((p[e] + p[e + 1]) + (p[e + 2] + p[e + 3])) + ((p[e + 4] + p[e + 5]) + (p[e + 6] + p[e + 7]));
-                // parts of 2^127 p, pairs of keys
-                uint32_t w[NP][8];
+                for (int i = 0; i < NV; i += 8)
+                    l += ((p[i] + p[i + 1]) + (p[i + 2] + p[i + 3])) + ((p[i + 4] + p[i + 5]) + (p[i + 6] + p[i + 7]));
+                if (raised) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float p0 = p[2 * i] * 0x1p127f, p1 = p[2 * i + 1] * 0x1p127f;
+                    for (int i = 0; i < NV; ++i) p[i] *= 0x1p127f;
+                    __asm__ volatile("" : "+v"(p[0])); // (a branch, not selections)
+                }
+                // parts of the weights, pairs of keys
+                uint32_t w[NP][NV / 2];
+#pragma unroll
+                for (int i = 0; i < NV / 2; ++i) {
+                    float p0 = p[2 * i], p1 = p[2 * i + 1];
 #pragma unroll
                     for (int k = 0; k < NP; ++k) {
                         w[k][i] = k + 1 < NP ? high_halves(p0, p1) : bf_pack(p0, p1);
@@ -294,34 +393,30 @@ namespace mg
                         p1 -= bf_hi(w[k][i]);
                     }
                 }
-                // V as B of P V: lane (dim n, c) needs keys 16 c .. + 15 of dim 16 s + n
-                const char *vr = sv + at_row(16 * c + n);
+                // V as B of P V: lane (dim n, c) has values (e, j) of dim 16 t + n. Of a pair, columns' weights meet both
+                // heads' values: rows of O below 8 count of the first head's, the others of the second's.
 #pragma unroll
                 for (int b = 0; b < KB; ++b) {
-                    Vec<uint32_t, 4> d[2];
-                    d[0] = *reinterpret_cast<const Vec<uint32_t, 4> *>(&vsc[wv][b][16 * c]);
-                    d[1] = *reinterpret_cast<const Vec<uint32_t, 4> *>(&vsc[wv][b][16 * c + 8]);
-                    Vec<uint32_t, 4> ws[NP][2];
+                    Vec<uint32_t, 4> ws[NP];
 #pragma unroll
-                    for (int k = 0; k < NP; ++k)
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) ws[k][i >> 2].v[i & 3] = pk_subsat_u16(w[k][i], d[i >> 2].v[i & 3]);
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const int t = 2 * b + u;
-                        const Vec<uint32_t, 2> x = lds_read_tr4(vr + 8 * t);
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            Vec<uint32_t, 4> vb = mx_bf16(x.v[h], 1.0f);
-                            if (nan_v) {
-#pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    if ((d[h].v[i] & 0x80008000u) != 0) vb.v[i] = 0x7fc07fc0u;
-                            }
+                    for (int e = 0; e < 2; ++e) {
+                        if (HP == 1 || e == 0) {
+                            const Vec<uint32_t, 4> d =
+                                *reinterpret_cast<const Vec<uint32_t, 4> *>(&vsc[wv][b][16 * c + 8 * (HP == 2 ? n >> 3 : e)]);
 #pragma unroll
                             for (int k = 0; k < NP; ++k)
-                                o[t] = mfma_bf16(__builtin_bit_cast(bf16x8, ws[k][h]), __builtin_bit_cast(bf16x8, vb), o[t]);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i)
+                                    ws[k].v[i] = pk_subsat_u16(w[k][HP == 1 ? 4 * e + i : i], d.v[i]);
                         }
+                        bf16x8 vb[2];
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) vb[u] = __builtin_bit_cast(bf16x8, mx_bf16(vx[2 * b + u].v[e], 1.0f));
+#pragma unroll
+                        for (int k = 0; k < NP; ++k)
+#pragma unroll
+                            for (int u = 0; u < 2; ++u)
+                                o[e % HP][2 * b + u] = mfma_bf16(__builtin_bit_cast(bf16x8, ws[k]), vb[u], o[e % HP][2 * b + u]);
                     }
                 }
                 wave_lds_sync(); // this step's reads are done before the next one's writes
@@ -334,63 +429,76 @@ namespace mg
                 load_q(next.b);
             }
 
-            // join the four waves: their outputs take the place of K and V in LDS
+            // join the four waves, 64 dims at a time, in the places of the steps they took last
+            const int mine = par ^ 1;
             l = rows4_sum(l);
-            float *so = reinterpret_cast<float *>(lds[wv]);
             // keys, but none above -inf: the sum, 0 (or NaN), says so by 1. Beside a maximum it weighs 0; where no
             // part has one the parts' sums are added as they are, and 0 means that nothing was attended.
             if (c == 0) {
                 wm[wv][n] = m;
                 wl[wv][n] = any && m == kLow ? l + 1.0f : l;
             }
+            if (lane == 0) place[wv] = uint32_t(2 * WB * mine);
+            if (nan_v != 0) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
+                for (int e = 0; e < HP; ++e)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) so[(4 * c + r) * SO4 + 16 * t + n] = o[t][r];
-            __syncthreads();
+                    for (int t = 0; t < NT; ++t)
+                        if ((nan_v >> (8 * e + t / 2) & 1) != 0)
+                            o[e][t] = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+            }
             const bool whole = cur.at == 0 && cur.end == cur.units;
             const int first = run.u1 - cur.behind - cur.end; // the request's first unit
             if (notes && leaves_cut(a.by_team, cur.at, cur.behind))
                 a.cut[a.by_team ? team : cur.b] =
                     cur.at == 0 ? paged_cut(run.d, team, cur.b, first, cur.units) : PagedCut{};
-            const int hh = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * (D / 16);
-            if (hh < a.hw) {
-                const float top = __builtin_fmaxf(__builtin_fmaxf(wm[0][hh], wm[1][hh]), __builtin_fmaxf(wm[2][hh], wm[3][hh]));
-                float sum = 0.0f, acc[D / 16];
+            const int hh = threadIdx.x >> 4, d0 = (threadIdx.x & 15) * 4;
+            float *so = reinterpret_cast<float *>(lds[wv][mine]);
 #pragma unroll
-                for (int e = 0; e < D / 16; ++e) acc[e] = 0.0f;
+            for (int part = 0; part < D / 64; ++part) {
+                if (part > 0) __syncthreads(); // those before are read
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const float f = weight_of(wm[w][hh], top);
-                    sum = __builtin_fmaf(f, wl[w][hh], sum);
-                    const float *src = reinterpret_cast<const float *>(lds[w]) + hh * SO4 + d0;
+                for (int t = 0; t < 4; ++t)
 #pragma unroll
-                    for (int e = 0; e < D / 16; e += 4) {
-                        const Vec<float, 4> x = *reinterpret_cast<const Vec<float, 4> *>(src + e);
+                    for (int r = 0; r < 4; ++r) // (rows 4 c + r, in turned order)
+                        so[(4 * c + r) * 64 + ((16 * t + n) ^ (16 * c))] =
+                            HP == 1 || c < 2 ? o[0][4 * part + t][r] : o[HP - 1][4 * part + t][r];
+                __syncthreads();
+                if (place_of(hh) < a.hw) {
+                    const float top = __builtin_fmaxf(__builtin_fmaxf(wm[0][hh], wm[1][hh]), __builtin_fmaxf(wm[2][hh], wm[3][hh]));
+                    float sum = 0.0f;
+                    Vec<float, 4> acc{{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) acc[e + i] = __builtin_fmaf(f, x.v[i], acc[e + i]);
+                    for (int w = 0; w < 4; ++w) {
+                        const float f = weight_of(wm[w][hh], top);
+                        sum = __builtin_fmaf(f, wl[w][hh], sum);
+                        const float *from = reinterpret_cast<const float *>(lds[w][0] + place[w]) + hh * 64 + (d0 ^ (16 * (hh >> 2)));
+                        const Vec<float, 4> x = *reinterpret_cast<const Vec<float, 4> *>(from);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) acc.v[i] = __builtin_fmaf(f, x.v[i], acc.v[i]);
                     }
-                }
-                if (whole) {
-                    const float inv = inverse(sum, top);
-                    raw *dst = static_cast<raw *>(a.out) + cur.b * a.ldo + int64_t(h0 + hh) * D + d0;
+                    const int d = 64 * part + d0;
+                    if (whole) {
+                        const float inv = inverse(sum, top);
+                        raw *dst = static_cast<raw *>(a.out) + cur.b * a.ldo + int64_t(head_of(hh)) * D + d;
 #pragma unroll
-                    for (int e = 0; e < D / 16; ++e) dst[e] = SO::enc32(acc[e] * inv);
-                } else {
-                    const int64_t row = (int64_t(team_place(run.d, team, first)) * a.vh + v) * a.hw + hh;
-                    float *dst = a.part + row * D + d0;
-#pragma unroll
-                    for (int e = 0; e < D / 16; e += 4)
-                        *reinterpret_cast<Vec<float, 4> *>(dst + e) = Vec<float, 4>{{acc[e], acc[e + 1], acc[e + 2], acc[e + 3]}};
-                    if (d0 == 0) {
-                        float *ml = a.part + 2 * int64_t(a.teams) * a.vh * a.hw * D + 2 * row;
-                        ml[0] = top;
-                        ml[1] = sum;
+                        for (int i = 0; i < 4; ++i) dst[i] = SO::enc32(acc.v[i] * inv);
+                    } else {
+                        const int vi = kv_of(hh) * nsub + sub;
+                        const int64_t row = (int64_t(team_place(run.d, team, first)) * a.vh + vi) * a.hw + place_of(hh);
+                        *reinterpret_cast<Vec<float, 4> *>(a.part + row * D + d) = acc;
+                        if (d == 0) {
+                            float *ml = a.part + 2 * int64_t(a.teams) * a.vh * a.hw * D + 2 * row;
+                            ml[0] = top;
+                            ml[1] = sum;
+                        }
                     }
                 }
             }
-            __syncthreads(); // the next part's first step writes where the outputs were
+            __syncthreads(); // the places are free
             if (!go_on) break;
+            full = false;
+            if (next0.is) then = stage(mine);
             cur = next;
         }
     }
@@ -406,20 +514,28 @@ namespace mg
         if (a.R == 0) return;
         need(ks && vs, "attn_decode_paged: MXFP4 pages need their scales");
         a.kd = reinterpret_cast<const uint16_t *>(ks), a.vd = reinterpret_cast<const uint16_t *>(vs);
-        paged_divide(c, a, D, 2, kMxStep);
+        // A pair of heads at a time, where their queries fit 16 columns: half the work a score takes, and lines of 128
+        // bytes where a head's row is 64 (40 / 8 heads, 64 ragged requests of up to 8000: 66 us, one at a time 76; 32 / 2
+        // heads in sets of their own 46, one at a time 42, five of 100003).
+        const bool pair = nkv % 2 == 0 && a.hw <= 8;
+        paged_divide(c, a, D, pair ? 4 : 2, pair ? 32 : 64);
         auto go = [&](auto kern) {
-            hipLaunchKernelGGL(kern, dim3(unsigned(a.teams * a.vh)), dim3(256), 0, c->stream, a);
+            hipLaunchKernelGGL(kern, dim3(unsigned(a.teams * (pair ? a.vh / 2 : a.vh))), dim3(256), 0, c->stream, a);
             check_launch("k_attn_mxfp4");
         };
-        auto sized = [&](auto s, auto so) {
+        auto sized = [&](auto s, auto so, auto kb) {
             using S = decltype(s);
             using SO = decltype(so);
-            D == 128 ? go(k_attn_mxfp4<S, SO, 4>) : go(k_attn_mxfp4<S, SO, 2>);
+            constexpr int KB = decltype(kb)::value;
+            pair ? go(k_attn_mxfp4<S, SO, KB, 2>) : go(k_attn_mxfp4<S, SO, KB, 1>);
+        };
+        auto with = [&](auto s, auto so) {
+            D == 128 ? sized(s, so, std::integral_constant<int, 4>{}) : sized(s, so, std::integral_constant<int, 2>{});
         };
         if (dt_out == F32)
-            dt == BF16 ? sized(SBf16{}, SF32{}) : sized(SF16{}, SF32{});
+            dt == BF16 ? with(SBf16{}, SF32{}) : with(SF16{}, SF32{});
         else
-            dt == BF16 ? sized(SBf16{}, SBf16{}) : sized(SF16{}, SF16{});
+            dt == BF16 ? with(SBf16{}, SBf16{}) : with(SF16{}, SF16{});
         paged_join(c, a, D, dt_out);
     }
 } // namespace mg

@@ -175,11 +175,17 @@ namespace mg
         else
             __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, %2" ::"s"(to), "v"(off), "s"(sb) : "memory");
     }
-    // the same from any address of each lane
-    MG_DEV void lds_load_at(const uint8_t *p, uint32_t to)
+    // the same from any address of each lane; 4 bytes, or two as a word, at `to` + 4 * lane
+    template <int BYTES = 16>
+    MG_DEV void lds_load_at(const void *p, uint32_t to)
     {
         to = uint32_t(__builtin_amdgcn_readfirstlane(int(to)));
-        __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(p) : "memory");
+        if constexpr (BYTES == 16)
+            __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(p) : "memory");
+        else if constexpr (BYTES == 4)
+            __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(to), "v"(p) : "memory");
+        else
+            __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ushort %1, off" ::"s"(to), "v"(p) : "memory");
     }
     MG_DEV uint32_t lds_address(const char *p) { return uint32_t(uintptr_t((__attribute__((address_space(3))) const char *)p)); }
 
