@@ -102,24 +102,23 @@ namespace mg
     }
 
     // ------------------------------------------- a wave by itself: 16-bit rows of up to four tokens, MXFP4 of up to 16
-    // A wave takes 16 weight rows in steps of 512 elements, 256 bytes a row (64 bytes of 16 rows an instruction: 19.3 us
-    // for 15 at [25600, 5120], one token), with its own ring of NB of them in LDS and no barrier. KS waves share
-    // a row's steps in turn and add their sums at the end.
-    template <class A, class SO, int XR, int KS, int NB, bool AL> // XR: token rows; AL: scales in whole 16s, aligned
-    __global__ __launch_bounds__(KS > 4 ? 64 * KS : 256) void k_mxfp4_gemv_wave(MxGemvArgs a)
+    // Bound by the weight's bytes. A wave takes 16 weight rows in steps of 512 elements, 256 bytes a row an instruction
+    // (64 bytes of 16 rows: 19.3 us for 16.4 at [25600, 5120], one token; that is 70 MB at 5.2 TB/s where they come from
+    // HBM in the run of a model, 13.5 us), with its own ring of two of them in LDS and no barrier. Four waves, a
+    // work-group, share a row's steps in turn and add their sums at the end.
+    template <class A, class SO, int XR, bool AL> // XR: token rows; AL: scales in whole 16s, aligned
+    __global__ __launch_bounds__(256) void k_mxfp4_gemv_wave(MxGemvArgs a)
     {
         constexpr bool MX = A::dt == kMxFp4;
-        constexpr int NW = KS > 4 ? KS : 4, NA = MX ? 1 : 4;
+        constexpr int KS = 4, NB = 2, NA = MX ? 1 : 4;
         constexpr int SS = AL ? 256 : 1024;               // scales of a step: 16 bytes a row, or each a word
         constexpr int XB = MX ? 4096 + SS : 1024 * XR;    // tokens
         constexpr int SB = 4096 + SS + XB;
         constexpr int LS = AL ? 1 : 4, L = 4 + LS + (MX ? 4 + LS : XR);
-        __shared__ __align__(16) char lds[NW][NB * SB];
+        __shared__ __align__(16) char lds[KS][NB * SB];
         const int wv = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)), lane = threadIdx.x & 63;
         const int n = lane & 15, c = lane >> 4;
-        const int kw = wv % KS;
-        const int64_t tile = int64_t(blockIdx.x) * (NW / KS) + wv / KS, t0 = int64_t(blockIdx.y) * XR;
-        const int64_t r0 = 16 * tile < a.rows ? 16 * tile : a.rows - 1; // (a wave past the last row reads it again)
+        const int64_t r0 = 16 * int64_t(blockIdx.x), t0 = int64_t(blockIdx.y) * XR;
         const int nblk = a.nblk, steps = a.steps;
         const uint32_t base = lds_address(lds[wv]);
         // Load j brings rows 4 j .. + 3, lane l piece (l % 16) ^ (row % 16) of row l / 16: reads of 16 rows' same piece hit
@@ -166,13 +165,13 @@ namespace mg
         f32x4 acc[1][1][NA];
 #pragma unroll
         for (int k = 0; k < NA; ++k) acc[0][0][k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        const int mine = steps > kw ? (steps - kw + KS - 1) / KS : 0; // steps kw, kw + KS ..
+        const int mine = steps > wv ? (steps - wv + KS - 1) / KS : 0; // steps wv, wv + KS ..
 #pragma unroll
         for (int p = 0; p < NB; ++p)
-            if (p < mine) load(kw + p * KS, p);
+            if (p < mine) load(wv + p * KS, p);
         int buf = 0;
         for (int k = 0; k < mine; ++k) {
-            const int m = kw + k * KS;
+            const int m = wv + k * KS;
             if (k + NB <= mine)
                 mx_wait<(NB - 1) * L>();
             else
@@ -227,14 +226,12 @@ namespace mg
         // lane (token n, c) holds rows 4 c .. 4 c + 3
         typename SO::raw *y = static_cast<typename SO::raw *>(a.y);
         f32x4 sum = mx_total(acc[0][0]);
-        if constexpr (KS > 1) {
-            *reinterpret_cast<f32x4 *>(lds[wv] + 16 * lane) = sum;
-            __syncthreads();
-            if (kw != 0) return;
+        *reinterpret_cast<f32x4 *>(lds[wv] + 16 * lane) = sum;
+        __syncthreads();
+        if (wv != 0) return;
 #pragma unroll
-            for (int k = 1; k < KS; ++k) sum += *reinterpret_cast<const f32x4 *>(lds[wv + k] + 16 * lane);
-        }
-        const int64_t tok = t0 + n, o = 16 * tile + 4 * c;
+        for (int k = 1; k < KS; ++k) sum += *reinterpret_cast<const f32x4 *>(lds[k] + 16 * lane);
+        const int64_t tok = t0 + n, o = r0 + 4 * c;
         if (n >= XR || tok >= a.T) return;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
@@ -242,20 +239,26 @@ namespace mg
     }
 
     // ------------------------------------------- a work-group for more tokens of 16 bits: they are shared by its waves
-    // NW waves of 16 RT rows each over 16 TT tokens; a ring of NB steps of 128 ES elements for all of them.
-    template <class A, class SO, int NW, int RT, int TT, int ES, int NB>
-    __global__ __launch_bounds__(64 * NW) void k_mxfp4_gemv(MxGemvArgs a)
+    // 128 rows over 16 TT tokens in a ring of three steps of 256 elements, loaded by all of eight waves; waves 2 g and
+    // 2 g + 1 take 32 rows, half of each step's elements each, and add at the end: a wave's reads of tokens, what bounds this
+    // kernel beside its waits at the barrier, then serve two tiles of rows ([25600, 5120] by 64, bf16: 40 us, eight waves of
+    // 16 rows and whole steps 48; by 8: 22.9 / 24.1, where the weight alone takes 10). Reading a step's operands beneath
+    // the products of the one before gains nothing (by 64: 49), nor do rings of two steps (by 5: 29.6) or four (22.7).
+    template <class A, class SO, int TT>
+    __global__ __launch_bounds__(512) void k_mxfp4_gemv(MxGemvArgs a)
     {
-        constexpr int NA = RT * TT <= 4 ? 4 : RT * TT <= 8 ? 2 : 1;
-        constexpr int BM = 16 * RT * NW, P = 4 * ES;             // pieces (blocks) of a weight row's step
+        constexpr int NW = 8, RT = 2, ES = 2, NB = 3;
+        constexpr int NA = TT == 1 ? 4 : TT == 2 ? 2 : 1;
+        constexpr int BM = 16 * NW, P = 4 * ES;                  // pieces (blocks) of a weight row's step
         constexpr int WB = BM * 16 * P, SCB = BM * 4 * P, XB = 16 * TT * 64 * P; // bytes of codes, scales (a word each), tokens
         constexpr int SB = WB + SCB + XB;
         constexpr int XL = (XB / 1024 + NW - 1) / NW;            // token loads a wave (the last ones may repeat)
-        constexpr int L = 2 * RT * ES + XL;
+        constexpr int L = 2 * ES + XL;
         __shared__ __align__(16) char lds[NB * SB];
         const int wv = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)), lane = threadIdx.x & 63;
         const int n = lane & 15, c = lane >> 4;
-        const int64_t r0 = int64_t(blockIdx.x) * BM + 16 * RT * wv; // the wave's rows
+        const int g = wv >> 1, half = wv & 1;
+        const int64_t r0 = int64_t(blockIdx.x) * BM + 16 * wv; // the rows it loads
         const int nblk = a.nblk;
         const int s0 = int(blockIdx.y) * a.splits, s1 = min(s0 + a.splits, a.steps);
         const uint32_t base = lds_address(lds);
@@ -266,19 +269,15 @@ namespace mg
         // all banks; of tokens 4 / ES, lane l piece (l % 4 P) ^ (token % 16). A block past the rows' ends is taken from their
         // last, and counts as zeros (below).
         auto f = [](int row) { return row >> 1 & 7; };
-        uint32_t off[RT * ES], soff[RT], xoff[XL];
-        int piece[RT * ES], xp[XL];
+        uint32_t off[ES], xoff[XL];
+        int piece[ES], xp[XL];
 #pragma unroll
-        for (int t = 0; t < RT * ES; ++t) {
+        for (int t = 0; t < ES; ++t) {
             const int lr = t * (64 / P) + lane / P, row = lr < last ? lr : int(last);
             piece[t] = lane % P ^ f(lr);
             off[t] = uint32_t(row) * (16u * uint32_t(nblk)) + 16u * uint32_t(piece[t]);
         }
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            const int row = 16 * t + n < last ? 16 * t + n : int(last);
-            soff[t] = uint32_t(row) * uint32_t(nblk) + uint32_t(c);
-        }
+        const uint32_t soff = uint32_t(n < last ? n : int(last)) * uint32_t(nblk) + uint32_t(c);
         const uint8_t *xb[XL];
         int xat[XL];
 #pragma unroll
@@ -296,19 +295,17 @@ namespace mg
             const int64_t at = int64_t(P) * m; // the step's first block
             const bool tail = P * m + P > nblk;
 #pragma unroll
-            for (int t = 0; t < RT * ES; ++t) {
+            for (int t = 0; t < ES; ++t) {
                 uint32_t o = off[t];
                 if (tail && P * m + piece[t] >= nblk) o -= 16u * uint32_t(P * m + piece[t] - nblk + 1);
-                lds_load(wb + 16 * at, o, to + 1024 * (RT * ES * wv + t));
+                lds_load(wb + 16 * at, o, to + 1024 * (ES * wv + t));
             }
 #pragma unroll
-            for (int t = 0; t < RT; ++t)
-#pragma unroll
-                for (int s = 0; s < ES; ++s) {
-                    uint32_t o = soff[t] + 4u * s;
-                    if (tail && P * m + 4 * s + c >= nblk) o -= uint32_t(P * m + 4 * s + c - nblk + 1);
-                    lds_load<1>(wsb + at, o, to + WB + 256 * (ES * (RT * wv + t) + s));
-                }
+            for (int s = 0; s < ES; ++s) {
+                uint32_t o = soff + 4u * s;
+                if (tail && P * m + 4 * s + c >= nblk) o -= uint32_t(P * m + 4 * s + c - nblk + 1);
+                lds_load<1>(wsb + at, o, to + WB + 256 * (ES * wv + s));
+            }
 #pragma unroll
             for (int u = 0; u < XL; ++u) {
                 uint32_t o = xoff[u];
@@ -323,27 +320,27 @@ namespace mg
             for (int u = 0; u < TT; ++u)
 #pragma unroll
                 for (int k = 0; k < NA; ++k) acc[t][u][k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        struct Part // a step's operands of 128 elements
+        struct Part // a half step's operands
         {
             Vec<uint32_t, 4> w[RT];
             uint32_t ws[RT];
             MxTok<A> x[TT];
         };
-        auto read = [&](Part &q, int buf, int s) {
+        auto read = [&](Part &q, int buf) {
             const char *b = lds + buf * SB;
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
-                q.w[t] = *reinterpret_cast<const Vec<uint32_t, 4> *>(b + 1024 * ES * (RT * wv + t) + 16 * P * n + 16 * ((4 * s + c) ^ f(n)));
-                q.ws[t] = *reinterpret_cast<const uint32_t *>(b + WB + 256 * (ES * (RT * wv + t) + s) + 4 * lane);
+                q.w[t] = *reinterpret_cast<const Vec<uint32_t, 4> *>(b + 1024 * ES * (RT * g + t) + 16 * P * n + 16 * ((4 * half + c) ^ f(n)));
+                q.ws[t] = *reinterpret_cast<const uint32_t *>(b + WB + 256 * (ES * (RT * g + t) + half) + 4 * lane);
             }
 #pragma unroll
             for (int u = 0; u < TT; ++u)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    q.x[u].v[i] = *reinterpret_cast<const Vec<uint32_t, 4> *>(b + WB + SCB + 64 * P * (16 * u + n) + 16 * ((16 * s + 4 * c + i) ^ n));
+                    q.x[u].v[i] = *reinterpret_cast<const Vec<uint32_t, 4> *>(b + WB + SCB + 64 * P * (16 * u + n) + 16 * ((16 * half + 4 * c + i) ^ n));
         };
-        auto products = [&](Part &q, int m, int s) {
-            if (P * m + P > nblk && P * m + 4 * s + c >= nblk) {
+        auto products = [&](Part &q, int m) {
+            if (P * m + P > nblk && P * m + 4 * half + c >= nblk) {
 #pragma unroll
                 for (int t = 0; t < RT; ++t) {
                     q.w[t] = Vec<uint32_t, 4>{{0u, 0u, 0u, 0u}};
@@ -369,24 +366,25 @@ namespace mg
 #pragma unroll
         for (int p = 0; p < NB - 1; ++p)
             if (s0 + p < s1) load(s0 + p, p);
-        Part q[2];
-        if (s0 < s1) {
-            arrive(s0);
-            read(q[0], 0, 0);
-        }
-        // a half's operands are read beneath the products of the one before
-        static_assert(ES == 2, "two halves");
         for (int m = s0; m < s1; ++m) {
-            read(q[1], buf, 1);
-            products(q[0], m, 0);
+            arrive(m);
+            Part q;
+            read(q, buf);
             buf = buf + 1 < NB ? buf + 1 : 0;
-            if (m + 1 < s1) {
-                arrive(m + 1);
-                read(q[0], buf, 0);
-            }
-            products(q[1], m, 1);
+            products(q, m);
         }
-        // lane (token n, c) holds rows 4 c .. 4 c + 3 of a tile
+        // lane (token n, c) holds rows 4 c .. 4 c + 3 of a tile; the second half's sums pass through LDS
+        __syncthreads();
+        f32x4 *sums = reinterpret_cast<f32x4 *>(lds) + RT * TT * 64 * g + lane;
+        static_assert(4 * RT * TT * 1024 <= NB * SB, "room for them");
+        if (half == 1) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int u = 0; u < TT; ++u) sums[64 * (TT * t + u)] = mx_total(acc[t][u]);
+        }
+        __syncthreads();
+        if (half == 1) return;
         typename SO::raw *y = static_cast<typename SO::raw *>(a.y) + blockIdx.y * a.ysplit;
 #pragma unroll
         for (int u = 0; u < TT; ++u) {
@@ -394,8 +392,8 @@ namespace mg
             if (tok >= a.T) continue;
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
-                const f32x4 s = mx_total(acc[t][u]);
-                const int64_t o = r0 + 16 * t + 4 * c;
+                const f32x4 s = mx_total(acc[t][u]) + sums[64 * (TT * t + u)];
+                const int64_t o = int64_t(blockIdx.x) * BM + 16 * (RT * g + t) + 4 * c;
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     if (o + r < a.rows) y[tok * a.ldy + o + r] = SO::enc32(s[r]);
@@ -405,8 +403,8 @@ namespace mg
 
     namespace
     {
-        // a wave a tile of 16 weight rows and XR tokens, four sharing its steps (of one token: two sharing 16.9 us, four
-        // 16.4, none 16.4 at [25600, 5120]; 20.2, 18.9 and 34.7 at [5120, 25600])
+        // (of one token: two waves sharing a row's steps 16.9 us, four 16.4, none 16.4 at [25600, 5120]; 20.2, 18.9 and 34.7
+        // at [5120, 25600])
         template <class A, class SO, int XR>
         void go_wave(mg_ctx *c, MxGemvArgs a)
         {
@@ -418,9 +416,9 @@ namespace mg
                 check_launch("k_mxfp4_gemv_wave");
             };
             if (a.nblk % 16 == 0 && aligned16(a.ws) && (A::dt != kMxFp4 || aligned16(a.xs)))
-                go(k_mxfp4_gemv_wave<A, SO, XR, 4, 2, true>);
+                go(k_mxfp4_gemv_wave<A, SO, XR, true>);
             else
-                go(k_mxfp4_gemv_wave<A, SO, XR, 4, 2, false>);
+                go(k_mxfp4_gemv_wave<A, SO, XR, false>);
         }
 
         // five to 64 tokens of 16 bits
@@ -430,8 +428,8 @@ namespace mg
             a.steps = (a.nblk + 7) / 8;
             const int64_t tiles = (a.rows + 127) / 128;
             need(tiles < (int64_t(1) << 31), "mxfp4 product: too many rows");
-            // parts of a row that fill the chip's CUs, of five steps at least ([6656, 19968] by 48: four 42 us, one 119; a
-            // second work-group a CU has to wait for its turn: [5120, 25600] by 64: six 58, eight 67)
+            // parts of a row that fill the chip's CUs, of five steps at least ([6656, 19968] by 48, f16: four 40 us, one 112;
+            // a second work-group a CU waits for its turn: nine 45; [5120, 25600] by 64: six 42, twelve 52)
             int64_t s = tiles < 256 ? 256 / tiles : 1;
             s = s < a.steps / 5 ? s : a.steps / 5;
             while (s > 1 && s * a.T * a.rows * 4 > c->work_bytes) --s;
@@ -446,20 +444,14 @@ namespace mg
             }
             auto tile = [&](auto so) {
                 using O = decltype(so);
-                auto go = [&](auto kern, int waves) {
-                    hipLaunchKernelGGL(kern, dim3(unsigned(tiles), unsigned(ns)), dim3(unsigned(64 * waves)), 0, c->stream, a);
+                auto go = [&](auto kern) {
+                    hipLaunchKernelGGL(kern, dim3(unsigned(tiles), unsigned(ns)), dim3(512), 0, c->stream, a);
                     check_launch("k_mxfp4_gemv");
                 };
-                if (a.T <= 16)
-                    go(k_mxfp4_gemv<A, O, 8, 1, 1, 2, 3>, 8);
-                else if (a.T <= 32)
-                    go(k_mxfp4_gemv<A, O, 8, 1, 2, 2, 3>, 8);
-                else if (a.T <= 48)
-                    go(k_mxfp4_gemv<A, O, 8, 1, 3, 2, 3>, 8);
-                else if constexpr (A::dt == F16) // (eight waves would spill: [25600, 5120] by 64 193 us for 56)
-                    go(k_mxfp4_gemv<A, O, 4, 2, 4, 2, 2>, 4);
+                if (a.T <= 32)
+                    a.T <= 16 ? go(k_mxfp4_gemv<A, O, 1>) : go(k_mxfp4_gemv<A, O, 2>);
                 else
-                    go(k_mxfp4_gemv<A, O, 8, 1, 4, 2, 3>, 8);
+                    a.T <= 48 ? go(k_mxfp4_gemv<A, O, 3>) : go(k_mxfp4_gemv<A, O, 4>);
             };
             if (ns > 1) {
                 tile(SF32{});
