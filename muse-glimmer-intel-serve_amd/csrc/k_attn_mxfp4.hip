@@ -3,23 +3,32 @@
 // and its join) where a key's row of a head is head_dim / 2 bytes of e2m1 codes
 // and head_dim / 32 bytes of powers of two.
 //
-// A wave takes steps of 64 keys, lane l the slot and the scales of key l; rows
-// come as there, in 16-byte pieces a step ahead, through LDS.
-//   S^T = K Q^T: 16 x 16 x 32 bf16 products, lane (key n, c) holding dims
-// c D/4 .. of its key, all of one block: codes become bf16 with that block's scale,
-// exactly, two an instruction. (bf16 holds every code at every scale; f16 queries
-// enter as the exact sum of two bf16 parts.) Row 4 a + b of tile t is key
-// 16 a + 4 t + b, so that lane (head n, c) ends with the scores of keys 16 c .. + 15.
-//   O += P V: a transposing 4-bit read gives lane (dim n, c) the codes of those
-// keys for one dim, a pair of keys a byte, so they become bf16 without a scale. A V
+// A wave takes steps of 64 rows: 64 keys of a head, or 32 keys of two heads that lie beside
+// each other. Rows, their scales and the table entries that lead to them are loaded
+// into LDS two steps ahead, counted by the kernel. (A step ahead through registers, with a
+// wait for table entries amid the rows on their way, took 88 us where this takes 66: 64
+// ragged requests of up to 8000 keys, 40 / 8 heads, 256 MB from HBM.)
+//   S^T = K Q^T: 16 x 16 x 32 bf16 products, lane (row n, c) holding dims c D/4 .. of
+// its row, all of one block: codes become bf16 with that block's scale, exactly, two an
+// instruction. (bf16 holds every code at every scale; f16 queries enter as the exact sum of
+// two bf16 parts.) Row 4 a + b of tiles is such that lane (query head n, c) ends with the
+// scores that O += P V wants of it, 16 keys'; of two heads with up to eight queries each,
+// columns below 8 are the first's, and a lane keeps its own head's eight scores of each:
+// exponentials and weights are then no more than a head's.
+//   O += P V: a transposing 4-bit read gives lane (dim n, c) the codes of 16 rows
+// for one dim, a pair of keys a byte, so they become bf16 without a scale. A V
 // block's scale goes to its weights: they are split into bf16 parts once, the
-// first by truncation, which keeps every part positive or zero, and each part takes
-// the power of two in its exponent field, for two keys at once by one saturating
-// subtraction of 254 - s from the field of 2^127 p. What falls below bf16's smallest
-// exponent becomes zero or less than 2^-126: weights times scales down to 2^-118 keep
-// 2^-16 of themselves. Block scales of 255 are looked for: the codes of such a pair
-// become NaN (0 of the other key's weight times NaN would be as wrong, but both are
-// attended, and the sums are NaN either way).
+// first by truncation, which keeps every part positive or zero (two parts for 16-bit
+// outputs, 2^-16 of a weight; three for f32), and each part takes the power of two in its
+// exponent field, for two keys at once by one saturating subtraction of 127 - s (254 -
+// s from the field of 2^127 p where an s is above 127). What falls below bf16's
+// smallest exponent becomes zero or less than 2^-126: weights times scales down to 2^-118
+// keep 2^-16 of themselves. V scales of 255 are looked for, and their blocks' outputs made NaN.
+//   A step of two heads is about 330 vector instructions and 48 products a wave; two waves
+// a SIMD (162 to 243 registers, 75 KB of LDS a work-group) are busy with them half of the
+// time, 6 TB/s in the run's middle. The rest is the start (sums of lengths, table, rows:
+// three trips to memory, 7 us for a single step), a last step shorter than others' and the
+// join's launch, 5 us.
 #include "mg_attn_paged.hpp"
 #include "mg_mxfp4.hpp"
 

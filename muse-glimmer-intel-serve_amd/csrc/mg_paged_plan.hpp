@@ -1,8 +1,9 @@
 // How decode attention over a paged cache divides its keys among work-groups:
 // plain arithmetic, the same on the host (its host test) and on the device.
 //
-// A request's attended keys [lo, n) are cut into units of 128 keys (256 of a
-// 4-bit cache) from `base`, lo rounded down to a step of 32 (64) (a request without keys has one empty unit,
+// A request's attended keys [lo, n) are cut into units of 128 keys (256 of an MXFP4
+// cache whose heads go one by one) from `base`, lo rounded down to a step of 32 (64)
+// (a request without keys has one empty unit,
 // so that somebody writes its zeros). The units of all requests form one line
 // of T; it is cut into `teams` equal runs, whatever requests they cross, and
 // each team has a work-group for every group of query heads. A request inside
