@@ -452,7 +452,10 @@ class Prims:
             if dim % 32 != 0:
                 raise MgError(f"{name}: MXFP4 pages hold rows of whole 32s, got head_dim {dim}")
             dim //= 2
-        if len(shape) != 4 or shape[3] != dim or heads is not None and shape[2] != heads:
+        if len(shape) != 4:
+            raise MgError(f"{name}: caches must be [num_pages, page_size, {heads or 'heads'}, {dim}], got {tuple(shape)}")
+        pages, page_size, held, width = shape
+        if width != dim or heads is not None and held != heads:
             raise MgError(f"{name}: caches must be [num_pages, page_size, {heads or 'heads'}, {dim}], got {tuple(shape)}")
         if v_cache.shape != shape:
             raise MgError(f"{name}: shape {tuple(shape)} and {tuple(v_cache.shape)} differ")
@@ -466,11 +469,11 @@ class Prims:
         if k_cache.dtype != want or v_cache.dtype != want:
             raise MgError(f"{name}: caches of {k_cache.dtype} and {v_cache.dtype}, {want} needed")
         if k_scale is not None:
-            want, kind = (*shape[:3], dim // (16 if mx else 32)), self._u8 if mx else self._f16
+            want, kind = (pages, page_size, held, dim // (16 if mx else 32)), self._u8 if mx else self._f16
             for t in (k_scale, v_scale):
                 if t.dtype != kind or t.shape != want or not t.is_contiguous():
                     raise MgError(f"{name}: scales must be contiguous {kind} {want}, got {t.dtype} {tuple(t.shape)}")
-        return shape[0], shape[1], shape[2], mx
+        return pages, page_size, held, mx
 
     def kv_pages(self, page_table, old_lens, new_lens, page_size, free_ring, ends, lens, ends_out, starts=None,
                  slot_map=None, positions=None):
@@ -606,11 +609,13 @@ class Prims:
     # two for every 32 of a row (e8m0)
     def _mx(self, name, qs, s):
         """(rows, in) of contiguous uint8 codes [rows, in / 2] and scales [rows, in / 32]"""
-        if qs.dtype != self._u8 or s.dtype != self._u8 or qs.dim() != 2 or s.dim() != 2:
+        shape, sshape = qs.shape, s.shape
+        if qs.dtype != self._u8 or s.dtype != self._u8 or len(shape) != 2 or len(sshape) != 2:
             raise MgError(f"{name}: codes and scales must be 2-d uint8, got {qs.dtype} {tuple(qs.shape)} and {s.dtype} "
                           f"{tuple(s.shape)}")
-        rows, n = qs.shape[0], 2 * qs.shape[1]
-        if n % 32 != 0 or tuple(s.shape) != (rows, n // 32):
+        rows, half = shape
+        n = 2 * half
+        if n % 32 != 0 or sshape != (rows, n // 32):
             raise MgError(f"{name}: codes {tuple(qs.shape)} need rows of whole 32s and scales {(rows, n // 32)}, got "
                           f"{tuple(s.shape)}")
         if not (qs.is_contiguous() and s.is_contiguous()):
