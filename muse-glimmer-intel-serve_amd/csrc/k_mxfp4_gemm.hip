@@ -4,15 +4,15 @@
 // A work-group of four waves takes a tile of BM weight rows and BN tokens; a wave
 // WM x WN of it, as 32 x 32 x 64 scaled products (v_mfma_scale_f32_32x32x64_f8f6f4:
 // lane 32 h + n holds block h of two, 16 bytes, of row n and its scale). Steps are of
-// 128 elements, 64 bytes a row, loaded straight into a ring of four buffers in LDS,
-// three steps ahead; the four steps of a round are one straight line of code, each product
-// followed by a load or an LDS read of the next ones (in runs of their own they cost
-// 387 us where this takes 355, [25600, 5120] by 4096 tokens). Results go out through LDS in
-// 16-byte pieces.
-//   At [25600, 5120] by 4096 (bf16 out) 320 us, 3.3 PFLOP/s, of which the products alone,
-// without what follows them, are 298: on random codes the matrix cores are held by power,
-// not by issue (8192^3: 3.8 PFLOP/s, zeros 5.6; from registers 6.2 and 9.0). A bf16 product
-// of 8192^3 by the library reaches 1.13 here.
+// 128 elements, loaded straight into LDS in pairs, 128 bytes a row an instruction (a step at a
+// time, 64 bytes a row, was bound by requests to the L2: [5120, 25600] by 333 tokens 50 us
+// for 44, [5120, 19968] by 4096 302 for 269), and read there one half ahead; the four steps of
+// a round are one straight line of code, each product followed by a load or an LDS
+// read of what comes next (in runs of their own they cost 387 us where this takes 355 at
+// [25600, 5120] by 4096). Results go out through LDS in 16-byte pieces.
+//   At [25600, 5120] by 4096 (bf16 out) 310 us, 3.5 PFLOP/s: on random codes the matrix
+// cores are held by power, not by issue (8192^3: 3.8 PFLOP/s, zeros 5.6; from registers
+// 6.2 and 9.0). A bf16 product of 8192^3 by the library reaches 1.13 here.
 #include "mg_device.hpp"
 #include "mg_internal.hpp"
 #include "mg_mxfp4.hpp"
@@ -73,15 +73,17 @@ namespace mg
 
     // TAIL: the last steps reach past the rows' ends. Blocks there take codes of block 0 and scales of 0 on both
     // sides: 2^-254 of a product of at most 36 is far below f32's smallest value, and adds nothing.
-    template <class SO, int BM, int BN, int WM, int WN, bool TAIL>
-    __global__ __launch_bounds__(256, BM * BN > 128 * 128 ? 1 : 2) void k_mxfp4_gemm(MxGemmArgs a)
+    // NB: steps in LDS.
+    template <class SO, int BM, int BN, int WM, int WN, int NB, bool TAIL>
+    __global__ __launch_bounds__(256, BM * BN * NB > 128 * 128 * 4 ? 1 : 2) void k_mxfp4_gemm(MxGemmArgs a)
     {
         static_assert((BM / WM) * (BN / WN) == 4, "four waves");
-        constexpr int NB = 4, R = BM + BN;   // buffers of a step; its rows
+        static_assert(NB == 4 || NB == 8, "a round of four steps in LDS, or two");
+        constexpr int R = BM + BN, NU = NB / 2, RP = 128; // a step's rows; pairs of steps in LDS; bytes of a pair's row
         constexpr int TM = WM / 32, TN = WN / 32;
-        constexpr int L = R / 64, LS = R / 256 > 0 ? R / 256 : 1; // loads a wave: of a step's codes, of four steps' scales
-        constexpr int CB = R * 64, SB = R * 16;
-        __shared__ __align__(16) char lds[NB * CB + 2 * SB];
+        constexpr int L = R / 32, LS = R / 256 > 0 ? R / 256 : 1; // loads a wave: of a pair's codes, of four steps' scales
+        constexpr int CB = R * RP, SB = R * 16;
+        __shared__ __align__(16) char lds[NU * CB + 2 * SB];
         const int wv = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)), lane = threadIdx.x & 63;
         const int split = blockIdx.y;
         int tm, tn;
@@ -92,16 +94,18 @@ namespace mg
         const int s0 = split * a.splits, s1 = min(s0 + a.splits, a.steps), S = s1 - s0;
         const uint32_t base = lds_address(lds);
         const uint32_t wbytes = 16u * uint32_t(a.nblk); // of a row
-        // A step's rows are the tile's weight rows, then its tokens; load j of wave w brings rows 16 (4 j + w) .. + 15,
-        // lane l piece (l % 4) ^ (row / 4 % 4) of row l / 4 (so that reads of 8 rows' same piece hit all banks)
+        // Rows are the tile's weight rows, then its tokens. Load j of wave w brings 128 bytes of rows 8 (4 j + w) .. + 7, lane
+        // l piece (l % 8) ^ turned(row) of row l / 8, so that reads of 16 rows' same piece hit all banks.
+        auto turned = [](int row) { return row >> 1 & 7; };
+        const int lp = lane % 8 ^ turned(8 * wv + lane / 8); // (32 j rows more turn it the same)
         uint32_t off[L], soff[LS];
 #pragma unroll
         for (int j = 0; j < L; ++j) {
-            const int r = 16 * (4 * j + wv) + (lane >> 2);
-            const bool isw = 16 * (4 * j + wv) < BM;
+            const int r = 8 * (4 * j + wv) + lane / 8;
+            const bool isw = 8 * (4 * j + wv) < BM;
             const int64_t last = isw ? a.rows - 1 - m0 : a.T - 1 - n0;
             const int rr = isw ? r : r - BM, row = rr < last ? rr : int(last);
-            off[j] = uint32_t(row) * wbytes + 16u * uint32_t((lane & 3) ^ (r >> 2 & 3));
+            off[j] = uint32_t(row) * wbytes + 16u * uint32_t(lp);
         }
 #pragma unroll
         for (int j = 0; j < LS; ++j) {
@@ -113,23 +117,22 @@ namespace mg
         }
         const uint8_t *wb = a.w + m0 * wbytes, *xb = a.x + n0 * wbytes;
         const uint8_t *wsb = a.ws + m0 * a.spitch, *xsb = a.xs + n0 * a.spitch;
-        auto load_codes = [&](int k, auto J) { // load j of step s0 + k
+        auto load_codes = [&](int u, auto J) { // load j of pair u, steps s0 + 2 u, + 1
             constexpr int j = decltype(J)::value;
-            const bool isw = 16 * (4 * j + wv) < BM;
-            const uint32_t to = base + (k % NB) * CB + 1024 * (4 * j + wv);
-            if constexpr (TAIL) {
-                const int piece = (lane & 3) ^ (lane >> 4 & 3), blk = 4 * (s0 + k) + piece; // (as in off[j])
-                lds_load(isw ? wb : xb, blk < a.nblk ? off[j] + 64u * uint32_t(s0 + k) : off[j] - 16u * uint32_t(piece), to);
-            } else {
-                lds_load((isw ? wb : xb) + 64 * int64_t(s0 + k), off[j], to);
-            }
+            const bool isw = 8 * (4 * j + wv) < BM;
+            const uint32_t to = base + (u % NU) * CB + 1024 * (4 * j + wv);
+            const int pair = s0 / 2 + u;
+            if constexpr (TAIL)
+                lds_load(isw ? wb : xb, 8 * pair + lp < a.nblk ? off[j] + uint32_t(RP) * uint32_t(pair) : off[j] - 16u * uint32_t(lp), to);
+            else
+                lds_load((isw ? wb : xb) + RP * int64_t(pair), off[j], to);
         };
         auto load_scales = [&](int g, auto J) { // load j of the scales of steps s0 + 4 g .. + 3
             constexpr int j = decltype(J)::value;
             const bool isw = 64 * (4 * j + wv) < BM;
-            lds_load((isw ? wsb : xsb) + 16 * (int64_t(s0 / 4) + g), soff[j], base + NB * CB + (g & 1) * SB + 1024 * (4 * j + wv));
+            lds_load((isw ? wsb : xsb) + 16 * (int64_t(s0 / 4) + g), soff[j], base + NU * CB + (g & 1) * SB + 1024 * (4 * j + wv));
         };
-        auto all_codes = [&](int k) { each<0, L>([&](auto J) { load_codes(k, J); }); };
+        auto all_codes = [&](int u) { each<0, L>([&](auto J) { load_codes(u, J); }); };
         auto all_scales = [&](int g) { each<0, LS>([&](auto J) { load_scales(g, J); }); };
         const int n = lane & 31, h = lane >> 5;
         const int wr = wv / (BN / WN) * WM, wc = wv % (BN / WN) * WN; // the wave's place in the tile
@@ -146,16 +149,18 @@ namespace mg
             uint32_t sa[TM], sb[TN];
         };
         // half s of a step: blocks 2 s + h; its scales come with the first, four to a word
-        const char *fa = lds + (wr + n) * 64, *fb = lds + (BM + wc + n) * 64;
-        const int piece[2] = {16 * (h ^ (n >> 2 & 3)), 16 * ((2 + h) ^ (n >> 2 & 3))};
-        auto read = [&](Frag &f, int buf, auto half, auto I) { // operand i of the wave's rows, then tokens
+        const char *fa = lds + (wr + n) * RP, *fb = lds + (BM + wc + n) * RP;
+        int pieces[4]; // of a pair's halves
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pieces[i] = 16 * ((2 * i + h) ^ turned(n));
+        auto read = [&](Frag &f, int pair, auto half, auto I) { // operand i of the wave's rows, then tokens
             constexpr int s = decltype(half)::value, i = decltype(I)::value;
             if constexpr (i < TM)
-                f.a[i] = *reinterpret_cast<const Vec<uint32_t, 4> *>(fa + buf * CB + piece[s] + 2048 * i);
+                f.a[i] = *reinterpret_cast<const Vec<uint32_t, 4> *>(fa + pair * CB + pieces[s] + 32 * RP * i);
             else
-                f.b[i - TM] = *reinterpret_cast<const Vec<uint32_t, 4> *>(fb + buf * CB + piece[s] + 2048 * (i - TM));
+                f.b[i - TM] = *reinterpret_cast<const Vec<uint32_t, 4> *>(fb + pair * CB + pieces[s] + 32 * RP * (i - TM));
         };
-        const char *ga = lds + NB * CB + 16 * (wr + n), *gb = lds + NB * CB + 16 * (BM + wc + n);
+        const char *ga = lds + NU * CB + 16 * (wr + n), *gb = lds + NU * CB + 16 * (BM + wc + n);
         auto read_scale = [&](Frag &f, int buf, int at, auto I) {
             constexpr int i = decltype(I)::value;
             if constexpr (i < TM)
@@ -177,28 +182,34 @@ namespace mg
                 __builtin_amdgcn_sched_barrier(0);
             });
         };
-        // Three steps' codes are in flight; scales of four steps come with the first of the four before (of the last
-        // four again, so that the counts hold). A step's arrival lies between the halves of the one before: its first
-        // half is read beneath those products, its second beneath its own first's.
-        all_scales(0);
-#pragma unroll
-        for (int p = 0; p < NB - 1; ++p) all_codes(p); // (S >= 4)
+        // A pair's buffer takes the pair NU behind it as soon as every wave has read its second step, whose second half
+        // is read beneath the products of its first; the next pair has to have landed there, too: the waves meet once a
+        // pair. Scales of four steps come with the fourth step of the round two before (of the last one again, so that
+        // the counts hold).
         const int last_g = S / 4 - 1;
-        Frag f0, f1;
-        if (last_g == 0)
-            wait_and_meet<0>();
-        else
-            wait_and_meet<2 * L>();
+        all_scales(0);
         all_scales(last_g > 0 ? 1 : 0);
-        all_codes(NB - 1);
-        static_assert(NB == 4, "a step's buffer is its place among four");
+        all_codes(0);
+        all_codes(1); // (S >= 4)
+        if (NU > 2 && last_g > 0) {
+            all_codes(2);
+            all_codes(3);
+            wait_and_meet<3 * L>();
+        } else {
+            wait_and_meet<L>();
+        }
+        Frag f0, f1;
         each<0, NR>([&](auto I) {
             read(f0, 0, H0{}, I);
             read_scale(f0, 0, 0, I);
         });
-        auto step = [&](int g, auto P, auto last) {
-            constexpr int p = decltype(P)::value;
-            constexpr bool end = decltype(last)::value;
+        // LEFT: rounds behind this one, two for any number
+        auto step = [&](int g, auto P, auto left) {
+            constexpr int p = decltype(P)::value, LEFT = decltype(left)::value;
+            constexpr bool loads = LEFT >= NB / 4, ends = p % 2 == 1; // a pair's second step
+            // the step's pair's place, and the next step's
+            const int pair = NB == 8 ? (g & 1) * 2 + p / 2 : p / 2;
+            const int next = p < 3 ? (NB == 8 ? (g & 1) * 2 : 0) + (p + 1) / 2 : NB == 8 ? (~g & 1) * 2 : 0;
             uint32_t sa[TM], sb[TN]; // the lane's blocks in bytes 0 and 2
 #pragma unroll
             for (int i = 0; i < TM; ++i) sa[i] = f0.sa[i] >> (8 * h);
@@ -210,37 +221,42 @@ namespace mg
                 if constexpr (m >= a && m < b) each<(m - a) * k / (b - a), (m - a + 1) * k / (b - a)>(item);
             };
             using Half = std::integral_constant<int, (NM + 1) / 2>;
-            using All = std::integral_constant<int, NM>;
             products(f0, sa, sb, H0{}, [&](auto M) {
-                spread(M, std::integral_constant<int, NR>{}, H0{}, Half{}, [&](auto I) { read(f1, p, H1{}, I); });
+                spread(M, std::integral_constant<int, NR>{}, H0{}, Half{},
+                       [&](auto I) { read(f1, pair, std::integral_constant<int, 2 * (p % 2) + 1>{}, I); });
             });
-            if constexpr (!end)
-                // (2 steps' loads behind those of the next step, and the scales where they came between)
-                wait_and_meet<2 * L + (p == 0 || p == 1 ? LS : 0)>();
-            else if constexpr (p < 3)
+            // the next pair has landed, but for those that were asked for behind it
+            if constexpr (ends && LEFT == 0 && p < 3)
                 wait_and_meet<0>();
+            else if constexpr (ends && LEFT > 0)
+                wait_and_meet<loads || p < 3 ? (NU - 2) * L : L>();
             products(f1, sa, sb, H1{}, [&](auto M) {
-                if constexpr (!end || p < 3)
+                if constexpr (p < 3 || LEFT > 0)
                     spread(M, std::integral_constant<int, NR>{}, H0{}, Half{}, [&](auto I) {
-                        read(f0, (p + 1) % 4, H0{}, I);
+                        read(f0, next, std::integral_constant<int, 2 * ((p + 1) % 2)>{}, I);
                         read_scale(f0, (g + (p == 3)) & 1, (p + 1) % 4, I);
                     });
-                if constexpr (!end) {
-                    // the buffer of this step, whose reads were done before the meeting
-                    if constexpr (p == 3)
-                        spread(M, std::integral_constant<int, LS>{}, H0{}, Half{}, [&](auto J) { load_scales(g + 2 < last_g ? g + 2 : last_g, J); });
-                    spread(M, std::integral_constant<int, L>{}, H0{}, All{}, [&](auto J) { load_codes(4 * g + p + NB, J); });
-                }
+                if constexpr (loads && p == 3 && decltype(M)::value == 0) all_scales(g + 2 < last_g ? g + 2 : last_g);
+                if constexpr (loads && ends)
+                    spread(M, std::integral_constant<int, L>{}, H0{}, Half{}, [&](auto J) { load_codes(2 * g + p / 2 + NU, J); });
             });
         };
-        auto four = [&](int g, auto last) {
-            step(g, std::integral_constant<int, 0>{}, last);
-            step(g, std::integral_constant<int, 1>{}, last);
-            step(g, std::integral_constant<int, 2>{}, last);
-            step(g, std::integral_constant<int, 3>{}, last);
+        auto four = [&](int g, auto left) {
+            step(g, std::integral_constant<int, 0>{}, left);
+            step(g, std::integral_constant<int, 1>{}, left);
+            step(g, std::integral_constant<int, 2>{}, left);
+            step(g, std::integral_constant<int, 3>{}, left);
         };
-        for (int g = 0; g < last_g; ++g) four(g, std::false_type{});
-        four(last_g, std::true_type{});
+        using R0 = std::integral_constant<int, 0>;
+        using R1 = std::integral_constant<int, 1>;
+        using R2 = std::integral_constant<int, 2>;
+        if constexpr (NB == 4) {
+            for (int g = 0; g < last_g; ++g) four(g, R1{});
+        } else {
+            for (int g = 0; g + 1 < last_g; ++g) four(g, R2{});
+            if (last_g > 0) four(last_g - 1, R1{});
+        }
+        four(last_g, R0{});
         // Lane (token n, h) holds rows 8 (e / 4) + 4 h + e % 4 of its column. 32 tokens at a time go through LDS, so
         // that a store instruction writes whole runs of a token's row.
         // (the sums are final here: without this the last products sink into the stores' branches, with copies and spills)
@@ -360,45 +376,56 @@ namespace mg
 
     namespace
     {
-        // How a product is divided: into 256 x 256 or 128 x 128 tiles, the sums into up to eight parts, whichever this
-        // estimate in us has soonest. Large tiles, one a CU, read half as much a product and take 0.66 us a step and 5 to
-        // start and end; of the small ones one alone on its CU takes 0.25 a step, and two share one at 0.68 for both and
-        // keep it busy through starts and ends; the parts' sums are written and read once more. Fitted to 121 products of
-        // 1024 to 19968 by 512 to 25600 weights and 8 to 4096 tokens in one, two, four or eight parts; what it picks takes
-        // 0.7% less than the best of those on average, 24% more at worst. ([25600, 5120] x 4096: large 347, small 450; x 200: 47 / 38;
-        // [25600, 1024] x 4096: 107 / 88; [5120, 19968] x 1024: two parts of large ones 93, one 126, small ones 118;
-        // x 64: small ones in four parts 25, in one 67.)
+        // How a product is divided: into 256 x 256 tiles, one a CU, or 128 x 128 ones, eight steps of one in LDS or four of
+        // each of two a CU, the sums into up to eight parts, whichever this estimate in us has soonest. Large tiles read
+        // half as much a product and take 0.78 us a step and 7 to start and end; of the small ones a deep one takes 0.26 a
+        // step and 2, two on a CU 0.57 for both, one's start and end beneath the other's steps; the parts' sums are written
+        // and read once more. Fitted to 77 products of 1024 to 19968 by 512 to 25600 weights and 129 to 4096 tokens; what
+        // it picks takes 1.2% more than the best of up to 11 tried there on average, 13% at worst. (Large, deep and two, the
+        // best parts of the first two: [25600, 5120] x 4096 313, 440, 380 us; x 200: 48, 38, 37; [25600, 1024] x
+        // 4096: 113, 134, 88; [5120, 5120] x 512: 35, 15, 17; x 4096: 88, 77, 68; [5120, 19968] x 1024: 88, 111, 105; x
+        // 200: 57, 31, 79.)
+        enum Tile
+        {
+            kLarge,
+            kDeep,
+            kTwo
+        };
         struct Tiling
         {
-            bool big;
+            Tile tile;
             int splits;
         };
         Tiling tiling(int64_t rows, int64_t T, int groups, int64_t room)
         {
             auto tiles = [&](int64_t b) { return ((rows + b - 1) / b) * ((T + b - 1) / b); };
-            Tiling best{false, 1};
+            Tiling best{kDeep, 1};
             float soonest = 0;
-            for (int big = 0; big < 2; ++big)
-                for (int s = 1; s <= (groups < 8 ? groups : 8); ++s) {
+            for (const Tile tile : {kDeep, kTwo, kLarge})
+                for (int s = 1; s <= (tile == kTwo ? 1 : groups < 8 ? groups : 8); ++s) {
                     const int64_t parts = int64_t(s) * T * rows * 4;
                     if (s > 1 && parts > room) break;
-                    const int64_t n = tiles(big ? 256 : 128) * s;
-                    const float steps = float((groups + s - 1) / s * 4), joined = s > 1 ? 3.f + float(parts) * (2 / 4.3e6f) : 0.f;
-                    const float t = joined + (big ? float((n + 255) / 256) * (0.66f * steps + 5.f)
-                                                  : n <= 256 ? 0.25f * steps
-                                                             : (n <= 512 ? 1.f : float(n) / 512) * (0.68f * steps + 0.3f));
-                    if ((big == 0 && s == 1) || t < soonest) {
+                    const int64_t n = tiles(tile == kLarge ? 256 : 128) * s, rounds = (n + 255) / 256;
+                    const float steps = float((groups + s - 1) / s * 4);
+                    float t = s > 1 ? 2.5f + float(parts) * (2 / 4.1e6f) : 0.f;
+                    if (tile == kLarge)
+                        t += float(rounds) * (0.78f * steps + 7.f);
+                    else if (tile == kDeep)
+                        t += float(rounds) * (0.26f * steps + 2.1f);
+                    else
+                        t += n <= 256 ? 0.33f * steps + 1.2f : (n <= 512 ? 1.f : float(n) / 512) * (0.57f * steps + 1.8f);
+                    if ((tile == kDeep && s == 1) || t < soonest) {
                         soonest = t;
-                        best = {big != 0, s};
+                        best = {tile, s};
                     }
                 }
             return best;
         }
 
         template <class SO>
-        void tiles_t(mg_ctx *c, MxGemmArgs a, bool big, int ns, bool tail)
+        void tiles_t(mg_ctx *c, MxGemmArgs a, Tile tile, int ns, bool tail)
         {
-            const int B = big ? 256 : 128;
+            const int B = tile == kLarge ? 256 : 128;
             const int64_t tm = (a.rows + B - 1) / B, tn = (a.T + B - 1) / B;
             need(tm * tn < (int64_t(1) << 31), "gemm_mxfp4: too many rows or tokens");
             a.tm = int(tm);
@@ -409,10 +436,14 @@ namespace mg
                 hipLaunchKernelGGL(kern, dim3(unsigned(tm * tn), unsigned(ns)), dim3(256), 0, c->stream, a);
                 check_launch("k_mxfp4_gemm");
             };
-            if (big)
-                tail ? go(k_mxfp4_gemm<SO, 256, 256, 128, 128, true>) : go(k_mxfp4_gemm<SO, 256, 256, 128, 128, false>);
-            else
-                tail ? go(k_mxfp4_gemm<SO, 128, 128, 64, 64, true>) : go(k_mxfp4_gemm<SO, 128, 128, 64, 64, false>);
+            auto of = [&](auto tail_) {
+                constexpr bool TAIL = decltype(tail_)::value;
+                if (tile == kLarge)
+                    go(k_mxfp4_gemm<SO, 256, 256, 128, 128, 4, TAIL>);
+                else
+                    tile == kDeep ? go(k_mxfp4_gemm<SO, 128, 128, 64, 64, 8, TAIL>) : go(k_mxfp4_gemm<SO, 128, 128, 64, 64, 4, TAIL>);
+            };
+            tail ? of(std::true_type{}) : of(std::false_type{});
         }
     }
 
@@ -443,15 +474,15 @@ namespace mg
         const int per = (groups + t.splits - 1) / t.splits, ns = (groups + per - 1) / per;
         a.splits = 4 * per;
         if (ns == 1) {
-            dt_out == F32 ? tiles_t<SF32>(c, a, t.big, 1, tail)
-                          : dt_out == BF16 ? tiles_t<SBf16>(c, a, t.big, 1, tail) : tiles_t<SF16>(c, a, t.big, 1, tail);
+            dt_out == F32 ? tiles_t<SF32>(c, a, t.tile, 1, tail)
+                          : dt_out == BF16 ? tiles_t<SBf16>(c, a, t.tile, 1, tail) : tiles_t<SF16>(c, a, t.tile, 1, tail);
             return true;
         }
         float *part = reinterpret_cast<float *>(work);
         a.y = part;
         a.ldy = rows;
         a.ysplit = tokens * rows;
-        tiles_t<SF32>(c, a, t.big, ns, tail);
+        tiles_t<SF32>(c, a, t.tile, ns, tail);
         join_splits(c, part, ns, y, ldy, rows, tokens, dt_out);
         return true;
     }

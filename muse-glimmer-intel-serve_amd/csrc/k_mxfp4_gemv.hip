@@ -506,8 +506,8 @@ namespace mg
         need(in == 0 || (aligned16(aq) && aligned16(qs)), "gemm_mxfp4: codes must be 16-byte aligned");
         need(in <= (int64_t(1) << 27), "gemm_mxfp4: input dim too large");
         // The waves' form reads the weight once for every 16 tokens and starts soonest: up to 16 tokens, and up to 128 where
-        // that is little to read, the tiles else ([5120, 5120] by 64: 10.8 us, tiles 12.6; by 128: 17.7 / 14.7;
-        // [1024, 19968] by 128: 11.8 / 15.9; [25600, 5120] by 17: 27 / 21; [25600, 1024] by 40: 17 / 7).
+        // that is little to read, the tiles else ([5120, 5120] by 64: 10.5 us, tiles 12.6; by 128: 17.7 / 14.0;
+        // [25600, 5120] by 17: 27 / 19; [25600, 1024] by 40: 17 / 7).
         const int64_t passes = (tokens + 15) / 16;
         const bool few = passes == 1 || (passes <= 8 && in >= 2048 && passes <= (int64_t(10) << 24) / (rows * in));
         if (!few && launch_mxfp4_tiles(c, aq, as, tokens, qs, s, rows, in, y, ldy, dt_out)) return;
