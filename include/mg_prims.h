@@ -366,8 +366,9 @@ int mg_dequant_mxfp4(mg_ctx *ctx, const uint8_t *qs, const uint8_t *scales, void
 /* y[b, o] = sum_i W[o, i] * x[b, i] for b < batch (1..64), W [rows, in] in MXFP4
  * (qs, scales), x [batch, in] at dtype MG_BF16 or MG_F16 (row stride ldx, 0 = in),
  * y at dtype_out, MG_F32 or dtype (row stride ldy, 0 = rows). Every product is of
- * the exact values; f32 sums, in an order that depends on batch and sizes: a row's
- * bits may differ between batches. qs and x 16-byte aligned, ldx % 8 == 0. (Longer
+ * the exact values; f32 sums, in an order that depends on batch and sizes (f16: on
+ * the scales of the 16 or 32 rows beside, too): a row's bits may differ between
+ * batches. qs and x 16-byte aligned, scales anywhere, ldx % 8 == 0. (Longer
  * batches: quantize the activations and call mg_gemm_mxfp4, or dequantize the
  * weight for a 16-bit product.) */
 int mg_gemv_mxfp4(mg_ctx *ctx, const uint8_t *qs, const uint8_t *scales, const void *x, int64_t batch, int64_t rows,
@@ -376,7 +377,8 @@ int mg_gemv_mxfp4(mg_ctx *ctx, const uint8_t *qs, const uint8_t *scales, const v
 /* y[t, o] = sum_i W[o, i] * A[t, i], both MXFP4: activations A [tokens, in] (a_qs,
  * a_scales), weight W [rows, in] (qs, scales) -> y [tokens, rows] at dtype_out
  * (MG_F32, MG_BF16 or MG_F16; row stride ldy, 0 = rows). Exact products, f32 sums in
- * an order that depends on the sizes, one rounding. a_qs and qs 16-byte aligned. */
+ * an order that depends on the sizes, one rounding. a_qs and qs 16-byte aligned. Both
+ * products may use the context's workspace, as much of it as there is. */
 int mg_gemm_mxfp4(mg_ctx *ctx, const uint8_t *a_qs, const uint8_t *a_scales, int64_t tokens, const uint8_t *qs,
                   const uint8_t *scales, int64_t rows, int64_t in, void *y, int64_t ldy, int dtype_out);
 

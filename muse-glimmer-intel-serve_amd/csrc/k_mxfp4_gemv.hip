@@ -408,17 +408,24 @@ namespace mg
         template <class A, class SO, int XR>
         void go_wave(mg_ctx *c, MxGemvArgs a)
         {
-            const int64_t tiles = (a.rows + 15) / 16, passes = (a.T + XR - 1) / XR;
-            need(tiles < (int64_t(1) << 31) && passes <= 65535, "mxfp4 product: too many rows or tokens");
+            const int64_t tiles = (a.rows + 15) / 16;
+            need(tiles < (int64_t(1) << 31), "mxfp4 product: too many rows");
             a.steps = (a.nblk + 15) / 16;
-            auto go = [&](auto kern) {
+            const bool aligned = a.nblk % 16 == 0 && aligned16(a.ws) && (A::dt != kMxFp4 || aligned16(a.xs));
+            auto go = [&](auto kern, int64_t passes) {
                 hipLaunchKernelGGL(kern, dim3(unsigned(tiles), unsigned(passes)), dim3(256), 0, c->stream, a);
                 check_launch("k_mxfp4_gemv_wave");
             };
-            if (a.nblk % 16 == 0 && aligned16(a.ws) && (A::dt != kMxFp4 || aligned16(a.xs)))
-                go(k_mxfp4_gemv_wave<A, SO, XR, true>);
-            else
-                go(k_mxfp4_gemv_wave<A, SO, XR, false>);
+            // (16-bit tokens are one pass)
+            for (const int64_t most = 65535 * XR; a.T > 0; a.T -= most) {
+                const int64_t passes = ((a.T < most ? a.T : most) + XR - 1) / XR;
+                aligned ? go(k_mxfp4_gemv_wave<A, SO, XR, true>, passes) : go(k_mxfp4_gemv_wave<A, SO, XR, false>, passes);
+                if constexpr (A::dt == kMxFp4) {
+                    a.x += most * 16 * a.nblk;
+                    a.xs += most * a.nblk;
+                    a.y = static_cast<typename SO::raw *>(a.y) + most * a.ldy;
+                }
+            }
         }
 
         // five to 64 tokens of 16 bits

@@ -135,6 +135,22 @@ def test_little_workspace(prims, room):
         p.close()
 
 
+def test_more_tokens_than_a_launch_takes():
+    """without room for laid-out scales, past 65535 passes of 16 tokens"""
+    import torch
+    import mgprims
+    T, rows, n = 65535 * 16 + 37, 3, 32
+    aq, as_, A = whole(13, T, n)
+    qs, s, W = whole(14, rows, n)
+    y = padded(T, rows, torch.float32)
+    p = mgprims.Prims(0, workspace_bytes=64)
+    try:
+        p.gemm_mxfp4(aq, as_, qs, s, y)
+        assert torch.equal(y.double(), A @ W.t().contiguous())
+    finally:
+        p.close()
+
+
 def test_values_of_all_sizes(prims):
     """real activations and weights against their kept values, in large tiles, in parts, and of 16 bits"""
     import torch
