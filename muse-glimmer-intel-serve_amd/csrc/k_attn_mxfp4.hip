@@ -24,7 +24,7 @@
 // s from the field of 2^127 p where an s is above 127). What falls below bf16's
 // smallest exponent becomes zero or less than 2^-126: weights times scales down to 2^-118
 // keep 2^-16 of themselves. V scales of 255 are looked for, and their blocks' outputs made NaN.
-//   A step of two heads is about 330 vector instructions and 48 products a wave; two waves
+//   A step of two heads is about 390 vector instructions and 48 products a wave; two waves
 // a SIMD (162 to 243 registers, 75 KB of LDS a work-group) are busy with them half of the
 // time, 6 TB/s in the run's middle. The rest is the start (sums of lengths, table, rows:
 // three trips to memory, 7 us for a single step), a last step shorter than others' and the
