@@ -161,7 +161,9 @@ namespace mg
     }
 
     // 64 lanes' 16 bytes (or one, as a word) from base + off, each lane its own, to LDS at `to` + 16 (or 4) * lane.
-    // (The compiler's own form would make every LDS read wait for all of them; here the kernel counts.)
+    // (The compiler's own form would make every LDS read wait for all of them; here the kernel counts.) A load may read
+    // scalar registers five wait states after a vector instruction wrote them, m0 one after a scalar one; the compiler
+    // does not look in here: the move of m0 is one and s_nop 3 four.
     template <int BYTES = 16>
     MG_DEV void lds_load(const uint8_t *base, uint32_t off, uint32_t to)
     {
@@ -171,9 +173,9 @@ namespace mg
                             uint32_t(__builtin_amdgcn_readfirstlane(int(uint32_t(b))));
         to = uint32_t(__builtin_amdgcn_readfirstlane(int(to)));
         if constexpr (BYTES == 16)
-            __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(sb) : "memory");
+            __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(sb) : "memory");
         else
-            __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, %2" ::"s"(to), "v"(off), "s"(sb) : "memory");
+            __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_ubyte %1, %2" ::"s"(to), "v"(off), "s"(sb) : "memory");
     }
     // the same from any address of each lane; 4 bytes, or two as a word, at `to` + 4 * lane
     template <int BYTES = 16>
