@@ -163,7 +163,9 @@ namespace mg
     // 64 lanes' 16 bytes (or one, as a word) from base + off, each lane its own, to LDS at `to` + 16 (or 4) * lane.
     // (The compiler's own form would make every LDS read wait for all of them; here the kernel counts.) A load may read
     // scalar registers five wait states after a vector instruction wrote them, m0 one after a scalar one; the compiler
-    // does not look in here: the move of m0 is one and s_nop 3 four.
+    // does not look in here: the move of m0 is one and s_nop 3 four. (m0 is reserved: it cannot be named as overwritten.
+    // The compiler writes it anew where it wants it, which it does nowhere in these kernels: the host test of the built
+    // code looks.)
     template <int BYTES = 16>
     MG_DEV void lds_load(const uint8_t *base, uint32_t off, uint32_t to)
     {
