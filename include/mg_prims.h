@@ -366,9 +366,10 @@ int mg_dequant_mxfp4(mg_ctx *ctx, const uint8_t *qs, const uint8_t *scales, void
 /* y[b, o] = sum_i W[o, i] * x[b, i] for b < batch (1..64), W [rows, in] in MXFP4
  * (qs, scales), x [batch, in] at dtype MG_BF16 or MG_F16 (row stride ldx, 0 = in),
  * y at dtype_out, MG_F32 or dtype (row stride ldy, 0 = rows). Every product is of
- * the exact values; f32 sums, in an order that depends on batch and sizes (f16: on
- * the scales of the 16 or 32 rows beside, too): a row's bits may differ between
- * batches. qs and x 16-byte aligned, scales anywhere, ldx % 8 == 0. (Longer
+ * the exact values; f32 sums, in an order that depends on batch and sizes (f16, and
+ * beside scales of 253 and 254: on those of the 16 or 32 rows beside, too): a row's bits
+ * may differ between batches. Sums below 2^-123 lose bits in rows beside a scale of 253 or
+ * 254 (f16: of 192 or more). qs and x 16-byte aligned, scales anywhere, ldx % 8 == 0. (Longer
  * batches: quantize the activations and call mg_gemm_mxfp4, or dequantize the
  * weight for a 16-bit product.) */
 int mg_gemv_mxfp4(mg_ctx *ctx, const uint8_t *qs, const uint8_t *scales, const void *x, int64_t batch, int64_t rows,

@@ -5,9 +5,9 @@
 // elements, its four scales beside), several steps ahead. Products are 16 x 16 (weight
 // rows x tokens): lane (n, c) holds block c of weight row n, 16 bytes, and of token n.
 // MXFP4 activations: one scaled product over 128. 16-bit ones: four over 32, the
-// codes become bf16 with their scale, exactly; beside f16 activations f16 where that
-// is exact too (scales of 2^-23 to 2^13, blocks of zeros, NaN), else the activations
-// are split into two bf16 parts.
+// codes become bf16 with their scale, exactly up to 2^125 (past that mx_far_sums takes
+// them); beside f16 activations f16 where that is exact too (scales of 2^-23 to 2^13,
+// blocks of zeros, NaN), else the activations are split into two bf16 parts.
 #include "mg_device.hpp"
 #include "mg_internal.hpp"
 #include "mg_mxfp4.hpp"
@@ -95,6 +95,82 @@ namespace mg
             return a[0];
     }
 
+    // Where weights pass bf16's largest value (scales of 253 and 254), or products with an f16 value's two bf16 parts may
+    // each pass f32's, so that what the two are together is lost (from 192 on: 6 2^63 by 2^16 is far from that for any
+    // number of them), the sums above are not these products'. A wave keeps the least of its scales less the first such
+    // (in the steps' loop a branch of its own took 20 % at one token), and then takes its sums anew.
+    template <class A>
+    MG_DEV uint32_t mx_past(uint32_t s)
+    {
+        return s - (A::dt == F16 ? 192u : 253u);
+    }
+    template <class A>
+    MG_DEV bool mx_any_past(uint32_t least) // (255 is NaN, whatever it meets)
+    {
+        return A::dt != kMxFp4 && __builtin_amdgcn_ballot_w64(least < (A::dt == F16 ? 63u : 2u)) != 0;
+    }
+    // The sums of RT tiles of 16 rows from row0 on with TT of 16 tokens from tok0 on, over the 128 elements of steps
+    // step(0), step(1) ..: weights less 2^2, f16 parts less 2^24, all exactly, the sums so far less both while a step is added
+    // (below 2^-123 they lose bits then). Straight from memory, for rows that are hardly ever there.
+    template <class A, int RT, int TT, class F>
+    MG_DEV void mx_far_sums(const MxGemvArgs &a, int64_t row0, int64_t tok0, int count, F step, f32x4 (&acc)[RT][TT])
+    {
+        constexpr float by = A::dt == F16 ? 0x1p-26f : 0x1p-2f;
+        const int lane = threadIdx.x & 63, n = lane & 15, c = lane >> 4;
+        auto times = [&](float f) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t)
+#pragma unroll
+                for (int u = 0; u < TT; ++u)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) acc[t][u][r] *= f;
+        };
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int u = 0; u < TT; ++u) acc[t][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = 0; k < count; ++k) {
+            const int64_t blk = 4 * int64_t(step(k)) + c;
+            const bool in = blk < a.nblk;
+            const Vec<uint32_t, 4> zero{{0u, 0u, 0u, 0u}};
+            Vec<uint32_t, 4> w[RT];
+            uint32_t ws[RT];
+#pragma unroll
+            for (int t = 0; t < RT; ++t) {
+                const int64_t r = row0 + 16 * t + n, row = r < a.rows ? r : a.rows - 1;
+                w[t] = zero;
+                ws[t] = 127u;
+                if (in) {
+                    w[t] = *reinterpret_cast<const Vec<uint32_t, 4> *>(a.w + 16 * (row * a.nblk + blk));
+                    ws[t] = a.ws[row * a.nblk + blk];
+                }
+            }
+            times(by);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                bf16x8 wb[RT];
+#pragma unroll
+                for (int t = 0; t < RT; ++t) wb[t] = __builtin_bit_cast(bf16x8, mx_bf16_quarter(w[t].v[i], ws[t]));
+#pragma unroll
+                for (int u = 0; u < TT; ++u) {
+                    const int64_t t0 = tok0 + 16 * u + n, tok = t0 < a.T ? t0 : a.T - 1;
+                    Vec<uint32_t, 4> hi = zero, lo = zero;
+                    if (in) hi = *reinterpret_cast<const Vec<uint32_t, 4> *>(a.x + 2 * (tok * a.ldx + 32 * blk + 8 * i));
+                    if constexpr (A::dt == F16) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) mx_halves(hi.v[e], hi.v[e], lo.v[e], 0x1p-24f);
+                    }
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) {
+                        if constexpr (A::dt == F16) acc[t][u] = mfma_bf16(wb[t], __builtin_bit_cast(bf16x8, lo), acc[t][u]);
+                        acc[t][u] = mfma_bf16(wb[t], __builtin_bit_cast(bf16x8, hi), acc[t][u]);
+                    }
+                }
+            }
+            times(1.0f / by);
+        }
+    }
+
     template <int N>
     MG_DEV void mx_wait() // all but the last N loads into LDS have landed
     {
@@ -165,6 +241,7 @@ namespace mg
         f32x4 acc[1][1][NA];
 #pragma unroll
         for (int k = 0; k < NA; ++k) acc[0][0][k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        uint32_t past = ~0u; // the least scale's place from where bf16 and f32 end
         const int mine = steps > wv ? (steps - wv + KS - 1) / KS : 0; // steps wv, wv + KS ..
 #pragma unroll
         for (int p = 0; p < NB; ++p)
@@ -220,12 +297,20 @@ namespace mg
 #pragma unroll
                     for (int i = 0; i < (MX ? 1 : 4); ++i) x[s][0].v[i] = Vec<uint32_t, 4>{{0u, 0u, 0u, 0u}};
                 }
+                if constexpr (!MX) past = min(past, mx_past<A>(ws[s][0]));
                 mx_step<A, 1, 1, NA>(w[s], ws[s], x[s], acc);
             }
         }
         // lane (token n, c) holds rows 4 c .. 4 c + 3
         typename SO::raw *y = static_cast<typename SO::raw *>(a.y);
         f32x4 sum = mx_total(acc[0][0]);
+        if constexpr (!MX) {
+            if (mx_any_past<A>(past)) {
+                f32x4 far[1][1];
+                mx_far_sums<A, 1, 1>(a, r0, t0, 4 * mine, [&](int k) { return 4 * (wv + KS * (k / 4)) + k % 4; }, far);
+                sum = far[0][0];
+            }
+        }
         *reinterpret_cast<f32x4 *>(lds[wv] + 16 * lane) = sum;
         __syncthreads();
         if (wv != 0) return;
@@ -339,6 +424,7 @@ namespace mg
                 for (int i = 0; i < 4; ++i)
                     q.x[u].v[i] = *reinterpret_cast<const Vec<uint32_t, 4> *>(b + WB + SCB + 64 * P * (16 * u + n) + 16 * ((16 * half + 4 * c + i) ^ n));
         };
+        uint32_t past = ~0u; // the least scale's place from where bf16 and f32 end
         auto products = [&](Part &q, int m) {
             if (P * m + P > nblk && P * m + 4 * half + c >= nblk) {
 #pragma unroll
@@ -351,6 +437,8 @@ namespace mg
 #pragma unroll
                     for (int i = 0; i < 4; ++i) q.x[u].v[i] = Vec<uint32_t, 4>{{0u, 0u, 0u, 0u}};
             }
+#pragma unroll
+            for (int t = 0; t < RT; ++t) past = min(past, mx_past<A>(q.ws[t]));
             mx_step<A, RT, TT, NA>(q.w, q.ws, q.x, acc);
         };
         int buf = 0, next = NB - 1; // of the step that arrives next, of the one to be loaded then
@@ -374,6 +462,13 @@ namespace mg
             products(q, m);
         }
         // lane (token n, c) holds rows 4 c .. 4 c + 3 of a tile; the second half's sums pass through LDS
+        f32x4 own[RT][TT];
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+#pragma unroll
+            for (int u = 0; u < TT; ++u) own[t][u] = mx_total(acc[t][u]);
+        if (mx_any_past<A>(past))
+            mx_far_sums<A, RT, TT>(a, int64_t(blockIdx.x) * BM + 16 * RT * g, 0, s1 - s0, [&](int k) { return 2 * (s0 + k) + half; }, own);
         __syncthreads();
         f32x4 *sums = reinterpret_cast<f32x4 *>(lds) + RT * TT * 64 * g + lane;
         static_assert(4 * RT * TT * 1024 <= NB * SB, "room for them");
@@ -381,7 +476,7 @@ namespace mg
 #pragma unroll
             for (int t = 0; t < RT; ++t)
 #pragma unroll
-                for (int u = 0; u < TT; ++u) sums[64 * (TT * t + u)] = mx_total(acc[t][u]);
+                for (int u = 0; u < TT; ++u) sums[64 * (TT * t + u)] = own[t][u];
         }
         __syncthreads();
         if (half == 1) return;
@@ -392,7 +487,7 @@ namespace mg
             if (tok >= a.T) continue;
 #pragma unroll
             for (int t = 0; t < RT; ++t) {
-                const f32x4 s = mx_total(acc[t][u]) + sums[64 * (TT * t + u)];
+                const f32x4 s = own[t][u] + sums[64 * (TT * t + u)];
                 const int64_t o = int64_t(blockIdx.x) * BM + 16 * (RT * g + t) + 4 * c;
 #pragma unroll
                 for (int r = 0; r < 4; ++r)

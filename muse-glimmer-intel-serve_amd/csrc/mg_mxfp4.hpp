@@ -111,10 +111,21 @@ namespace mg
                                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, f, 2)),
                                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, f, 3))}};
     }
-    // f16 pairs of a word as sums of two bf16 pairs: 11 bits are 8 and 3 (an infinity or a NaN is its high part)
-    MG_DEV void mx_halves(uint32_t w, uint32_t &hi, uint32_t &lo)
+    // The same less 2^2, exactly: 6 2^127 of scale 254 is past bf16's largest value. (What is left of the smallest scales' 2^-128
+    // is a subnormal that bf16 holds.)
+    MG_DEV Vec<uint32_t, 4> mx_bf16_quarter(uint32_t q, uint32_t s)
     {
-        const float a = f16_f32(uint16_t(w)), b = f16_f32(uint16_t(w >> 16));
+        Vec<uint32_t, 4> w = mx_bf16(q, mx_scale(s == 255u ? s : s > 2u ? s - 2u : 0u));
+        const float f = s == 0u ? 0.25f : s == 1u ? 0.5f : 1.0f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w.v[i] = bf_pack(bf_lo(w.v[i]) * f, bf_hi(w.v[i]) * f);
+        return w;
+    }
+    // f16 pairs of a word, times a power of two, as sums of two bf16 pairs: 11 bits are 8 and 3 (an infinity or a NaN is its
+    // high part)
+    MG_DEV void mx_halves(uint32_t w, uint32_t &hi, uint32_t &lo, float f = 1.0f)
+    {
+        const float a = f16_f32(uint16_t(w)) * f, b = f16_f32(uint16_t(w >> 16)) * f;
         hi = bf_pack(a, b);
         lo = bf_pack(__builtin_isfinite(a) ? a - bf_lo(hi) : 0.0f, __builtin_isfinite(b) ? b - bf_hi(hi) : 0.0f);
     }
