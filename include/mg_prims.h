@@ -397,7 +397,8 @@ int mg_qk_norm_rope_paged_mxfp4(mg_ctx *ctx, void *q, int64_t q_heads, int64_t l
  * all else as there, the scales 8-byte aligned. An attended block of scale 255 makes
  * the outputs it enters NaN (a key's: all of its request's for its query heads; a
  * value's: those of the block's 32 dims). Weights count with their V block's scale:
- * a product of the two keeps 2^-16 of itself down to 2^-118 and is lost below 2^-126. */
+ * a product of the two keeps 2^-16 of itself down to 2^-118 and is lost below 2^-126.
+ * Sums q . k below 2^-123 lose bits within 64 rows of a key with a scale of 192 or more. */
 int mg_attn_decode_paged_mxfp4(mg_ctx *ctx, const void *q, int64_t ldq, const uint8_t *k_cache, const uint8_t *v_cache,
                                const uint8_t *k_scale, const uint8_t *v_scale, const int32_t *page_table, int64_t ldt,
                                int64_t max_pages, const int32_t *lens, int64_t requests, int64_t q_heads,

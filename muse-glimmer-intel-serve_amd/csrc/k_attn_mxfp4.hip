@@ -10,9 +10,9 @@
 // ragged requests of up to 8000 keys, 40 / 8 heads, 256 MB from HBM.)
 //   S^T = K Q^T: 16 x 16 x 32 bf16 products, lane (row n, c) holding dims c D/4 .. of
 // its row, all of one block: codes become bf16 with that block's scale, exactly, two an
-// instruction. (bf16 holds every code at every scale; f16 queries enter as the exact sum of
-// two bf16 parts.) Row 4 a + b of tiles is such that lane (query head n, c) ends with the
-// scores that O += P V wants of it, 16 keys'; of two heads with up to eight queries each,
+// instruction. (bf16 holds every code up to scale 252, a quarter of it past that; f16
+// queries enter as the exact sum of two bf16 parts.) Row 4 a + b of tiles is such that lane
+// (query head n, c) ends with the scores that O += P V wants of it, 16 keys'; of two heads with up to eight queries each,
 // columns below 8 are the first's, and a lane keeps its own head's eight scores of each:
 // exponentials and weights are then no more than a head's.
 //   O += P V: a transposing 4-bit read gives lane (dim n, c) the codes of 16 rows
@@ -25,7 +25,7 @@
 // smallest exponent becomes zero or less than 2^-126: weights times scales down to 2^-118
 // keep 2^-16 of themselves. V scales of 255 are looked for, and their blocks' outputs made NaN.
 //   A step of two heads is about 390 vector instructions and 48 products a wave; two waves
-// a SIMD (162 to 243 registers, 75 KB of LDS a work-group) are busy with them half of the
+// a SIMD (153 to 253 registers, 75 KB of LDS a work-group) are busy with them half of the
 // time, 6 TB/s in the run's middle. The rest is the start (sums of lengths, table, rows:
 // three trips to memory, 7 us for a single step), a last step shorter than others' and the
 // join's launch, 5 us.
@@ -278,7 +278,7 @@ namespace mg
                 Vec<uint32_t, KW> kw[4]; // row 4 a + b of tile 2 e + t is value (e, 4 t + b) of lanes c = a
                 float kf[4];             // the scales of this lane's row of each tile
                 Vec<uint32_t, 2> vx[NT];
-                bool raised = false;
+                bool raised = false, past = false;
                 if (now != 0) {
                     const char *sk = lds[wv][par], *sv = sk + WB;
 #pragma unroll
@@ -291,10 +291,11 @@ namespace mg
 #pragma unroll
                     for (int t = 0; t < NT; ++t)
                         vx[t] = lds_read_tr4(sv + vrow * RB + 8 * (t & 1) + ((8 * (t & ~1)) ^ 16 * turned(vrow)));
-                    const uint32_t ssv = scales[wv][par][1][lane];
+                    const uint32_t ssk = scales[wv][par][0][lane], ssv = scales[wv][par][1][lane];
                     // V blocks' scales; past 127 anywhere they are taken from 254 and the weights by 2^127 higher, and
-                    // a NaN is among those
-                    raised = (__builtin_amdgcn_ballot_w64((ssv & 0x80808080u) != 0) & now) != 0;
+                    // a NaN is among those. So are K scales from 192 on, which want another way (below).
+                    const uint32_t far = ssk & ssk << 1;
+                    raised = (__builtin_amdgcn_ballot_w64(((ssv | far) & 0x80808080u) != 0) & now) != 0;
                     const uint32_t from = raised ? 0x00fe00feu : 0x007f007fu;
                     const int at = HP == 1 ? lane : (lane & 48) + 8 * (lane & 1) + (lane & 15) / 2;
                     const uint32_t even = KB == 4 ? ssv & 0x00ff00ffu : (ssv & 0xffu) | (ssv & 0xff00u) << 8;
@@ -307,6 +308,7 @@ namespace mg
                         vsc[wv][3][at] = uint16_t(d1 >> 16);
                     }
                     if (raised) {
+                        past = (__builtin_amdgcn_ballot_w64((far & 0x80808080u) != 0) & now) != 0;
 #pragma unroll
                         for (int e = 0; e < HP; ++e) {
                             const uint64_t of = HP == 1 ? now : now & (0x5555555555555555u << e);
@@ -342,10 +344,45 @@ namespace mg
                     }
                 // a pair's: lanes of columns below 8 take the first head's
                 float p[NV], mx = kLow;
+                auto pick = [&]() {
 #pragma unroll
-                for (int i = 0; i < NV; ++i)
-                    p[i] = HP == 1 || n < 8 ? sc[i >> 2][i & 3] : sc[(2 + (i >> 2)) & 3][i & 3];
-                if (rows != ~uint64_t(0)) {
+                    for (int i = 0; i < NV; ++i)
+                        p[i] = HP == 1 || n < 8 ? sc[i >> 2][i & 3] : sc[(2 + (i >> 2)) & 3][i & 3];
+                };
+                pick();
+                if (past || rows != ~uint64_t(0)) {
+                    if (past) {
+                        // Anew, with keys less 2^2, for scales of 253 and 254, and f16 queries' parts less 2^24, so that none
+                        // of their sums passes f32 (from 192 on they can, with either sign, which is NaN).
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) sc[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int i = 0; i < KW; ++i) {
+                            bf16x8 q[QF16 ? 2 : 1];
+#pragma unroll
+                            for (int h = 0; h < (QF16 ? 2 : 1); ++h) {
+                                Vec<uint32_t, 4> w = __builtin_bit_cast(Vec<uint32_t, 4>, qop[h][i]);
+#pragma unroll
+                                for (int e = 0; e < (QF16 ? 4 : 0); ++e) {
+                                    __asm__ volatile("" : "+v"(w.v[e])); // (not ahead of the steps' loop, where they would take registers)
+                                    w.v[e] = bf_pack(bf_lo(w.v[e]) * 0x1p-24f, bf_hi(w.v[e]) * 0x1p-24f);
+                                }
+                                q[h] = __builtin_bit_cast(bf16x8, w);
+                            }
+#pragma unroll
+                            for (int t = 0; t < 4; ++t) {
+                                const bf16x8 k =
+                                    __builtin_bit_cast(bf16x8, mx_bf16_quarter(kw[t].v[i], __builtin_bit_cast(uint32_t, kf[t]) >> 23));
+                                if constexpr (QF16) sc[t] = mfma_bf16(k, q[1], sc[t]);
+                                sc[t] = mfma_bf16(k, q[0], sc[t]);
+                            }
+                        }
+#pragma unroll
+                        for (int t = 0; t < 4; ++t)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) sc[t][r] *= QF16 ? 0x1p26f : 0x1p2f;
+                        pick();
+                    }
                     const uint32_t bits = uint32_t(rows >> (16 * c)) & 0xffffu;
 #pragma unroll
                     for (int i = 0; i < NV; ++i) p[i] = (bits >> (HP * i) & 1) != 0 ? p[i] : kLow;

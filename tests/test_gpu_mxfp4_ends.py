@@ -1,11 +1,13 @@
-"""GPU: MXFP4 products at the ends of the format's scales, where a code's value is
-a subnormal of bf16 (0 to 3) or passes it (253 and 254: 2^128 and above), against
-64-bit forms (tests/mxfp4_oracle.py)."""
+"""GPU: MXFP4 products and decode attention at the ends of the format's scales,
+where a code's value is a subnormal of bf16 (0 to 3) or passes it (253 and 254:
+2^128 and above), against 64-bit forms (tests/mxfp4_oracle.py): values as any other."""
 import numpy as np
 import pytest
 
 import mxfp4_oracle as MO
-from test_gpu_mxfp4 import dtypes, gemm, gemv, weight
+import paged_oracle as PO
+from test_gpu_mxfp4 import DEV, dtypes, gemm, gemv, u8, weight
+from test_gpu_mxfp4_paged import attend, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -84,3 +86,49 @@ def test_gemm_largest_scales(prims, T):
     got = gemm(prims, aq, as_, qs, s, "f32")
     ref, bound = MO.product(MO.values(qs, s), MO.values(aq, as_))
     assert np.isfinite(ref).all() and np.all(np.abs(got - ref) <= bound)
+
+
+@pytest.mark.parametrize("dtype", ("bf16", "f16"))
+@pytest.mark.parametrize("nq,nkv,D", ((4, 2, 64), (10, 2, 128), (12, 1, 128), (3, 1, 64)))
+@pytest.mark.parametrize("lo,hi", ((253, 255), (249, 255), (190, 194)))
+def test_scores_of_largest_scales(prims, dtype, nq, nkv, D, lo, hi):
+    """keys up to 6 2^127 beside ordinary, smallest and zero ones, queries and scaling such that scores stay within tens"""
+    R, ps, W = 3, 16, 20
+    lens = [300, 64, 1]
+    rng = np.random.default_rng(lo + nq)
+    kq = rng.integers(0, 256, (R * W, ps, nkv, D // 2), dtype=np.uint8)
+    ks = rng.integers(lo, hi, (R * W, ps, nkv, D // 32)).astype(np.uint8)
+    ks[::3, ::2] = rng.integers(100, 130, ks[::3, ::2].shape)
+    ks[1::4, 3, :, 0] = rng.integers(0, 3, ks[1::4, 3, :, 0].shape)
+    kq[2, 5] = 0x88
+    vq, vs = MO.quantize(rng.standard_normal((R * W, ps, nkv, D)))
+    q = normal(nq, (R, nq, D), 2.0**-15, dtype)
+    scaling = 2.0**(127 - hi + 15 - 3)
+    table = rng.permutation(R * W).reshape(R, W)
+    got = attend(prims, q.to(DEV), (u8(kq), u8(ks)), (u8(vq), u8(vs)), i32(table), i32(lens), scaling).double().cpu().numpy()
+    ref, bound = PO.attn_decode(q.double().numpy(), MO.values(kq, ks), MO.values(vq, vs), table, lens, ps, 0, scaling)
+    assert np.isfinite(ref).all() and np.all(np.abs(got - ref) <= bound), np.argwhere(~(np.abs(got - ref) <= bound))[:4].tolist()
+
+
+@pytest.mark.parametrize("dtype", ("bf16", "f16"))
+@pytest.mark.parametrize("nq,nkv", ((2, 1), (4, 2), (12, 1)))
+@pytest.mark.parametrize("size", (4.0, 60000.0))
+@pytest.mark.parametrize("s", (252, 254))
+def test_infinite_scores_of_either_type(prims, dtype, nq, nkv, size, s):
+    """a key of score -inf weighs nothing beside another, also where the queries' second parts have the other sign; such
+    keys alone give NaN; no key gives zeros"""
+    import torch
+    D, ps = 64, 16
+    rng = np.random.default_rng(3)
+    kq, ks = MO.quantize(rng.standard_normal((8, ps, nkv, D)) / size)
+    vq, vs = MO.quantize(rng.standard_normal((8, ps, nkv, D)))
+    kq[2, 3], ks[2, 3] = 0xff, s  # -6 2^(s - 127) in every dim: products' sums with q > 0 are past f32
+    kq[4], ks[4] = 0xff, s
+    q = (torch.rand((3, nq, D), generator=torch.Generator().manual_seed(4)) / 16 + 1).mul_(size).to(dtypes()[dtype])
+    pools = ((u8(kq), u8(ks)), (u8(vq), u8(vs)))
+    got = attend(prims, q.to(DEV), *pools, i32([[0, 1, 2, 3], [4, 4, 4, 4], [5, 6, 7, 0]]), i32([64, 40, 0]), 0.1)
+    assert torch.isnan(got[1]).all() and not got[2].any()
+    live = np.arange(64) != 35
+    K, V = (MO.values(a, b)[:4].reshape(64, 1, nkv, D)[live] for a, b in ((kq, ks), (vq, vs)))
+    ref, bound = PO.attn_decode(q[:1].double().numpy(), K, V, np.arange(63)[None], [63], 1, 0, 0.1)
+    assert np.all(np.abs(got[:1].double().cpu().numpy() - ref) <= bound)
