@@ -38,7 +38,7 @@ def test_what_parts_keep(parts, kept):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", ("bfloat16", "float16"))
 @pytest.mark.parametrize("nq,nkv,D", ((8, 2, 128), (8, 2, 64), (16, 1, 128), (4, 1, 64)))
-@pytest.mark.parametrize("lo,hi", ((110, 128), (100, 150)))
+@pytest.mark.parametrize("lo,hi", ((110, 128), (100, 150), (245, 253)))
 def test_f32_outputs(prims, dtype, nq, nkv, D, lo, hi):
     """(V scales past 127 take the weights' other way)"""
     import torch
