@@ -354,12 +354,14 @@ int mg_gemv_q8_0(mg_ctx *ctx, const int8_t *qs, const uint16_t *d, const uint16_
  * in) -> s = floor(log2 amax) - 2 + 127 within [0, 254] (amax 0: 0), codes the
  * nearest of x / 2^(s - 127), ties to the even code, past 6: 6 (an amax of 6 to 8
  * scales loses up to a quarter, the format's own rule). A block that holds an
- * infinity or a NaN: s = 255. x 16-byte, qs 4-byte aligned, ldx of whole 16 bytes. */
+ * infinity or a NaN: s = 255. x 16-byte, qs 4-byte aligned, ldx of whole 16 bytes.
+ * At most 2^36 - 2^12 elements. */
 int mg_quantize_mxfp4(mg_ctx *ctx, const void *x, int64_t ldx, int64_t rows, int64_t in, int dtype, uint8_t *qs,
                       uint8_t *scales);
 
 /* out [rows, in] = rnd(code * 2^(s - 127)) at dtype_out (MG_BF16, MG_F16 or MG_F32),
- * one rounding; a block of scale 255 gives NaN. out 16-byte, qs 4-byte aligned. */
+ * one rounding; a block of scale 255 gives NaN. out 16-byte, qs 4-byte aligned. At most
+ * 2^35 - 2^11 elements. */
 int mg_dequant_mxfp4(mg_ctx *ctx, const uint8_t *qs, const uint8_t *scales, void *out, int64_t rows, int64_t in,
                      int dtype_out);
 

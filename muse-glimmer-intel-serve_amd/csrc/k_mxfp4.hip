@@ -68,6 +68,7 @@ namespace mg
              "quantize_mxfp4: rows must be 16-byte and codes 4-byte aligned");
         need(rows <= (int64_t(1) << 38) / in, "quantize_mxfp4: tensor too large");
         const int64_t pieces = rows * (in / 8);
+        need(launchable((pieces + 511) / 512, 256), "quantize_mxfp4: tensor too large");
         auto go = [&](auto s_) {
             using S = decltype(s_);
             hipLaunchKernelGGL(k_quantize_mxfp4<S>, dim3(unsigned((pieces + 511) / 512)), dim3(256), 0, c->stream,
@@ -88,6 +89,7 @@ namespace mg
              "dequant_mxfp4: output must be 16-byte and codes 4-byte aligned");
         need(rows <= (int64_t(1) << 38) / in, "dequant_mxfp4: tensor too large");
         const int64_t pieces = rows * (in / 8);
+        need(launchable((pieces + 255) / 256, 256), "dequant_mxfp4: tensor too large");
         auto go = [&](auto so) {
             using SO = decltype(so);
             hipLaunchKernelGGL(k_dequant_mxfp4<SO>, dim3(unsigned((pieces + 255) / 256)), dim3(256), 0, c->stream,

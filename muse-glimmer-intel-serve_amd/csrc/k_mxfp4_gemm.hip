@@ -404,7 +404,7 @@ namespace mg
             for (const Tile tile : {kDeep, kTwo, kLarge})
                 for (int s = 1; s <= (tile == kTwo ? 1 : groups < 8 ? groups : 8); ++s) {
                     const int64_t parts = int64_t(s) * T * rows * 4;
-                    if (s > 1 && parts > room) break;
+                    if (s > 1 && (parts > room || !launchable((T * rows + 255) / 256, 256))) break; // (the join's)
                     const int64_t n = tiles(tile == kLarge ? 256 : 128) * s, rounds = (n + 255) / 256;
                     const float steps = float((groups + s - 1) / s * 4);
                     float t = s > 1 ? 2.5f + float(parts) * (2 / 4.1e6f) : 0.f;
@@ -427,7 +427,7 @@ namespace mg
         {
             const int B = tile == kLarge ? 256 : 128;
             const int64_t tm = (a.rows + B - 1) / B, tn = (a.T + B - 1) / B;
-            need(tm * tn < (int64_t(1) << 31), "gemm_mxfp4: too many rows or tokens");
+            need(launchable(tm * tn, 256), "gemm_mxfp4: too many rows or tokens");
             a.tm = int(tm);
             a.tn = int(tn);
             constexpr int64_t per = 16 / sizeof(typename SO::raw); // elements of a 16-byte store
@@ -461,7 +461,7 @@ namespace mg
             a.spitch = 16 * groups;
             const int64_t words = (rows + tokens) * (a.spitch / 4), blocks = (words + 255) / 256;
             const int64_t bytes = (4 * words + 255) / 256 * 256;
-            if (bytes > room || blocks >= (int64_t(1) << 31)) return false;
+            if (bytes > room || !launchable(blocks, 256)) return false;
             hipLaunchKernelGGL(k_mxfp4_scales, dim3(unsigned(blocks)), dim3(256), 0, c->stream, s, rows, as, rows + tokens, nblk,
                                a.spitch, reinterpret_cast<uint32_t *>(work));
             check_launch("k_mxfp4_scales");

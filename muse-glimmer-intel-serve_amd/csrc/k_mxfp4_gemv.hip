@@ -504,7 +504,7 @@ namespace mg
         void go_wave(mg_ctx *c, MxGemvArgs a)
         {
             const int64_t tiles = (a.rows + 15) / 16;
-            need(tiles < (int64_t(1) << 31), "mxfp4 product: too many rows");
+            need(launchable(tiles, 256), "mxfp4 product: too many rows");
             a.steps = (a.nblk + 15) / 16;
             const bool aligned = a.nblk % 16 == 0 && aligned16(a.ws) && (A::dt != kMxFp4 || aligned16(a.xs));
             auto go = [&](auto kern, int64_t passes) {
@@ -529,7 +529,7 @@ namespace mg
         {
             a.steps = (a.nblk + 7) / 8;
             const int64_t tiles = (a.rows + 127) / 128;
-            need(tiles < (int64_t(1) << 31), "mxfp4 product: too many rows");
+            need(launchable(tiles, 512), "mxfp4 product: too many rows");
             // parts of a row that fill the chip's CUs, of five steps at least ([6656, 19968] by 48, f16: four 40 us, one 112;
             // a second work-group a CU waits for its turn: nine 45; [5120, 25600] by 64: six 42, twelve 52)
             int64_t s = tiles < 256 ? 256 / tiles : 1;

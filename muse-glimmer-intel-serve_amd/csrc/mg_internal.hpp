@@ -33,6 +33,8 @@ namespace mg
         if (e != hipSuccess) fail(std::string(what) + ": " + hipGetErrorString(e));
     }
     inline void check_launch(const char *what) { check(hipGetLastError(), what); }
+    // whether a launch takes them: its threads along an axis are counted in 32 bits
+    inline bool launchable(int64_t groups, int threads) { return groups <= int64_t(0xffffffff) / threads; }
     inline bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
     using mgm::recip_rn; // RN(1 / c), mg_softcap_fast.hpp (shared with its host checker)
     inline int dt_size(int dt)

@@ -132,3 +132,24 @@ def test_infinite_scores_of_either_type(prims, dtype, nq, nkv, size, s):
     K, V = (MO.values(a, b)[:4].reshape(64, 1, nkv, D)[live] for a, b in ((kq, ks), (vq, vs)))
     ref, bound = PO.attn_decode(q[:1].double().numpy(), K, V, np.arange(63)[None], [63], 1, 0, 0.1)
     assert np.all(np.abs(got[:1].double().cpu().numpy() - ref) <= bound)
+
+
+def test_more_than_a_launch_takes(prims):
+    """threads past 2^32 along an axis are refused by name, before anything is launched"""
+    import torch
+    t = torch.zeros(4096, dtype=torch.uint8, device=DEV)
+    p, L, h, bf = t.data_ptr(), prims.lib, prims.h, 1
+
+    def refused(rc):
+        return rc == -1 and (b"too large" in L.mg_last_error() or b"too many" in L.mg_last_error())
+
+    for rows, n in ((2**31, 32), (2**26, 1024), (1, 2**36), (2**26 - 4, 1024 + 32)):
+        assert refused(L.mg_quantize_mxfp4(h, p, 0, rows, n, bf, p, p)), (rows, n)
+    for rows, n in ((2**30, 32), (2**25, 1024), (1, 2**35), (2**35 // 96 + 1, 96)):
+        assert refused(L.mg_dequant_mxfp4(h, p, p, p, rows, n, bf)), (rows, n)
+    for batch in (1, 3):
+        assert refused(L.mg_gemv_mxfp4(h, p, p, p, batch, 2**28, 32, 0, p, 0, bf, bf))
+    assert refused(L.mg_gemv_mxfp4(h, p, p, p, 64, 2**30, 32, 0, p, 0, bf, bf))
+    assert refused(L.mg_gemm_mxfp4(h, p, p, 5, p, p, 2**28, 32, p, 0, bf))
+    torch.cuda.synchronize()
+    assert not t.any()
