@@ -396,7 +396,7 @@ namespace mg
             Tile tile;
             int splits;
         };
-        Tiling tiling(int64_t rows, int64_t T, int groups, int64_t room)
+        Tiling tiling(int64_t rows, int64_t T, int groups, int64_t room, int64_t cus)
         {
             auto tiles = [&](int64_t b) { return ((rows + b - 1) / b) * ((T + b - 1) / b); };
             Tiling best{kDeep, 1};
@@ -405,7 +405,7 @@ namespace mg
                 for (int s = 1; s <= (tile == kTwo ? 1 : groups < 8 ? groups : 8); ++s) {
                     const int64_t parts = int64_t(s) * T * rows * 4;
                     if (s > 1 && (parts > room || !launchable((T * rows + 255) / 256, 256))) break; // (the join's)
-                    const int64_t n = tiles(tile == kLarge ? 256 : 128) * s, rounds = (n + 255) / 256;
+                    const int64_t n = tiles(tile == kLarge ? 256 : 128) * s, rounds = (n + cus - 1) / cus;
                     const float steps = float((groups + s - 1) / s * 4);
                     float t = s > 1 ? 2.5f + float(parts) * (2 / 4.1e6f) : 0.f;
                     if (tile == kLarge)
@@ -413,7 +413,7 @@ namespace mg
                     else if (tile == kDeep)
                         t += float(rounds) * (0.26f * steps + 2.1f);
                     else
-                        t += n <= 256 ? 0.33f * steps + 1.2f : (n <= 512 ? 1.f : float(n) / 512) * (0.57f * steps + 1.8f);
+                        t += n <= cus ? 0.33f * steps + 1.2f : (n <= 2 * cus ? 1.f : float(n) / float(2 * cus)) * (0.57f * steps + 1.8f);
                     if ((tile == kDeep && s == 1) || t < soonest) {
                         soonest = t;
                         best = {tile, s};
@@ -470,7 +470,7 @@ namespace mg
             work += bytes;
             room -= bytes;
         }
-        const Tiling t = tiling(rows, tokens, groups, room);
+        const Tiling t = tiling(rows, tokens, groups, room, c->num_cus);
         const int per = (groups + t.splits - 1) / t.splits, ns = (groups + per - 1) / per;
         a.splits = 4 * per;
         if (ns == 1) {

@@ -532,7 +532,7 @@ namespace mg
             need(launchable(tiles, 512), "mxfp4 product: too many rows");
             // parts of a row that fill the chip's CUs, of five steps at least ([6656, 19968] by 48, f16: four 40 us, one 112;
             // a second work-group a CU waits for its turn: nine 45; [5120, 25600] by 64: six 42, twelve 52)
-            int64_t s = tiles < 256 ? 256 / tiles : 1;
+            int64_t s = tiles < c->num_cus ? c->num_cus / tiles : 1;
             s = s < a.steps / 5 ? s : a.steps / 5;
             while (s > 1 && s * a.T * a.rows * 4 > c->work_bytes) --s;
             a.splits = s > 1 ? int((a.steps + s - 1) / s) : a.steps;
