@@ -665,9 +665,7 @@ namespace mg
 
     void paged_divide(mg_ctx *c, PagedArgs &a, int64_t D, int per_cu, int step)
     {
-        const int64_t tokens = int64_t(a.W) << a.sh, unit = 4 * step;
-        const int64_t span = a.window > 0 && a.window < tokens ? a.window + step : tokens;
-        const int64_t most = a.R * (span / unit + 1);
+        const int64_t most = a.R * paged_most_units(int64_t(a.W) << a.sh, a.window, step);
         need(most < (int64_t(1) << 31), "attn_decode_paged: the table must stand for fewer than 2^38 keys");
         // not more teams than there can be units, nor than the workspace has room for
         int64_t teams = per_cu * int64_t(c->num_cus) / a.vh;

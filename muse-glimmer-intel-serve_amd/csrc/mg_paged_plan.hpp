@@ -2,9 +2,9 @@
 // plain arithmetic, the same on the host (its host test) and on the device.
 //
 // A request's attended keys [lo, n) are cut into units of 128 keys (256 of an MXFP4
-// cache whose heads go one by one) from `base`, lo rounded down to a step of 32 (64)
-// (a request without keys has one empty unit,
-// so that somebody writes its zeros). The units of all requests form one line
+// cache whose heads go one by one) from `base`, lo rounded down to a step of 32 (64; a
+// request without keys has one empty unit, so that somebody writes its zeros). The
+// units of all requests form one line
 // of T; it is cut into `teams` equal runs, whatever requests they cross, and
 // each team has a work-group for every group of query heads. A request inside
 // one team is finished there; one that a team's edge cuts leaves a partial
@@ -42,6 +42,13 @@ namespace mg
         const int u = (s.n - s.base) / U + ((s.n - s.base) % U != 0);
         s.units = u > 0 ? u : 1;
         return s;
+    }
+
+    // units that a request can have at most, whatever its length (tokens, window >= 0)
+    MG_HD int64_t paged_most_units(int64_t tokens, int64_t window, int step)
+    {
+        const int64_t span = window > 0 && window < tokens ? window + step : tokens;
+        return span / (4 * step) + 1;
     }
 
     // The line's division among `teams` <= total teams: `per` units each, the first `rem` one more.
