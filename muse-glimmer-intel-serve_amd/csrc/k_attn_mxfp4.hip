@@ -101,8 +101,8 @@ namespace mg
         // In LDS a step is 64 rows, a key's two heads one behind the other. A lane's values of it: (e, j), e the head
         // (or 8 keys' half of 16), j the key, which are this row.
         auto row_of = [](int cc, int e, int j) { return HP == 1 ? 16 * cc + 8 * e + j : 16 * cc + 2 * j + e; };
-        // A row's 16-byte pieces lie in turned order, so that 16 rows' reads of one piece meet no bank twice or, K's of
-        // a pair, few: rows with equal row % 4 differ in one of these.
+        // A row's 16-byte pieces lie in turned order, so that 16 rows' reads of one piece meet fewer banks twice: rows with
+        // equal row % 4 differ in one of these. (A third of the LDS cycles are conflicts still, of a pair; 28 % of one head.)
         auto turned = [](int row) { return LPR == 4 ? ((row >> 2) ^ (row >> 4)) & 3 : ((row >> 3) ^ (row >> 4)) & 1; };
         const int pr = lane / LPR;
         const int64_t rowb = int64_t(a.nkv) * RB; // bytes between slots

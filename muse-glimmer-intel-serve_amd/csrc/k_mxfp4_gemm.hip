@@ -10,9 +10,15 @@
 // a round are one straight line of code, each product followed by a load or an LDS
 // read of what comes next (in runs of their own they cost 387 us where this takes 355 at
 // [25600, 5120] by 4096). Results go out through LDS in 16-byte pieces.
-//   At [25600, 5120] by 4096 (bf16 out) 310 us, 3.5 PFLOP/s: on random codes the matrix
-// cores are held by power, not by issue (8192^3: 3.8 PFLOP/s, zeros 5.6; from registers
-// 6.2 and 9.0). A bf16 product of 8192^3 by the library reaches 1.13 here.
+//   At [25600, 5120] by 4096 (bf16 out) 305-320 us, 3.4-3.5 PFLOP/s: 1600 tiles are 6.25
+// rounds of the CUs, paid as seven (15 % of the cycles a CU has none); 8192^3, four
+// rounds, reaches 3.8. What holds that is power (zeros 5.6; from registers 6.2 and 9.0)
+// and the reads from LDS: 39 % of its cycles are conflicts, by their counts those of the
+// scales, a word a row 16 bytes apart. A bf16 product of 8192^3 by the library
+// reaches 1.13 here. Rows that are not whole 512s are taken as if they were, their loads
+// checked one by one, after a launch that lays both operands' scales out, at every call:
+// [5120, 25632] by 333 64 us where 25600 takes 48, [5120, 5152] by 512 27 for 20, [25600,
+// 5152] by 4096 412 for 342 (weights in turn, from HBM).
 #include "mg_device.hpp"
 #include "mg_internal.hpp"
 #include "mg_mxfp4.hpp"
@@ -380,7 +386,7 @@ namespace mg
         // each of two a CU, the sums into up to eight parts, whichever this estimate in us has soonest. Large tiles read
         // half as much a product and take 0.78 us a step and 7 to start and end; of the small ones a deep one takes 0.26 a
         // step and 2, two on a CU 0.57 for both, one's start and end beneath the other's steps; the parts' sums are written
-        // and read once more. Fitted to 77 products of 1024 to 19968 by 512 to 25600 weights and 129 to 4096 tokens; what
+        // and read once more. Fitted to 77 products of 1024 to 19968 by 512 to 25600 weights, whole 512s, and 129 to 4096 tokens; what
         // it picks takes 1.2% more than the best of up to 11 tried there on average, 13% at worst. (Large, deep and two, the
         // best parts of the first two: [25600, 5120] x 4096 313, 440, 380 us; x 200: 48, 38, 37; [25600, 1024] x
         // 4096: 113, 134, 88; [5120, 5120] x 512: 35, 15, 17; x 4096: 88, 77, 68; [5120, 19968] x 1024: 88, 111, 105; x

@@ -1,9 +1,11 @@
 // Products of an MXFP4 weight with few tokens, for gfx950: y[t, o] = sum_i W[o, i]
 // x[t, i], x in 16 bits or in MXFP4 itself.
 //
-// The weight is read once, straight into LDS (64 bytes of a row and step of 128
-// elements, its four scales beside), several steps ahead. Products are 16 x 16 (weight
-// rows x tokens): lane (n, c) holds block c of weight row n, 16 bytes, and of token n.
+// Weights go straight into LDS, steps ahead: of 512 elements, a wave by itself in a
+// ring of two (up to four tokens of 16 bits, and MXFP4's, 16 a pass over the weight),
+// or of 256, shared by eight waves, in a ring of three (five to 64 tokens of 16 bits).
+// Products are 16 x 16 (weight rows x tokens) of 128 elements: lane (n, c) holds block c
+// of weight row n, 16 bytes, and of token n.
 // MXFP4 activations: one scaled product over 128. 16-bit ones: four over 32, the
 // codes become bf16 with their scale, exactly up to 2^125 (past that mx_far_sums takes
 // them); beside f16 activations f16 where that is exact too (scales of 2^-23 to 2^13,
@@ -20,7 +22,7 @@ namespace mg
         void *y;
         int64_t ldx, ldy, rows, T;
         int64_t ysplit;    // elements of y between splits' results
-        int nblk, steps;   // in / 32; steps of 128 elements
+        int nblk, steps;   // in / 32; the kernel's steps of a row (set by its launcher), of 512 or of 256 elements
         int splits;        // steps a split takes
     };
 
@@ -178,10 +180,12 @@ namespace mg
     }
 
     // ------------------------------------------- a wave by itself: 16-bit rows of up to four tokens, MXFP4 of up to 16
-    // Bound by the weight's bytes. A wave takes 16 weight rows in steps of 512 elements, 256 bytes a row an instruction
-    // (64 bytes of 16 rows: 19.3 us for 16.4 at [25600, 5120], one token; that is 70 MB at 5.2 TB/s where they come from
-    // HBM in the run of a model, 13.5 us), with its own ring of two of them in LDS and no barrier. Four waves, a
-    // work-group, share a row's steps in turn and add their sums at the end.
+    // A wave takes 16 weight rows in steps of 512 elements, 256 bytes a row an instruction (64 bytes of 16 rows: 19.3 us
+    // for 16.4 at [25600, 5120], one token), with its own ring of two of them in LDS and no barrier. Four waves, a
+    // work-group, share a row's steps in turn and add their sums at the end. That weight, 70 MB, from HBM, as in the run of a
+    // model (17 of them in turn): one token 17.0 us, 4.1 TB/s, four 19.6 (f16: 20.4 and 21.8); three in turn stay in the
+    // last cache, 14.0. Not bound by HBM, whose 9.9 it is far from: a ring starts empty for every 16 rows, and ten steps
+    // are shared as three, three, two and two.
     template <class A, class SO, int XR, bool AL> // XR: token rows; AL: scales in whole 16s, aligned
     __global__ __launch_bounds__(256) void k_mxfp4_gemv_wave(MxGemvArgs a)
     {
@@ -327,7 +331,7 @@ namespace mg
     // 128 rows over 16 TT tokens in a ring of three steps of 256 elements, loaded by all of eight waves; waves 2 g and
     // 2 g + 1 take 32 rows, half of each step's elements each, and add at the end: a wave's reads of tokens, what bounds this
     // kernel beside its waits at the barrier, then serve two tiles of rows ([25600, 5120] by 64, bf16: 40 us, eight waves of
-    // 16 rows and whole steps 48; by 8: 22.9 / 24.1, where the weight alone takes 10). Reading a step's operands beneath
+    // 16 rows and whole steps 48; by 8: 22.9 / 24.1, where the weight alone takes 10). Weights from HBM, 17 in turn: 40.7 by 64, 23.2 by 8. Reading a step's operands beneath
     // the products of the one before gains nothing (by 64: 49), nor do rings of two steps (by 5: 29.6) or four (22.7).
     template <class A, class SO, int TT>
     __global__ __launch_bounds__(512) void k_mxfp4_gemv(MxGemvArgs a)
@@ -351,8 +355,9 @@ namespace mg
         const int64_t first = r0 < a.rows ? r0 : a.rows - 1, last = a.rows - 1 - first;
         const uint8_t *wb = a.w + first * (16 * int64_t(nblk)), *wsb = a.ws + first * nblk;
         // A load brings 64 / P rows, lane l piece (l % P) ^ f(row) of its row, f so that reads of 16 rows' same piece hit
-        // all banks; of tokens 4 / ES, lane l piece (l % 4 P) ^ (token % 16). A block past the rows' ends is taken from their
-        // last, and counts as zeros (below).
+        // all banks; of tokens 4 / ES, lane l piece (l % 4 P) ^ (token % 16). (A read of tokens takes a lane's own c's piece,
+        // four pieces from the next c's: lanes whose tokens differ by four meet, four cycles a read, 44 % of the LDS cycles at
+        // [6656, 19968] by 48.) A block past the rows' ends is taken from their last, and counts as zeros (below).
         auto f = [](int row) { return row >> 1 & 7; };
         uint32_t off[ES], xoff[XL];
         int piece[ES], xp[XL];
@@ -580,7 +585,7 @@ namespace mg
         need(ldx < (int64_t(1) << 30), "gemv_mxfp4: leading dimension too large");
         need(in <= (int64_t(1) << 27), "gemv_mxfp4: input dim too large");
         const int nblk = int(in / 32);
-        const MxGemvArgs a{qs, s, static_cast<const uint8_t *>(x), nullptr, y, ldx, ldy, rows, batch, 0, nblk, (nblk + 3) / 4, 0};
+        const MxGemvArgs a{qs, s, static_cast<const uint8_t *>(x), nullptr, y, ldx, ldy, rows, batch, 0, nblk, 0, 0};
         auto go = [&](auto s_, auto so) {
             using S = decltype(s_);
             using SO = decltype(so);
@@ -614,7 +619,7 @@ namespace mg
         const bool few = passes == 1 || (passes <= 8 && in >= 2048 && passes <= (int64_t(10) << 24) / (rows * in));
         if (!few && launch_mxfp4_tiles(c, aq, as, tokens, qs, s, rows, in, y, ldy, dt_out)) return;
         const int nblk = int(in / 32);
-        const MxGemvArgs a{qs, s, aq, as, y, 0, ldy, rows, tokens, 0, nblk, (nblk + 3) / 4, 0};
+        const MxGemvArgs a{qs, s, aq, as, y, 0, ldy, rows, tokens, 0, nblk, 0, 0};
         if (dt_out == F32)
             go_wave<SMxFp4, SF32, 16>(c, a);
         else
